@@ -1,0 +1,289 @@
+// Attention over drafted trees and the paged cache (attention_tree.cuh says which keys a row sees) in 32-bit arithmetic, for float32 and
+// bfloat16, any head size up to 256, any page size and alignment.
+//
+// A CTA takes 64 rows (node, query head) of an entry and KV head and a part of the keys, 32 at a time, in shared memory as float32; 256
+// threads have 4 rows x 2 keys of the scores and 4 rows x (head size / 16) columns of the output each.  Sums, reference and exponents are
+// 32-bit, the reference is the running maximum.
+//
+// Which keys a row sees is decided by a select, never by adding: a hidden score may be anything.  A hidden value takes part as 0 * v, so
+// values that are not finite are put aside as zeros and added where they are seen.
+#include "attention_tree.cuh"
+
+namespace {
+
+using tree::Entry;
+using tree::Params;
+
+constexpr int ROWS = 64, KEYS = 32, THREADS = 256, STAGED_NODES = 1024;
+
+template <int DMAX>
+struct Layout {
+    static constexpr int LD = DMAX + 4;                              // floats of a row: eight rows' quads meet no bank twice
+    static constexpr int P_LD = KEYS + 4;
+    static constexpr int FLOATS = ROWS * LD + 2 * KEYS * LD + ROWS * P_LD;
+};
+
+template <typename T, int DMAX>
+__global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p) {
+    using L = Layout<DMAX>;
+    constexpr int COLS = DMAX / 64;                                  // quads of output columns a thread has
+    extern __shared__ __align__(16) float smem[];
+    float* const q_s = smem;
+    float* const k_s = q_s + ROWS * L::LD;
+    float* const v_s = k_s + KEYS * L::LD;
+    float* const p_s = v_s + KEYS * L::LD;
+    __shared__ int ups[STAGED_NODES];
+    __shared__ unsigned seen[ROWS];                                  // of a key tile, by row: a bit a key
+    __shared__ int lowest[ROWS];                                     // a row's first cached key
+    __shared__ long long key_row[KEYS];                              // where a key's row lies in the cache; -1: there is none
+    __shared__ unsigned keys_there;
+    __shared__ int place_entry, place_tile;
+    pdl_enter();
+    const int part = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
+    if (tid < 32) {
+        int entry, within;
+        tree::find_tile(p, blockIdx.z, ROWS, entry, within);
+        if (tid == 0) {
+            place_entry = entry;
+            place_tile = within;
+        }
+    }
+    __syncthreads();
+    if (place_entry < 0) return;
+    const int r = place_entry, group = p.num_heads / p.num_kv_heads;
+    const Entry e = tree::entry_of(p, r);
+    if (e.n == 0) return;
+    const int D = p.head_dim, row0 = place_tile * ROWS, count = min(ROWS, e.n * group - row0);
+    const int last_node = (row0 + count - 1) / group;
+    const int first = tree::first_key(p, e), end = e.context + last_node + 1;    // the tile's keys: first .. end - 1
+    const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
+    if (part >= parts) return;
+    const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
+
+    // ---- the tree: parents of the nodes up to the tile's last one, and every row's first cached key
+    for (int i = tid; i <= last_node && i < STAGED_NODES; i += THREADS) ups[i] = tree::parent_of(p, e, i);
+    __syncthreads();
+    auto up_of = [&](int i) { return i < STAGED_NODES ? ups[i] : tree::parent_of(p, e, i); };
+    if (tid < ROWS) {
+        int low = 0;
+        if (p.window > 0 && tid < count) {
+            int depth = 0;
+            for (int i = up_of((row0 + tid) / group); i >= 0; i = up_of(i)) ++depth;
+            low = max(0ll, (long long)e.context + depth - p.window + 1);
+        }
+        lowest[tid] = low;
+    }
+    // ---- the rows of q
+    for (int i = tid; i < ROWS * DMAX; i += THREADS) {
+        const int row = i / DMAX, d = i % DMAX;
+        float x = 0.f;
+        if (row < count && d < D) {
+            const int node = (row0 + row) / group, head = kvh * group + (row0 + row) % group;
+            x = to_f32<T>(static_cast<const T*>(p.q)[(size_t)(e.first + node) * p.ldq + (size_t)head * D + d]);
+        }
+        q_s[row * L::LD + d] = x;
+    }
+    const int tx = tid & 15, ty = tid >> 4;                          // keys tx, tx + 16; rows 4 ty ..; columns 4 tx + 64 c ..
+    const float scale_log2 = p.scale * 1.4426950408889634f;
+    float m[4], l[4], acc[4][COLS][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
+    }
+    for (int tile = begin; tile < stop; ++tile) {
+        const int key0 = tile * KEYS;
+        __syncthreads();                                             // the last tile has been read
+        if (tid < KEYS) {
+            const int at = key0 + tid, slot = at / p.page_size;
+            long long row = -1;
+            if (at >= first && at < end) {
+                const int page = slot < p.table_pages ? p.block_table[(size_t)r * p.table_stride + slot] : -1;
+                if (page < 0 || page >= p.num_pages) atomicOr(p.status, EG_STATUS_BAD_PAGE);
+                else row = page * p.page_stride + kvh * p.head_stride + (long long)(at % p.page_size) * D;
+            }
+            key_row[tid] = row;
+            const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
+            if (tid == 0) keys_there = there;
+        }
+        __syncthreads();
+        bool odd = false;                                            // a value that is not finite
+        for (int i = tid; i < KEYS * DMAX; i += THREADS) {
+            const int key = i / DMAX, d = i % DMAX;
+            const long long row = key_row[key];
+            float k = 0.f, v = 0.f;
+            if (d < D && row >= 0) {
+                k = to_f32<T>(static_cast<const T*>(p.k_cache)[row + d]);
+                v = to_f32<T>(static_cast<const T*>(p.v_cache)[row + d]);
+            }
+            odd |= !isfinite(v);
+            k_s[key * L::LD + d] = k;
+            v_s[key * L::LD + d] = v;
+        }
+        if (tid < ROWS) {
+            unsigned bits = 0;
+            if (tid < count) {
+                const int low = max(lowest[tid], key0), high = min(e.context, key0 + KEYS);      // the cached keys that it sees
+                if (low < high) bits = 0xffffffffu >> (KEYS - (high - low)) << (low - key0);
+                int left = p.window > 0 ? p.window : 0x7fffffff;
+                for (int i = (row0 + tid) / group; i >= 0 && e.context + i >= key0 && left > 0; i = up_of(i), --left)
+                    if (e.context + i < key0 + KEYS) bits |= 1u << (e.context + i - key0);
+            }
+            seen[tid] = bits & keys_there;
+        }
+        odd = __syncthreads_or(odd);
+        // ---- scores
+        float s[4][2] = {};
+        for (int d = 0; d < DMAX; d += 4) {
+            float4 a[4], b[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (4 * ty + i) * L::LD + d);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * L::LD + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned bits = seen[4 * ty + i];
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                s[i][j] = bits >> (tx + 16 * j) & 1 ? s[i][j] * scale_log2 : -INFINITY;
+                top = fmaxf(top, s[i][j]);
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float now = fmaxf(m[i], top), ref = now == -INFINITY ? 0.f : now;     // a row that has seen nothing: every weight 0
+            const float keep = exp2f(m[i] - ref);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float w = exp2f(s[i][j] - ref);
+                p_s[(4 * ty + i) * L::P_LD + tx + 16 * j] = w;
+                sum += w;
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[i] = l[i] * keep + sum;
+            m[i] = now;
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) acc[i][c][x] *= keep;
+        }
+        __syncwarp();                                                // a row's weights come from its own half warp
+        // ---- output
+        for (int key = 0; key < KEYS; ++key) {
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = p_s[(4 * ty + i) * L::P_LD + key];
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) {
+                float4 v = *reinterpret_cast<const float4*>(v_s + key * L::LD + 4 * tx + 64 * c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (odd && !(seen[4 * ty + i] >> key & 1)) continue;
+                    acc[i][c][0] = fmaf(w[i], v.x, acc[i][c][0]);
+                    acc[i][c][1] = fmaf(w[i], v.y, acc[i][c][1]);
+                    acc[i][c][2] = fmaf(w[i], v.z, acc[i][c][2]);
+                    acc[i][c][3] = fmaf(w[i], v.w, acc[i][c][3]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 4 * ty + i;
+        if (row >= count) continue;
+        const int node = (row0 + row) / group, head = kvh * group + (row0 + row) % group;
+        const float inv = parts > 1 ? 1.f : l[i] > 0.f ? 1.f / l[i] : 0.f;
+        const size_t line = (size_t)(e.first + node) * p.num_heads + head, slot = (size_t)part * p.rows * p.num_heads + line;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int d = 4 * tx + 64 * c + x;
+                if (d >= D) continue;
+                if (parts > 1) p.partial_o[slot * D + d] = acc[i][c][x];
+                else static_cast<T*>(p.out)[(size_t)(e.first + node) * p.ldo + (size_t)head * D + d] = from_f32<T>(acc[i][c][x] * inv);
+            }
+        if (parts > 1 && tx == 0) *reinterpret_cast<float2*>(p.partial_ml + slot * 2) = make_float2(m[i], l[i]);
+    }
+}
+
+// Adds the parts of a (row, head) up, in their order: a warp a line of the output, lanes over its columns.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) attention_tree_merge_kernel(const Params p, int row_tile, int key_tile) {
+    pdl_enter();
+    const int r = blockIdx.y, group = p.num_heads / p.num_kv_heads, lane = threadIdx.x & 31;
+    const Entry e = tree::entry_of(p, r);
+    const int first = tree::first_key(p, e);
+    const long long lines = (long long)e.n * p.num_heads;
+    for (long long line = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); line < lines; line += (long long)gridDim.x * (THREADS / 32)) {
+        const int node = (int)(line / p.num_heads), head = (int)(line % p.num_heads);
+        const int tile = (node * group + head % group) / row_tile, count = min(row_tile, e.n * group - tile * row_tile);
+        const int end = e.context + (tile * row_tile + count - 1) / group + 1;
+        const int parts = tree::parts_of(p, (end - 1) / key_tile - first / key_tile + 1);
+        if (parts <= 1) continue;
+        const size_t at = (size_t)e.first * p.num_heads + line, stride = (size_t)p.rows * p.num_heads;
+        float top = -INFINITY, total = 0.f;
+        for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(p.partial_ml + (at + i * stride) * 2));
+        for (int i = 0; i < parts; ++i) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + (at + i * stride) * 2));
+            total += ml.x == -INFINITY ? 0.f : exp2f(ml.x - top) * ml.y;
+        }
+        const float inv = total > 0.f ? 1.f / total : 0.f;
+        for (int d = lane; d < p.head_dim; d += 32) {
+            float sum = 0.f;
+            for (int i = 0; i < parts; ++i) {
+                const float m = __ldcg(p.partial_ml + (at + i * stride) * 2);
+                if (m != -INFINITY) sum = fmaf(exp2f(m - top), __ldcg(p.partial_o + (at + i * stride) * p.head_dim + d), sum);
+            }
+            static_cast<T*>(p.out)[(size_t)(e.first + node) * p.ldo + (size_t)head * p.head_dim + d] = from_f32<T>(sum * inv);
+        }
+    }
+}
+
+template <typename T, int DMAX>
+int launch(cudaStream_t stream, const Params& p, int tiles) {
+    const int bytes = Layout<DMAX>::FLOATS * 4;
+    const cudaError_t set = cudaFuncSetAttribute(attention_tree_kernel<T, DMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (set != cudaSuccess) return (int)set;
+    eg_pdl_launch(attention_tree_kernel<T, DMAX>, dim3(p.max_parts, p.num_kv_heads, tiles), dim3(THREADS), bytes, stream, p);
+    return eg_launch_status();
+}
+
+}  // namespace
+
+// q: [rows, ldq], out: [rows, ldo] of num_heads * head_dim columns; k_cache, v_cache: [num_pages][num_kv_heads][page_size][head_dim] with the same strides (in
+// elements); block_table: [entries, table_pages] with row stride table_stride; entry_starts: [entries + 1]; context: [entries]; parents: [rows].  A tile's keys
+// are cut into up to max_parts parts of at least part_tiles key tiles (of 32): partial_o takes max_parts * rows * num_heads * head_dim floats, partial_ml
+// max_parts * rows * num_heads * 2 (neither is used with max_parts 1).
+EG_API int eg_attention_tree(cudaStream_t stream, int dtype, const void* q, long long ldq, const void* k_cache, const void* v_cache, long long page_stride,
+                             long long head_stride, const int* block_table, int table_stride, int table_pages, int num_pages, const int* entry_starts, const int* context,
+                             const int* parents, void* out, long long ldo, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int window,
+                             float scale, int max_parts, int part_tiles, float* partial_o, float* partial_ml, int* status) {
+    if (entries <= 0 || rows <= 0) return 0;
+    if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads || num_kv_heads > 65535 || head_dim < 1 || head_dim > 256 || page_size < 1 || num_pages < 1 ||
+        table_pages < 0 || entries > 65535 || max_parts < 1 || part_tiles < 1 || (max_parts > 1 && (!partial_o || !partial_ml)) || !status || (dtype != EG_F32 && dtype != EG_BF16))
+        return (int)cudaErrorInvalidValue;
+    const long long tiles = (long long)rows * (num_heads / num_kv_heads) / ROWS + entries;      // at most: every entry's last tile may be a short one
+    if (tiles > 65535 || (long long)rows * num_heads > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    const Params p = {q, ldq, k_cache, v_cache, page_stride, head_stride, block_table, table_stride, table_pages, num_pages, entry_starts, context, parents, out, ldo,
+                      rows, entries, num_heads, num_kv_heads, head_dim, page_size, window, scale, max_parts, part_tiles, partial_o, partial_ml, status};
+    int code;
+    if (dtype == EG_F32)
+        code = head_dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);
+    else
+        code = head_dim <= 64 ? launch<bf16, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<bf16, 128>(stream, p, (int)tiles) : launch<bf16, 256>(stream, p, (int)tiles);
+    if (code || max_parts == 1) return code;
+    const dim3 grid((unsigned)min((long long)1024, ((long long)rows * num_heads + THREADS / 32 - 1) / (THREADS / 32)), entries);
+    if (dtype == EG_F32) eg_pdl_launch(attention_tree_merge_kernel<float>, grid, dim3(THREADS), 0, stream, p, ROWS, KEYS);
+    else eg_pdl_launch(attention_tree_merge_kernel<bf16>, grid, dim3(THREADS), 0, stream, p, ROWS, KEYS);
+    return eg_launch_status();
+}

@@ -20,6 +20,7 @@ enum {
     EG_STATUS_BAD_PAGE = 2,       // block table entry outside [0, num_pages) where a key was needed
     EG_STATUS_BAD_SLOT = 4,       // cache write position outside the pool
     EG_STATUS_WAIT_TIMEOUT = 8,   // a bounded wait on a barrier gave up
+    EG_STATUS_BAD_TREE = 16,      // rows of a drafted tree, a parent or an accepted path that cannot be one
 };
 
 template <typename T> __device__ __forceinline__ float to_f32(T v);

@@ -8,6 +8,7 @@ library cannot be built or loaded, importing it raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -24,7 +25,8 @@ _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16}
 STATUS_BITS = {1: "a token id lies outside the vocabulary",
                2: "a block table entry needed by attention is not a valid page",
                4: "a cache write position lies outside the pool",
-               8: "a bounded wait inside a kernel gave up"}
+               8: "a bounded wait inside a kernel gave up",
+               16: "rows of a drafted tree, a parent or an accepted path that cannot be one"}
 
 
 class KernelError(RuntimeError):
@@ -96,6 +98,12 @@ class _Signatures:
     eg_argmax = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p]
     eg_wait_probe = [c_void_p, ctypes.c_uint, c_int, c_void_p, c_void_p]
     eg_sample = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    eg_sample_min_p = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    eg_attention_tree = [c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
+                         c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p]
+    eg_tree_accept = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
+    eg_cache_keep = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_void_p, c_int, c_int,
+                     c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]
 
 
 class Timeline:
@@ -162,6 +170,20 @@ def _cuda(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(*tensors):
+    """CUDA tensors of one device, and that device as the current one for the launch."""
+    device = tensors[0].device
+    for t in tensors:
+        if not t.is_cuda:
+            raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
+        if t.device != device:
+            raise KernelError("tensors of one device")
+    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def embedding_gather(ids: torch.Tensor, table: torch.Tensor, residual: torch.Tensor, status: torch.Tensor) -> None:
@@ -892,6 +914,106 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
     _need(min(temperature.numel(), top_k.numel(), top_p.numel(), uniform.numel(), out.numel()) >= rows, "one value per row")
     _check(library().eg_sample(_stream(), _ptr(logits), logits.stride(0), rows, logits.shape[1], _ptr(temperature),
                                _ptr(top_k), _ptr(top_p), _ptr(uniform), _ptr(out)), "sample")
+
+
+def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
+                 uniform: torch.Tensor, out: torch.Tensor) -> None:
+    """``sample`` with a further cut, and with its sums in 64 bits: per row temperature <= 0 -> greedy; else softmax(logits / T)
+    cut by top_k (0 = off), then top_p (1 = off), then to the tokens with at least min_p times the largest one's probability
+    (0 = off), drawn by inverse CDF in index order with uniform[r].  Ties go to the lower index; NaN is never kept; tokens of less
+    than 2^-43 of the largest one's probability are never drawn; a row without a number above -inf gives 0."""
+    with _on(logits, temperature, top_k, top_p, min_p, uniform, out):
+        _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1, "float32 rows")
+        rows, vocab = logits.shape
+        _need(1 <= vocab <= SAMPLE_MAX_VOCAB, f"1 to {SAMPLE_MAX_VOCAB} logits a row")
+        _need(temperature.dtype == top_p.dtype == min_p.dtype == uniform.dtype == torch.float32 and top_k.dtype == out.dtype == torch.int32,
+              "float32 temperature/top_p/min_p/uniform, int32 top_k/out")
+        for t in (temperature, top_k, top_p, min_p, uniform, out):
+            _need(t.numel() >= rows and t.is_contiguous(), "one value per row, contiguous")
+        _check(library().eg_sample_min_p(_stream(), _ptr(logits), logits.stride(0), rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                         _ptr(min_p), _ptr(uniform), _ptr(out)), "sample_min_p")
+
+
+SAMPLE_MAX_VOCAB = 1 << 20
+
+
+def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, entry_starts: torch.Tensor,
+                   context: torch.Tensor, parents: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
+                   window: Optional[int], scale: float, status: torch.Tensor, max_context: Optional[int] = None) -> None:
+    """Attention of drafted trees over the paged cache.  Entry r's nodes are the rows entry_starts[r] .. entry_starts[r + 1] - 1 of q
+    [>= T, >= NH*HD] and out [>= T, >= NH*HD] (rows behind the last entry's are left as they are), numbered from 0; parents[row] of
+    parents [T] is the number of a node's parent, lower than its own, or -1.  context[r] keys are cached before the step; node i's keys and values were stored at
+    cache position context[r] + i (and rotated at position context[r] + depth).  A node sees the cached keys, its ancestors and itself;
+    with a window, those of them whose position is above its own minus the window.  Caches [pages, NKV, page_size, HD], block_table
+    [entries, pages of a request], all int32 but q, out and the caches (float32 or bfloat16).  ``max_context``: the most keys an entry
+    has, cached and its own, as far as the caller knows (how the work is split follows it; by default what the block table has room for).
+    Bits of ``status``: 16 rows or a parent that cannot be (such rows are left, such a node has no parent), 2 a page that is none (its
+    keys are not seen)."""
+    with _on(q, k_cache, v_cache, block_table, entry_starts, context, parents, out, status):
+        T, entries, page_size, dtype = parents.numel(), block_table.shape[0], k_cache.shape[2], dtype_code(q.dtype)
+        _need(0 < num_kv_heads <= num_heads and num_heads % num_kv_heads == 0 and 0 < head_dim <= 256, "heads in whole groups, head sizes up to 256")
+        _need(q.dim() == 2 and out.dim() == 2 and q.stride(1) == 1 and out.stride(1) == 1 and q.dtype == out.dtype == k_cache.dtype == v_cache.dtype
+              and q.shape[1] >= num_heads * head_dim and out.shape[1] >= num_heads * head_dim and q.shape[0] >= T
+              and out.shape[0] >= T, "q/out/cache layout")
+        _need(block_table.dtype == entry_starts.dtype == context.dtype == parents.dtype == status.dtype == torch.int32 and block_table.dim() == 2
+              and (block_table.stride(1) == 1 or block_table.shape[1] <= 1), "int32 metadata")
+        _need(entry_starts.numel() == entries + 1 and context.numel() >= entries and entry_starts.is_contiguous() and context.is_contiguous()
+              and parents.is_contiguous(), "entry_starts [entries + 1], context [entries], contiguous parents")
+        _need(k_cache.dim() == 4 and tuple(k_cache.shape[1:]) == (num_kv_heads, page_size, head_dim) and k_cache.shape == v_cache.shape
+              and k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1 and k_cache.stride(2) == head_dim, "cache shape [pages, NKV, page_size, HD]")
+        _need(window is None or window > 0, "a window of one key at least")
+        if max_context is None:
+            max_context = block_table.shape[1] * page_size
+        group = num_heads // num_kv_heads
+        units = max(1, entries * -(-T * group // (64 * max(1, entries))) * num_kv_heads)
+        parts = max(1, min(-(-2 * sm_count() // units), max_context // 64, 128))
+        scratch = torch.empty(parts * T * num_heads * (head_dim + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
+        partial_o = _ptr(scratch)
+        partial_ml = partial_o + parts * T * num_heads * head_dim * 4 if parts > 1 else None
+        _check(library().eg_attention_tree(
+            _stream(), dtype, _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), k_cache.stride(0), k_cache.stride(1), _ptr(block_table),
+            block_table.stride(0), block_table.shape[1], k_cache.shape[0], _ptr(entry_starts), _ptr(context), _ptr(parents), _ptr(out), out.stride(0), T, entries,
+            num_heads, num_kv_heads, head_dim, page_size, int(window or 0), float(scale), parts, 2, partial_o, partial_ml, _ptr(status)), "attention_tree")
+
+
+def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch.Tensor, parents: torch.Tensor, path: torch.Tensor,
+                accepted: torch.Tensor, emitted: torch.Tensor, status: torch.Tensor) -> None:
+    """The drafted tokens that the model agrees with.  tokens[row] is the token at a node, targets[row] the model's answer behind it
+    (``argmax`` or a sample of the row's logits), entry_starts and parents as in ``attention_tree``; all int32.  From node 0 of every entry
+    (its last known token) the walk goes to the first child with the token that the model answered, and on.  path [entries, P]: the walk's
+    nodes (at most P), then -1; accepted [entries]: how many they are; emitted [entries, P]: the model's answer at each, which is the entry's
+    new tokens (the last one is drafted by nobody), then -1.  An entry without rows accepts 0."""
+    with _on(tokens, targets, entry_starts, parents, path, accepted, emitted, status):
+        entries, rows = entry_starts.numel() - 1, tokens.numel()
+        for t in (tokens, targets, entry_starts, parents, path, accepted, emitted, status):
+            _need(t.dtype == torch.int32 and t.is_contiguous(), "contiguous int32 tensors")
+        _need(entries >= 0 and targets.numel() == rows and parents.numel() >= rows, "one target and one parent per token, entry_starts [entries + 1]")
+        _need(path.dim() == 2 and path.shape[0] == entries and path.shape[1] >= 1 and emitted.shape == path.shape and accepted.numel() >= entries,
+              "path and emitted [entries, P], accepted [entries]")
+        _check(library().eg_tree_accept(_stream(), _ptr(tokens), _ptr(targets), _ptr(entry_starts), _ptr(parents), entries, rows, path.shape[1], _ptr(path),
+                                        _ptr(accepted), _ptr(emitted), _ptr(status)), "tree_accept")
+
+
+def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, context: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor,
+               status: torch.Tensor) -> None:
+    """Moves the accepted nodes' keys and values to where they belong: of every request r and j < accepted[r], the row at cache position
+    context[r] + path[r, j] goes to context[r] + j, in every layer, plane and head of kv [layers, pages, 2, NKV, page_size, HD] (a cache
+    group's pool), through block_table [entries, pages of a request]; context, path [entries, P] and accepted as in ``tree_accept``.
+    Bits of ``status``: 16 a path that does not ascend, or accepted outside 0 .. P (nothing of that request is moved), 2 a page that is none
+    (that row is not moved)."""
+    with _on(kv, block_table, context, path, accepted, status):
+        _need(kv.dim() == 6 and kv.shape[2] == 2 and kv.element_size() in (2, 4) and (kv.shape[5] == 1 or kv.stride(5) == 1)
+              and (kv.shape[4] == 1 or kv.stride(4) == kv.shape[5]), "kv [layers, pages, 2, NKV, page_size, HD] of 2 or 4 bytes, whole rows")
+        for t in (block_table, context, path, accepted, status):
+            _need(t.dtype == torch.int32, "int32 metadata")
+        entries = path.shape[0]
+        _need(path.dim() == 2 and path.is_contiguous() and path.shape[1] >= 1 and accepted.numel() >= entries and context.numel() >= entries
+              and accepted.is_contiguous() and context.is_contiguous(), "path [entries, P], accepted and context [entries]")
+        _need(block_table.dim() == 2 and block_table.shape[0] >= entries and (block_table.stride(1) == 1 or block_table.shape[1] <= 1), "block table")
+        layers, pages, _, kv_heads, page_size, head_dim = kv.shape
+        _check(library().eg_cache_keep(_stream(), _ptr(kv), kv.element_size(), layers, pages, kv_heads, page_size, head_dim, kv.stride(0), kv.stride(1), kv.stride(2),
+                                       kv.stride(3), _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(context), _ptr(path), _ptr(accepted),
+                                       entries, path.shape[1], _ptr(status)), "cache_keep")
 
 
 def wait_probe(limit: int, threads: int, status: torch.Tensor) -> int:

@@ -1,0 +1,95 @@
+"""What the operators of a step over drafted trees refuse before anything is launched (no GPU): by their Python faces, and by the launchers alone."""
+import contextlib
+
+import pytest
+import torch
+
+from easy_gpt.cpp_b200 import kernels
+
+
+class Reached(Exception):
+    pass
+
+
+@pytest.fixture
+def on_the_host(monkeypatch):
+    """Tensors of the host pass for tensors of a device, and a launch is an exception of its own."""
+    def reached():
+        raise Reached
+
+    monkeypatch.setattr(kernels, "_on", lambda *tensors: contextlib.nullcontext())
+    monkeypatch.setattr(kernels, "library", reached)
+    monkeypatch.setattr(kernels, "_stream", lambda: 0)
+
+
+def i32(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+CACHE = torch.zeros((4, 2, 2, 16, 64), dtype=torch.bfloat16)
+ROWS = torch.zeros((10, 256), dtype=torch.bfloat16)
+ATTENTION = dict(q=ROWS, k_cache=CACHE[:, 0], v_cache=CACHE[:, 1], block_table=i32(2, 3), entry_starts=i32(3), context=i32(2), parents=i32(10), out=ROWS.clone(), num_heads=4, num_kv_heads=2,
+                 head_dim=64, window=None, scale=0.125, status=i32(1))
+NUMBERS = torch.zeros(2)
+SAMPLE = dict(logits=torch.zeros((2, 8)), temperature=NUMBERS, top_k=i32(2), top_p=NUMBERS, min_p=NUMBERS, uniform=NUMBERS, out=i32(2))
+ACCEPT = dict(tokens=i32(2), targets=i32(2), entry_starts=i32(3), parents=i32(2), path=i32(2, 3), accepted=i32(2), emitted=i32(2, 3), status=i32(1))
+KV = torch.zeros((1, 4, 2, 2, 16, 64))
+KEEP = dict(kv=KV, block_table=i32(2, 2), context=i32(2), path=i32(2, 3), accepted=i32(2), status=i32(1))
+REFUSED = [
+    *(("attention_tree", ATTENTION, w) for w in (
+        dict(q=ROWS.float()), dict(q=ROWS.half(), out=ROWS.half(), k_cache=CACHE[:, 0].half(), v_cache=CACHE[:, 1].half()), dict(num_heads=3), dict(num_kv_heads=0), dict(num_heads=0), dict(head_dim=32),
+        dict(head_dim=300), dict(block_table=i32(2, 3).long()), dict(block_table=i32(3, 2).t()), dict(block_table=i32(6)), dict(entry_starts=i32(2)), dict(context=i32(1)), dict(context=i32(4)[::2]),
+        dict(parents=i32(11)), dict(parents=i32(20)[::2]), dict(out=ROWS[:4]), dict(out=ROWS[:, :255]), dict(v_cache=CACHE[:1, 1]), dict(k_cache=CACHE[:, 0].transpose(2, 3)), dict(k_cache=CACHE[0, 0]),
+        dict(status=i32(1).long()), dict(q=ROWS[:, :64]), dict(q=ROWS[0]), dict(window=-3), dict(window=0), dict(v_cache=CACHE[:, 1].float()))),
+    *(("sample_min_p", SAMPLE, w) for w in (
+        dict(logits=torch.zeros((2, 8), dtype=torch.float64)), dict(logits=torch.zeros((8, 2)).t()), dict(logits=torch.zeros(8)), dict(temperature=NUMBERS.double()), dict(top_k=NUMBERS),
+        dict(min_p=NUMBERS[:1]), dict(out=i32(2).long()), dict(logits=torch.zeros((2, 0))), dict(logits=torch.zeros((1, 1)).expand(2, (1 << 20) + 1)), dict(top_p=torch.zeros(4)[::2]))),
+    *(("tree_accept", ACCEPT, w) for w in (
+        dict(tokens=i32(2).long()), dict(targets=i32(1)), dict(parents=i32(1)), dict(path=i32(1, 3)), dict(emitted=i32(2, 2)), dict(accepted=i32(1)), dict(path=i32(2, 0), emitted=i32(2, 0)),
+        dict(path=i32(3, 2).t()), dict(path=i32(6)), dict(entry_starts=i32(0)))),
+    *(("cache_keep", KEEP, w) for w in (
+        dict(kv=KV[0]), dict(kv=KV.double()), dict(kv=KV[:, :, :1]), dict(kv=KV.transpose(4, 5)), dict(kv=KV[..., ::2]), dict(block_table=i32(1, 2)), dict(block_table=i32(4)), dict(context=i32(1)),
+        dict(path=i32(2, 3).long()), dict(accepted=i32(1)), dict(path=i32(3)), dict(path=i32(2, 0)), dict(path=i32(2, 6)[:, ::2]))),
+]
+
+
+@pytest.mark.parametrize("name, base, wrong", REFUSED)
+def test_refused_before_a_launch(name, base, wrong, on_the_host):
+    with pytest.raises(kernels.KernelError):
+        getattr(kernels, name)(**{**base, **wrong})
+
+
+@pytest.mark.parametrize("name, base", [("attention_tree", ATTENTION), ("sample_min_p", SAMPLE), ("tree_accept", ACCEPT), ("cache_keep", KEEP)])
+def test_taken(name, base, on_the_host):
+    with pytest.raises(Reached):
+        getattr(kernels, name)(**base)
+
+
+@pytest.mark.parametrize("name, base", [("attention_tree", ATTENTION), ("sample_min_p", SAMPLE), ("tree_accept", ACCEPT), ("cache_keep", KEEP)])
+def test_there_is_no_cpu_path(name, base):
+    with pytest.raises(kernels.KernelError, match="no CPU path"):
+        getattr(kernels, name)(**base)
+
+
+def test_launchers_refuse_sizes_they_do_not_take():
+    """The C entry points by themselves: cudaErrorInvalidValue (1) for what their callers could get wrong, 0 for nothing to do; nothing is launched."""
+    lib, at = kernels.library(), 0x1000
+    sample = lambda rows, vocab: lib.eg_sample_min_p(None, at, vocab, rows, vocab, at, at, at, at, at, at)  # noqa: E731
+    assert [sample(0, 8), sample(1, 0), sample(1, (1 << 20) + 1)] == [0, 1, 1]
+    accept = lambda entries, rows, longest, status=at: lib.eg_tree_accept(None, at, at, at, at, entries, rows, longest, at, at, at, status)  # noqa: E731
+    assert [accept(0, 0, 1), accept(1, -1, 1), accept(1, 1, 0), accept(1, 1, 1, None)] == [0, 1, 1, 1]
+
+    def keep(kv=at, size=2, layers=1, pages=4, heads=2, page=16, dim=64, entries=1, longest=3, status=at):
+        return lib.eg_cache_keep(None, kv, size, layers, pages, heads, page, dim, 0, 2 * heads * page * dim, heads * page * dim, page * dim, at, 2, 2, at, at, at, entries, longest, status)
+
+    assert [keep(entries=0), keep(layers=0)] == [0, 0]
+    assert [keep(size=1), keep(size=8), keep(pages=0), keep(heads=0), keep(page=0), keep(dim=0), keep(longest=0), keep(status=None), keep(entries=65536), keep(kv=at + 1),
+            keep(layers=1 << 30)] == [1] * 11
+
+    def attend(dtype=kernels.BF16, rows=4, entries=1, heads=4, kv_heads=2, dim=64, page=16, pages=4, parts=1, tiles=1, scratch=at, status=at):
+        return lib.eg_attention_tree(None, dtype, at, 256, at, at, 4096, 1024, at, 3, 3, pages, at, at, at, at, 256, rows, entries, heads, kv_heads, dim, page, 0, 0.125, parts, tiles, scratch,
+                                     scratch, status)
+
+    assert [attend(rows=0), attend(entries=0)] == [0, 0]
+    assert [attend(dtype=2), attend(heads=3), attend(kv_heads=0), attend(dim=0), attend(dim=257), attend(page=0), attend(pages=0), attend(parts=0), attend(tiles=0), attend(parts=2, scratch=None),
+            attend(status=None), attend(entries=65536), attend(rows=1 << 30)] == [1] * 13
