@@ -37,23 +37,13 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     __shared__ int lowest[ROWS];                                     // a row's first cached key
     __shared__ long long key_row[KEYS];                              // where a key's row lies in the cache; -1: there is none
     __shared__ unsigned keys_there;
-    __shared__ int place_entry, place_tile;
     pdl_enter();
     const int part = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
-    if (tid < 32) {
-        int entry, within;
-        tree::find_tile(p, blockIdx.z, ROWS, entry, within);
-        if (tid == 0) {
-            place_entry = entry;
-            place_tile = within;
-        }
-    }
-    __syncthreads();
-    if (place_entry < 0) return;
-    const int r = place_entry, group = p.num_heads / p.num_kv_heads;
-    const Entry e = tree::entry_of(p, r);
-    if (e.n == 0) return;
-    const int D = p.head_dim, row0 = place_tile * ROWS, count = min(ROWS, e.n * group - row0);
+    const int group = p.num_heads / p.num_kv_heads;
+    int r, within;
+    Entry e;
+    if (!tree::find_tile(p, blockIdx.z, ROWS, r, e, within)) return;
+    const int D = p.head_dim, row0 = within * ROWS, count = min(ROWS, e.n * group - row0);
     const int last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;    // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
@@ -221,7 +211,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS) attention_tree_merge_kernel(const Params p, int row_tile, int key_tile) {
     pdl_enter();
     const int r = blockIdx.y, group = p.num_heads / p.num_kv_heads, lane = threadIdx.x & 31;
-    const Entry e = tree::entry_of(p, r);
+    const Entry e = tree::sound(p, p.entry_starts[r], p.entry_starts[r + 1], p.context[r]);
     const int first = tree::first_key(p, e);
     const long long lines = (long long)e.n * p.num_heads;
     for (long long line = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); line < lines; line += (long long)gridDim.x * (THREADS / 32)) {
@@ -260,30 +250,57 @@ int launch(cudaStream_t stream, const Params& p, int tiles) {
 
 }  // namespace
 
+// How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (16, 32 or 64: the tensor-core kernel; 0: the 32-bit one),
+// plan[1] and plan[2] the max_parts and part_tiles of eg_attention_tree.  aligned: q, out and their rows start on 4-byte boundaries, the
+// caches, their pages and heads on 16-byte ones.  max_context: the most keys of an entry, as far as known.
+EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count,
+                                  int* plan) {
+    if (rows < 1 || entries < 1 || num_kv_heads < 1 || num_heads % num_kv_heads || num_heads < 1 || page_size < 1 || sm_count < 1 || !plan) return (int)cudaErrorInvalidValue;
+    const int group = num_heads / num_kv_heads;
+    const long long lines = ((long long)rows * group + entries - 1) / entries;      // of an entry, on the average
+    const bool tiled = dtype == EG_BF16 && aligned && page_size % 16 == 0 && (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256);
+    const int row_tile = !tiled ? ROWS : lines <= 16 ? 16 : lines <= 32 ? 32 : 64;
+    const long long units = entries * ((lines + row_tile - 1) / row_tile) * num_kv_heads, key_tiles = ((long long)max_context + 63) / 64;
+    const long long places = (long long)sm_count * (tiled ? 3 : 2);
+    long long parts = (places + units - 1) / units;
+    if (parts > key_tiles / 2) parts = key_tiles / 2;
+    plan[0] = tiled ? row_tile : 0;
+    plan[1] = (int)(parts < 1 ? 1 : parts > 128 ? 128 : parts);
+    plan[2] = 2;
+    return 0;
+}
+
 // q: [rows, ldq], out: [rows, ldo] of num_heads * head_dim columns; k_cache, v_cache: [num_pages][num_kv_heads][page_size][head_dim] with the same strides (in
 // elements); block_table: [entries, table_pages] with row stride table_stride; entry_starts: [entries + 1]; context: [entries]; parents: [rows].  A tile's keys
-// are cut into up to max_parts parts of at least part_tiles key tiles (of 32): partial_o takes max_parts * rows * num_heads * head_dim floats, partial_ml
+// are cut into up to max_parts parts of at least part_tiles times 64 keys: partial_o takes max_parts * rows * num_heads * head_dim floats, partial_ml
 // max_parts * rows * num_heads * 2 (neither is used with max_parts 1).
 EG_API int eg_attention_tree(cudaStream_t stream, int dtype, const void* q, long long ldq, const void* k_cache, const void* v_cache, long long page_stride,
                              long long head_stride, const int* block_table, int table_stride, int table_pages, int num_pages, const int* entry_starts, const int* context,
                              const int* parents, void* out, long long ldo, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int window,
-                             float scale, int max_parts, int part_tiles, float* partial_o, float* partial_ml, int* status) {
+                             float scale, int row_tile, int max_parts, int part_tiles, float* partial_o, float* partial_ml, int* status) {
     if (entries <= 0 || rows <= 0) return 0;
     if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads || num_kv_heads > 65535 || head_dim < 1 || head_dim > 256 || page_size < 1 || num_pages < 1 ||
-        table_pages < 0 || entries > 65535 || max_parts < 1 || part_tiles < 1 || (max_parts > 1 && (!partial_o || !partial_ml)) || !status || (dtype != EG_F32 && dtype != EG_BF16))
+        table_pages < 0 || entries > 65535 || max_parts < 1 || part_tiles < 1 || (max_parts > 1 && (!partial_o || !partial_ml)) || !status || (dtype != EG_F32 && dtype != EG_BF16) ||
+        part_tiles > 1 << 20 || (row_tile != 0 && row_tile != 16 && row_tile != 32 && row_tile != 64))
         return (int)cudaErrorInvalidValue;
-    const long long tiles = (long long)rows * (num_heads / num_kv_heads) / ROWS + entries;      // at most: every entry's last tile may be a short one
+    if (row_tile && (dtype != EG_BF16 || (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) || page_size % 16 || (uintptr_t)q % 4 || ldq % 2 ||
+                     (uintptr_t)out % 4 || ldo % 2 || (uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || page_stride % 8 || head_stride % 8))
+        return (int)cudaErrorInvalidValue;
+    const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
+    const long long tiles = (long long)rows * (num_heads / num_kv_heads) / tile_rows + entries; // at most: every entry's last tile may be a short one
     if (tiles > 65535 || (long long)rows * num_heads > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const Params p = {q, ldq, k_cache, v_cache, page_stride, head_stride, block_table, table_stride, table_pages, num_pages, entry_starts, context, parents, out, ldo,
-                      rows, entries, num_heads, num_kv_heads, head_dim, page_size, window, scale, max_parts, part_tiles, partial_o, partial_ml, status};
+                      rows, entries, num_heads, num_kv_heads, head_dim, page_size, window, scale, max_parts, part_tiles * (64 / tile_keys), partial_o, partial_ml, status};
     int code;
-    if (dtype == EG_F32)
+    if (row_tile)
+        code = tree::launch_mma(stream, p, row_tile, (int)tiles);
+    else if (dtype == EG_F32)
         code = head_dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);
     else
         code = head_dim <= 64 ? launch<bf16, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<bf16, 128>(stream, p, (int)tiles) : launch<bf16, 256>(stream, p, (int)tiles);
     if (code || max_parts == 1) return code;
     const dim3 grid((unsigned)min((long long)1024, ((long long)rows * num_heads + THREADS / 32 - 1) / (THREADS / 32)), entries);
-    if (dtype == EG_F32) eg_pdl_launch(attention_tree_merge_kernel<float>, grid, dim3(THREADS), 0, stream, p, ROWS, KEYS);
-    else eg_pdl_launch(attention_tree_merge_kernel<bf16>, grid, dim3(THREADS), 0, stream, p, ROWS, KEYS);
+    if (dtype == EG_F32) eg_pdl_launch(attention_tree_merge_kernel<float>, grid, dim3(THREADS), 0, stream, p, tile_rows, tile_keys);
+    else eg_pdl_launch(attention_tree_merge_kernel<bf16>, grid, dim3(THREADS), 0, stream, p, tile_rows, tile_keys);
     return eg_launch_status();
 }

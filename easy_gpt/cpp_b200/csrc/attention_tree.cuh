@@ -35,18 +35,15 @@ struct Params {
     int* status;
 };
 
-// An entry's place in the step; n = 0 where its rows cannot be what they say (and a status bit).
+// An entry's place in the step.
 struct Entry {
     int first, n, context;
 };
-__device__ __forceinline__ Entry entry_of(const Params& p, int r) {
-    Entry e;
-    e.first = p.entry_starts[r];
-    const int end = p.entry_starts[r + 1];
-    e.context = p.context[r];
-    e.n = end - e.first;
-    if (e.first < 0 || end < e.first || end > p.rows || e.context < 0 || e.context > 0x7fffffff - e.n) {
-        if (threadIdx.x == 0) atomicOr(p.status, EG_STATUS_BAD_TREE);
+// Entry r as the metadata has it; n = 0 where its rows cannot be what they say (and a status bit).
+__device__ __forceinline__ Entry sound(const Params& p, int first, int end, int context) {
+    Entry e = {first, end - first, context};
+    if (first < 0 || end < first || end > p.rows || context < 0 || context > 0x7fffffff - e.n) {
+        atomicOr(p.status, EG_STATUS_BAD_TREE);
         e.n = 0;
     }
     return e;
@@ -62,19 +59,14 @@ __device__ __forceinline__ int parent_of(const Params& p, const Entry& e, int i)
     return up;
 }
 
-// The entry whose tile number `tile` is, counting ceil(n * group / row_tile) tiles an entry, and the tile's number within it; entry -1: there
-// is none.  For a whole warp: 32 entries at a time.
-__device__ __forceinline__ void find_tile(const Params& p, int tile, int row_tile, int& entry, int& within) {
+// The entry whose tile number `tile` is, counting ceil(n * group / row_tile) tiles an entry, and the tile's number within it; false: there
+// is none.  For a whole warp: 32 entries at a time, in one trip to memory.
+__device__ __forceinline__ bool find_tile(const Params& p, int tile, int row_tile, int& r, Entry& e, int& within) {
     const int lane = threadIdx.x & 31, group = p.num_heads / p.num_kv_heads;
-    entry = -1;
-    within = 0;
     for (int base = 0; base < p.entries; base += 32) {
-        int tiles = 0;
-        if (base + lane < p.entries) {
-            const int first = p.entry_starts[base + lane], end = p.entry_starts[base + lane + 1];
-            if (first >= 0 && end >= first && end <= p.rows) tiles = (int)(((long long)(end - first) * group + row_tile - 1) / row_tile);
-            else atomicOr(p.status, EG_STATUS_BAD_TREE);
-        }
+        Entry mine = {0, 0, 0};
+        if (base + lane < p.entries) mine = sound(p, p.entry_starts[base + lane], p.entry_starts[base + lane + 1], p.context[base + lane]);
+        const int tiles = (int)(((long long)mine.n * group + row_tile - 1) / row_tile);
         int upto = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
@@ -84,17 +76,24 @@ __device__ __forceinline__ void find_tile(const Params& p, int tile, int row_til
         const unsigned here = __ballot_sync(0xffffffffu, tile < upto);
         if (here) {
             const int who = __ffs(here) - 1;
-            entry = base + who;
+            r = base + who;
+            e.first = __shfl_sync(0xffffffffu, mine.first, who);
+            e.n = __shfl_sync(0xffffffffu, mine.n, who);
+            e.context = __shfl_sync(0xffffffffu, mine.context, who);
             within = tile - __shfl_sync(0xffffffffu, upto - tiles, who);
-            return;
+            return true;
         }
         tile -= __shfl_sync(0xffffffffu, upto, 31);
     }
+    return false;
 }
 
 // A tile's first key that any of its rows may see, and the key behind its last one.
 __device__ __forceinline__ int first_key(const Params& p, const Entry& e) { return p.window > 0 && e.context >= p.window ? e.context - p.window + 1 : 0; }
 
 __device__ __forceinline__ int parts_of(const Params& p, int key_tiles) { return max(1, min(p.max_parts, key_tiles / p.part_tiles)); }
+
+// The kernel in attention_tree_mma.cu (16, 32 or 64 rows a CTA, key tiles of 64).  Its caller has checked what it takes.
+int launch_mma(cudaStream_t stream, const Params& p, int row_tile, int tiles);
 
 }  // namespace tree

@@ -100,7 +100,8 @@ class _Signatures:
     eg_sample = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_sample_min_p = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_attention_tree = [c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
-                         c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p, c_void_p, c_void_p]
+                         c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]
+    eg_attention_tree_plan = [c_int] * 10 + [c_void_p]
     eg_tree_accept = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_cache_keep = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_void_p, c_int, c_int,
                      c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]
@@ -937,6 +938,14 @@ def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
 SAMPLE_MAX_VOCAB = 1 << 20
 
 
+@functools.lru_cache(maxsize=4096)
+def attention_tree_plan(dtype: int, aligned: bool, rows: int, entries: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_context: int):
+    """(rows of a CTA or 0 for the 32-bit kernel, the most parts a row tile's keys are cut into, the fewest times 64 keys of a part)."""
+    plan = (c_int * 3)()
+    _need(library().eg_attention_tree_plan(dtype, aligned, rows, entries, num_heads, num_kv_heads, head_dim, page_size, max_context, sm_count(), plan) == 0, "sizes of a step")
+    return tuple(plan)
+
+
 def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, entry_starts: torch.Tensor,
                    context: torch.Tensor, parents: torch.Tensor, out: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int,
                    window: Optional[int], scale: float, status: torch.Tensor, max_context: Optional[int] = None) -> None:
@@ -964,16 +973,17 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _need(window is None or window > 0, "a window of one key at least")
         if max_context is None:
             max_context = block_table.shape[1] * page_size
-        group = num_heads // num_kv_heads
-        units = max(1, entries * -(-T * group // (64 * max(1, entries))) * num_kv_heads)
-        parts = max(1, min(-(-2 * sm_count() // units), max_context // 64, 128))
+        row_tile, parts, part_tiles = attention_tree_plan(
+            dtype, (q.data_ptr() | out.data_ptr() | (q.stride(0) | out.stride(0)) * q.element_size()) % 4 == 0
+            and (k_cache.data_ptr() | v_cache.data_ptr() | (k_cache.stride(0) | k_cache.stride(1)) * q.element_size()) % 16 == 0,
+            T, entries, num_heads, num_kv_heads, head_dim, page_size, int(max_context)) if T and entries else (0, 1, 1)
         scratch = torch.empty(parts * T * num_heads * (head_dim + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
         partial_o = _ptr(scratch)
         partial_ml = partial_o + parts * T * num_heads * head_dim * 4 if parts > 1 else None
         _check(library().eg_attention_tree(
             _stream(), dtype, _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), k_cache.stride(0), k_cache.stride(1), _ptr(block_table),
             block_table.stride(0), block_table.shape[1], k_cache.shape[0], _ptr(entry_starts), _ptr(context), _ptr(parents), _ptr(out), out.stride(0), T, entries,
-            num_heads, num_kv_heads, head_dim, page_size, int(window or 0), float(scale), parts, 2, partial_o, partial_ml, _ptr(status)), "attention_tree")
+            num_heads, num_kv_heads, head_dim, page_size, int(window or 0), float(scale), row_tile, parts, part_tiles, partial_o, partial_ml, _ptr(status)), "attention_tree")
 
 
 def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch.Tensor, parents: torch.Tensor, path: torch.Tensor,
