@@ -121,6 +121,19 @@ static inline void eg_pdl_launch(void (*kernel)(P...), dim3 grid, dim3 block, si
     eg_pdl_launch_if(true, kernel, grid, block, shared_bytes, stream, args...);
 }
 
+// Whether a kernel's attributes are still to be set on the current device (they are a device's own): `seen` is a static of the caller's, a bit a
+// device.  Two threads may both be told so, which sets the same attributes twice.
+static inline bool eg_first_on_device(unsigned long long& seen, int& device) {
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device > 63) {
+        device = -1;
+        return true;
+    }
+    return !(__atomic_load_n(&seen, __ATOMIC_ACQUIRE) >> device & 1);
+}
+static inline void eg_done_on_device(unsigned long long& seen, int device) {
+    if (device >= 0) __atomic_fetch_or(&seen, 1ull << device, __ATOMIC_RELEASE);
+}
+
 static inline int eg_launch_status() { return (int)cudaGetLastError(); }
 
 #ifdef EG_NEEDS_TENSOR_MAPS
