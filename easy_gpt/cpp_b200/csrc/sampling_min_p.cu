@@ -13,18 +13,21 @@
 // are the same in every order (shared-memory atomics among them).  Tokens below half of that have no weight.
 //
 // A row is a cluster's, up to 16 CTAs with a slice of it each in shared memory, so that it is read once however often it is passed over.
-// What most rows come to is a short list: the k largest, or what min-p or top-p leave.  A histogram over 512 equal steps below the largest
-// logit (of counts, or of weights too where top-p looks at the whole row) says up to which step; the tokens up to there, at most 1,024, go to
-// the first CTA, which sorts them and has all three cuts and the draw among them.  A row that keeps more finds the last token of top-k's and
-// top-p's runs by the same histogram, refined until a step's tokens are a short list (or all equal); then every CTA sums what is kept of its
-// slice, and the one in whose part the draw falls finds it.
+// What most rows come to is a short list: the k largest, or what min-p or top-p leave.  The tokens that can be among those, at most 1,024, go to the
+// first CTA, which puts them in order and has all three cuts and the draw among them.  With top-k they are those that are not below the k-th
+// largest of the threads' own maxima; with min-p its threshold says it; with top-p alone a histogram over 512 equal steps below the largest logit, of
+// counts and weights.  A row that keeps more finds the last token of top-k's and top-p's runs by such histograms, refined until a step's tokens
+// are a short list (or all equal); then every CTA sums what is kept of its slice, and the one in whose part the draw falls finds it.
+//
+// (A histogram's weights are three sums of 14 bits each: shared-memory atomics on 64 bits are loops of compare-and-swap, 5 to 18 times slower.)
 #include "common.cuh"
 
 namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = 1024, MOST_CTAS = 16;
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = 1024, SHORT = 128, MOST_CTAS = 16;
+constexpr int LIMBS = 3, LIMB_BITS = 14;                             // of a weight, at most 2^42: sums of 2^17 of them stay below 2^32
 constexpr int SLICE = 20480, MOST_SLICE = 51200;                     // logits of a slice: two CTAs an SM, and what fits at all
 constexpr double ONE = 4398046511104.0;                              // 2^42: with 2^20 tokens sums stay below 2^62
 constexpr int MOST_TOKENS = 1 << 20;
@@ -63,11 +66,6 @@ __device__ __forceinline__ unsigned remote(const void* mine, unsigned rank) {
     return a;
 }
 __device__ __forceinline__ void remote_store(unsigned at, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
-__device__ __forceinline__ u64 remote_load64(unsigned at) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ unsigned remote_load(unsigned at) {
     unsigned v;
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
@@ -79,38 +77,46 @@ __device__ __forceinline__ unsigned remote_add(unsigned at, unsigned n) {
     return v;
 }
 
+// 2^(i / 64), filled in by the first threads
+constexpr int POWERS = 64;
+
+template <int N, typename T, typename F>
+__device__ __forceinline__ T sum_of_loads(unsigned ctas, F load) {
+    T sum = 0, v[N];
+    for (unsigned q0 = 0; q0 < ctas; q0 += N) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = q0 + i < ctas ? load(q0 + i) : 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += v[i];
+    }
+    return sum;
+}
+
 struct Shared {
-    u64 slot[2][MOST_CTAS][2];                                       // what the CTAs tell each other, in turn
+    double power[POWERS];
+    __align__(16) u64 slot[2][MOST_CTAS][2];                                       // what the CTAs tell each other, in turn
     u64 warp_a[WARPS], warp_b[WARPS];
     u64 list[LIST], weights[LIST];
-    u64 bin_weight[BINS];
-    unsigned bin_count[BINS];
+    unsigned bin_weight[LIMBS][BINS], bin_count[BINS];
     unsigned listed;
     int found;
+    float floats[WARPS];
+    u64 pair[2];
 };
 
-// sums (or maxima) of a pair over the CTA
+// the sum (or the maximum) over the CTA
 template <bool MAX>
-__device__ __forceinline__ void block_join(u64& a, u64& b, Shared& s) {
+__device__ __forceinline__ u64 block_join(u64 a, Shared& s) {
     auto join = [](u64 x, u64 y) { return MAX ? (x > y ? x : y) : x + y; };
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
-        b = join(b, __shfl_xor_sync(0xffffffffu, b, o));
-    }
+    for (int o = 16; o > 0; o >>= 1) a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) {
-        s.warp_a[threadIdx.x >> 5] = a;
-        s.warp_b[threadIdx.x >> 5] = b;
-    }
+    if ((threadIdx.x & 31) == 0) s.warp_a[threadIdx.x >> 5] = a;
     __syncthreads();
     a = s.warp_a[threadIdx.x & (WARPS - 1)];
-    b = s.warp_b[threadIdx.x & (WARPS - 1)];
 #pragma unroll
-    for (int o = WARPS / 2; o > 0; o >>= 1) {
-        a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
-        b = join(b, __shfl_xor_sync(0xffffffffu, b, o));
-    }
+    for (int o = WARPS / 2; o > 0; o >>= 1) a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
+    return a;
 }
 // the inclusive sums of a pair over the CTA's threads
 __device__ __forceinline__ void block_scan(u64& a, u64& b, Shared& s) {
@@ -123,7 +129,14 @@ __device__ __forceinline__ void block_scan(u64& a, u64& b, Shared& s) {
     __syncthreads();
     if (lane == 31) s.warp_a[warp] = a, s.warp_b[warp] = b;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) a += s.warp_a[w], b += s.warp_b[w];
+    u64 x = lane < warp ? s.warp_a[lane] : 0, y = lane < warp ? s.warp_b[lane] : 0;
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        y += __shfl_xor_sync(0xffffffffu, y, o);
+    }
+    a += __shfl_sync(0xffffffffu, x, 0);
+    b += __shfl_sync(0xffffffffu, y, 0);
 }
 
 // descending, n a power of two
@@ -143,7 +156,7 @@ __device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (3
 
 // RESIDENT: the slice is in shared memory; else (vocabularies beyond what 16 CTAs hold) it is read from memory at every pass.
 template <bool RESIDENT>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 2)
 sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, int slice, const float* __restrict__ temperature, const int* __restrict__ top_k,
                     const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniform, int* __restrict__ out) {
     extern __shared__ __align__(16) float slice_s[];
@@ -152,8 +165,11 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     const int r = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int lo = min(vocab, (int)rank * slice), n = min(vocab, lo + slice) - lo;      // this CTA's tokens: lo .. lo + n - 1
     const float* const row = logits + (size_t)r * ld + lo;
-    for (int i = tid; i < BINS; i += THREADS) s.bin_count[i] = 0, s.bin_weight[i] = 0;
+    static_assert(BINS == THREADS, "a thread a step");
+    auto clear_bins = [&]() { s.bin_count[tid] = s.bin_weight[0][tid] = s.bin_weight[1][tid] = s.bin_weight[2][tid] = 0; };
+    clear_bins();
     if (tid == 0) s.listed = 0;
+    if (tid < POWERS) s.power[tid] = exp2((double)tid / POWERS);
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // the others may write here once they know that this CTA runs
     pdl_enter();
     const float T = temperature[r], p = top_p[r], u = uniform[r];
@@ -170,128 +186,175 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;\n" ::: "memory");
         __syncthreads();
     }
+    // f(x, i) for the thread's tokens, four at a time
+    auto for_all = [&](auto f) {
+        if constexpr (RESIDENT) {
+            for (int q = tid; q < n / 4; q += THREADS) {
+                const float4 v = reinterpret_cast<const float4*>(slice_s)[q];
+                f(v.x, 4 * q);
+                f(v.y, 4 * q + 1);
+                f(v.z, 4 * q + 2);
+                f(v.w, 4 * q + 3);
+            }
+            for (int i = n / 4 * 4 + tid; i < n; i += THREADS) f(slice_s[i], i);
+        } else {
+            for (int i = tid; i < n; i += THREADS) f(__ldg(row + i), i);
+        }
+    };
     auto at = [&](int i) { return RESIDENT ? slice_s[i] : __ldg(row + i); };
 
     int turn = 0;
     // every CTA's pair, after a barrier: what the CTAs in front of this one have (front), and all of them
-    auto exchange = [&](u64 a, u64 b, bool max, u64 (&all)[2], u64 (&front)[2]) {
+    auto exchange = [&](u64 a, u64 b, bool max, u64 (&all)[2], u64& front) {
         if (tid < (int)ctas) {
             const unsigned to = remote(&s.slot[turn][rank][0], tid);
             remote_store(to, a);
             remote_store(to + 8, b);
         }
         cluster_barrier();
-        all[0] = all[1] = front[0] = front[1] = 0;
-        for (unsigned c = 0; c < ctas; ++c)
-            for (int h = 0; h < 2; ++h) {
-                const u64 v = s.slot[turn][c][h];
-                all[h] = max ? (v > all[h] ? v : all[h]) : all[h] + v;
-                if (c < rank) front[h] += v;
-            }
+        all[0] = all[1] = front = 0;
+#pragma unroll
+        for (unsigned c = 0; c < MOST_CTAS; ++c) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&s.slot[turn][c][0]);
+            if (c >= ctas) continue;
+            all[0] = max ? (v.x > all[0] ? v.x : all[0]) : all[0] + v.x;
+            all[1] = max ? (v.y > all[1] ? v.y : all[1]) : all[1] + v.y;
+            if (c < rank) front += v.x;
+        }
         turn ^= 1;                                                   // a slot is written again behind another barrier, which its readers have to reach
     };
-    u64 all[2], front[2];
+    u64 all[2], front;
 
-    // ---- the first token in the descending order
-    u64 best = 0, none = 0;
-    for (int i = tid; i < n; i += THREADS) {
-        const u64 mine = token_of(key_of(at(i)), lo + i);
-        best = mine > best ? mine : best;
-    }
-    block_join<true>(best, none, s);
+    // ---- the largest logit, and every thread's
+    float mine_most = -INFINITY;                                     // NaN is passed over
+    for_all([&](float x, int) { mine_most = fmaxf(mine_most, x); });
+    float most = mine_most;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) s.floats[warp] = most;
+    __syncthreads();
+    most = s.floats[lane & (WARPS - 1)];
+#pragma unroll
+    for (int o = WARPS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-    exchange(best, 0, true, all, front);
-    const unsigned top = (unsigned)(all[0] >> 32);
-    const int first_best = index_of(all[0]);
+    exchange(key_of(most), 0, true, all, front);
+    const unsigned top = (unsigned)all[0];
     const float largest = value_of(top);
-    if (!(T > 0.f) || top <= MINUS_INFINITY_KEY) {
-        if (rank == 0 && tid == 0) out[r] = top <= MINUS_INFINITY_KEY ? 0 : first_best;
+    if (top <= MINUS_INFINITY_KEY) {
+        if (rank == 0 && tid == 0) out[r] = 0;
         return;
     }
-    const double inverse = 1.0 / (double)T;
+    if (!(T > 0.f)) {                                                // the first of the largest
+        u64 best = 0;
+        for_all([&](float x, int i) {
+            const u64 token = x == largest ? token_of(top, lo + i) : 0;
+            best = token > best ? token : best;
+        });
+        best = block_join<true>(best, s);
+        exchange(best, 0, true, all, front);
+        if (rank == 0 && tid == 0) out[r] = index_of(all[0]);
+        return;
+    }
+    // exp(t) for t in -31 .. 0 as 2^(n / 64) exp(z) with n the whole number next to 64 t / ln 2 and |z| <= ln 2 / 128, where the powers up to
+    // z^4 / 24 leave 4e-14; n = 64 e + i, a table has 2^(i / 64), and adding e + 42 to its exponent scales it to whole 2^-42.  Adding 1.5 2^52 and
+    // taking it off rounds to a whole number, which then stands in the low bits.
+    const double per_step = 64.0 / 0.69314718055994530942 / (double)T, step_size = 0.69314718055994530942 / 64.0;
+    const double top_value = (double)largest;
     const float no_weight = NO_WEIGHT * T;
     auto weight = [&](float x) -> u64 {
         if (x == largest) return (u64)ONE;                           // +inf too
         if (!(x > -INFINITY) || largest == INFINITY || largest - x > no_weight) return 0;
-        return (u64)__double2ll_rn(exp(((double)x - (double)largest) * inverse) * ONE);
+        constexpr double WHOLE = 6755399441055744.0;                 // 1.5 2^52
+        const double y = ((double)x - top_value) * per_step, shifted = y + WHOLE;
+        const int whole = __double2loint(shifted);                   // n
+        const double z = (y - (shifted - WHOLE)) * step_size;
+        const double power = s.power[whole & (POWERS - 1)];
+        const double scaled = __hiloint2double(__double2hiint(power) + ((whole >> 6) + 42 << 20), __double2loint(power));
+        const double series = fma(fma(fma(z, 1.0 / 24, 1.0 / 6), z, 0.5), z * z, z);
+        const double w = fma(scaled, series, scaled) + WHOLE;        // exp(z) = 1 + series
+        return (u64)__double_as_longlong(w) & 0x7ffffffffffffull;
     };
     const bool k_on = k > 0 && k < vocab, p_on = p > 0.f && p < 1.f, m_on = least > 0.0;
 
-    // A histogram's step of a logit, larger ones in front.
-    auto step_of = [&](float x, float scale) { return min(BINS - 1, (int)((largest - x) * scale)); };
-    // After all CTAs have counted: the sums of the steps up to the first one where they reach `goal` (of the counts, or `share` of the weights' sum).
-    struct Cut {
-        int step;
-        u64 count_before, count, weight_before, weight, weight_sum;
-    };
-    auto cut_at = [&](bool by_weight, u64 goal, double share) {
-        cluster_barrier();
-        u64 c = 0, w = 0;
-        for (unsigned q = 0; q < ctas; ++q) {
-            c += remote_load(remote(&s.bin_count[tid], q));
-            if (by_weight) w += remote_load64(remote(&s.bin_weight[tid], q));
-        }
-        u64 c_sum = c, w_sum = w;
-        block_scan(c_sum, w_sum, s);
-        u64* const totals = s.weights;                               // free between the lists
-        if (tid == BINS - 1) totals[0] = w_sum;
-        if (tid == 0) s.found = BINS - 1;
-        __syncthreads();
-        const double target = share * (double)totals[0];
-        const bool reached = by_weight ? (double)w_sum >= target && w_sum > 0 : c_sum >= goal;
-        if (reached) atomicMin(&s.found, tid);
-        __syncthreads();
-        if (tid == s.found) {
-            totals[1] = c_sum - c;
-            totals[2] = c;
-            totals[3] = w_sum - w;
-            totals[4] = w;
-        }
-        __syncthreads();
-        const Cut cut = {s.found, totals[1], totals[2], totals[3], totals[4], totals[0]};
-        __syncthreads();
-        return cut;
-    };
-    static_assert(BINS == THREADS, "a thread a step");
+    // ---- the short list, in the first CTA
     auto put_in_list = [&](u64 token) {
         const unsigned place = remote_add(remote(&s.listed, 0), 1);
         if (place < LIST) remote_store(remote(&s.list[place], 0), token);
     };
-
-    // The list's cuts and the draw, by the first CTA.  by_k: top-k is still to be cut, and top-p goes by what that leaves; else by `whole`.
-    auto finish_list = [&](bool by_k, u64 whole) {
-        cluster_barrier();
-        if (rank != 0) return;
-        const int listed = (int)s.listed, padded = power_of_two(listed);
+    // The first token whose running sum passes u times the whole: at least 1, and at most the whole itself.
+    auto goal_of = [&](u64 total) -> u64 {
+        const double asked = (double)u * (double)total;
+        const u64 passed = asked > 0 ? (u64)asked + 1 : 1;
+        return passed < total ? passed : total;
+    };
+    // The list's cuts and the draw.  by_k: top-k is still to be cut, and top-p goes by what that leaves; else by `whole`.
+    auto draw_from_list = [&](int listed, bool by_k, u64 whole) {
+        const int kept_k = by_k ? min(k, listed) : listed;
+        if (listed <= SHORT) {                                       // places by counting: four threads a token
+            static_assert(THREADS == 4 * SHORT, "four threads a token");
+            const int e = tid / 4, part = tid % 4;
+            if (tid < listed) s.weights[tid] = weight(value_of((unsigned)(s.list[tid] >> 32)));
+            __syncthreads();
+            const u64 token = e < listed ? s.list[e] : 0, w = e < listed ? s.weights[e] : 0;
+            int place = 0;
+            u64 before = 0;
+            for (int j = part; j < listed; j += 4) {
+                const bool ahead = s.list[j] > token;
+                place += ahead;
+                before += ahead ? s.weights[j] : 0;
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o *= 2) {
+                place += __shfl_xor_sync(0xffffffffu, place, o);
+                before += __shfl_xor_sync(0xffffffffu, before, o);
+            }
+            const bool in_k = e < listed && place < kept_k;
+            if (in_k && place == kept_k - 1 && part == 0) s.pair[0] = before + w;      // the weights of all k
+            __syncthreads();
+            if (by_k) whole = s.pair[0];
+            const bool kept = in_k && (place == 0 || !p_on || (double)before < (double)p * (double)whole) && (double)w >= least;
+            if (part == 0 && e < listed) s.weights[e] = kept ? w : 0;
+            __syncthreads();
+            u64 upto = 0, total = 0;
+            for (int j = part; j < listed; j += 4) {
+                const u64 v = s.weights[j];
+                total += v;
+                upto += (unsigned)s.list[j] >= (unsigned)token ? v : 0;                // lower indices have larger low halves
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o *= 2) {
+                upto += __shfl_xor_sync(0xffffffffu, upto, o);
+                total += __shfl_xor_sync(0xffffffffu, total, o);
+            }
+            const u64 goal = goal_of(total);
+            if (kept && part == 0 && upto >= goal && upto - w < goal) out[r] = index_of(token);
+            return;
+        }
+        const int padded = power_of_two(listed);
         for (int i = listed + tid; i < padded; i += THREADS) s.list[i] = 0;
         sort_descending(s.list, padded);
-        const int kept_k = by_k ? min(k, listed) : listed;
         u64 w[2], c[2];                                              // a thread has two neighbours of the list
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int i = 2 * tid + h;
             w[h] = i < kept_k ? weight(value_of((unsigned)(s.list[i] >> 32))) : 0;
+            if (i < kept_k) s.weights[i] = w[h];
         }
         u64 sum = w[0] + w[1], unused = 0;
         block_scan(sum, unused, s);
         c[0] = sum - w[0] - w[1];
         c[1] = sum - w[1];
+        if (tid == THREADS - 1) s.pair[0] = sum;
         __syncthreads();
-        if (tid == THREADS - 1) s.warp_a[0] = sum;
-        __syncthreads();
-        if (by_k) whole = s.warp_a[0];
+        if (by_k) whole = s.pair[0];
         const double target = (double)p * (double)whole;
-        int mine = 0;
+        u64 mine = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int i = 2 * tid + h;
             mine += i < kept_k && (i == 0 || !p_on || (double)c[h] < target) && (double)w[h] >= least;
-            if (i < kept_k) s.weights[i] = w[h];
         }
-        u64 kept_sum = mine;
-        unused = 0;
-        block_join<false>(kept_sum, unused, s);
-        const int kept = max(1, (int)kept_sum), places = power_of_two(kept);
+        const int kept = max(1, (int)block_join<false>(mine, s)), places = power_of_two(kept);
         // in the order of the indices: sorted by (all ones - index), with the place in the list beside it
         for (int i = tid; i < places; i += THREADS) s.list[i] = i < kept ? (s.list[i] & 0xffffffffu) << 32 | (unsigned)i : 0;
         sort_descending(s.list, places);
@@ -303,63 +366,133 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         sum = w[0] + w[1];
         unused = 0;
         block_scan(sum, unused, s);
+        if (tid == THREADS - 1) s.pair[1] = sum;
         __syncthreads();
-        if (tid == THREADS - 1) s.warp_a[0] = sum;
-        __syncthreads();
-        const u64 total = s.warp_a[0];
-        const double asked = (double)u * (double)total;
-        const u64 passed = asked > 0 ? (u64)asked + 1 : 1, goal = passed < total ? passed : total;
+        const u64 goal = goal_of(s.pair[1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const u64 upto = h ? sum : sum - w[1];
             if (upto >= goal && upto - w[h] < goal) out[r] = index_of(s.list[2 * tid + h] >> 32);
         }
     };
+    // After the candidates have been put in the list: whether that was all (the draw is done then), or there are too many, which the first CTA tells
+    // the others while it goes on.
+    auto finish_list = [&](bool by_k, u64 whole) {
+        cluster_barrier();
+        bool done = true;
+        if (rank == 0) {
+            const unsigned listed = s.listed;
+            done = listed <= LIST;
+            if (tid < (int)ctas) remote_store(remote(&s.slot[turn][0][0], tid), done);
+            asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+            if (done) draw_from_list((int)listed, by_k, whole);
+            asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+            if (tid == 0) s.listed = 0;
+        } else {
+            cluster_barrier();
+            done = s.slot[turn][0][0] != 0;
+        }
+        turn ^= 1;
+        return done;
+    };
+
+    // ---- histograms: a logit's step, larger ones in front
+    auto step_of = [&](float x, float scale) { return min(BINS - 1, (int)((largest - x) * scale)); };
+    auto add_weight = [&](int step, u64 w) {
+        atomicAdd(&s.bin_count[step], 1u);
+#pragma unroll
+        for (int h = 0; h < LIMBS; ++h) {
+            const unsigned limb = (unsigned)(w >> (LIMB_BITS * h)) & (h < LIMBS - 1 ? (1u << LIMB_BITS) - 1 : ~0u);
+            if (limb) atomicAdd(&s.bin_weight[h][step], limb);
+        }
+    };
+    struct Cut {
+        int step;
+        u64 count_before, count, weight_before, weight_sum;
+    };
+    // After all CTAs have counted: the first step where `before` and the sums up to it reach the goal, which is a count, or a weight: `share` of all of
+    // the histogram's (weight_goal < 0), or weight_goal.
+    auto cut_at = [&](bool by_weight, u64 before, u64 goal, double share, double weight_goal) {
+        __syncthreads();
+        cluster_barrier();
+        const u64 c = sum_of_loads<8, unsigned>(ctas, [&](unsigned q) { return remote_load(remote(&s.bin_count[tid], q)); });
+        u64 w = 0;
+        if (by_weight) {
+#pragma unroll
+            for (int h = 0; h < LIMBS; ++h) {
+                u64 sum = 0;                                         // a limb's sums over 16 CTAs pass 32 bits
+                unsigned v[8];
+                for (unsigned q0 = 0; q0 < ctas; q0 += 8) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = q0 + i < ctas ? remote_load(remote(&s.bin_weight[h][tid], q0 + i)) : 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum += v[i];
+                }
+                w += sum << (LIMB_BITS * h);
+            }
+        }
+        u64 c_sum = c, w_sum = w;
+        block_scan(c_sum, w_sum, s);
+        if (tid == BINS - 1) s.pair[0] = w_sum;
+        if (tid == 0) s.found = BINS - 1;
+        __syncthreads();
+        const u64 weight_sum = s.pair[0];
+        if (weight_goal < 0) weight_goal = share * (double)weight_sum;
+        if (by_weight ? w_sum > 0 && (double)(before + w_sum) >= weight_goal : before + c_sum >= goal) atomicMin(&s.found, tid);
+        __syncthreads();
+        if (tid == s.found) {
+            s.weights[0] = c_sum - c;
+            s.weights[1] = c;
+            s.weights[2] = w_sum - w;
+        }
+        __syncthreads();
+        const Cut cut = {s.found, s.weights[0], s.weights[1], s.weights[2], weight_sum};
+        __syncthreads();
+        return cut;
+    };
+    const float count_scale = BINS / COUNT_RANGE, weight_scale = BINS / (WEIGHT_RANGE * T);
 
     // ---- what is kept as a short list
-    const float count_scale = BINS / COUNT_RANGE, weight_scale = BINS / (WEIGHT_RANGE * T);
-    Cut cut = {};
-    if (k_on ? k <= LIST : !(p_on || m_on) ? vocab <= LIST : false) {
-        if (vocab > LIST) {
-            for (int i = tid; i < n; i += THREADS) {
-                const float x = at(i);
-                if (x > -INFINITY) atomicAdd(&s.bin_count[step_of(x, count_scale)], 1u);
-            }
-            __syncthreads();
-            cut = cut_at(false, k, 0.0);
+    bool counted = false;                                            // the histograms have been used
+    if (k_on && vocab <= LIST && 4 * k > THREADS) {
+        for_all([&](float x, int i) {
+            if (x > -INFINITY) put_in_list(token_of(key_of(x), lo + i));
+        });
+        finish_list(true, 0);
+        return;
+    } else if (k_on && k <= LIST && 4ll * k <= (long long)ctas * THREADS) {
+        // the k-th largest of the threads' maxima is no larger than the k-th largest logit
+        if (mine_most > -INFINITY) atomicAdd(&s.bin_count[step_of(mine_most, count_scale)], 1u);
+        counted = true;
+        const Cut cut = cut_at(false, 0, k, 0.0, 0.0);
+        if (cut.count_before + cut.count >= (u64)k) {
+            for_all([&](float x, int i) {
+                if (x > -INFINITY && step_of(x, count_scale) <= cut.step) put_in_list(token_of(key_of(x), lo + i));
+            });
+            if (finish_list(true, 0)) return;
         }
-        if (vocab <= LIST || cut.count_before + cut.count <= LIST) {
-            for (int i = tid; i < n; i += THREADS) {
-                const float x = at(i);
-                if (x > -INFINITY && (vocab <= LIST || step_of(x, count_scale) <= cut.step)) put_in_list(token_of(key_of(x), lo + i));
-            }
-            finish_list(k_on, 0);
-            return;
+    } else if (!k_on && (m_on || (vocab <= LIST && !p_on))) {
+        u64 whole = 0;
+        if (p_on) {
+            u64 sum = 0;
+            for_all([&](float x, int) { sum += weight(x); });
+            exchange(block_join<false>(sum, s), 0, false, all, front);
+            whole = all[0];
         }
-    } else if (!k_on && m_on) {
-        u64 count = 0, sum = 0;
-        for (int i = tid; i < n; i += THREADS) {
-            const u64 w = weight(at(i));
-            count += (double)w >= least;
-            sum += w;
-        }
-        block_join<false>(count, sum, s);
-        exchange(count, sum, false, all, front);
-        if (all[0] <= LIST) {
-            const u64 whole = all[1];
-            for (int i = tid; i < n; i += THREADS) {
-                const float x = at(i);
-                if ((double)weight(x) >= least) put_in_list(token_of(key_of(x), lo + i));
-            }
-            finish_list(false, whole);
-            return;
-        }
+        // what is far below min-p's border (by more than a float's rounding moves it) needs no weight
+        const float border = m_on ? largest + T * (logf(fminf(min_p[r], 1.f)) - 1e-3f) - 1e-5f * fabsf(largest) : -INFINITY;
+        for_all([&](float x, int i) {
+            if (x < border || !(x > -INFINITY)) return;
+            const u64 w = weight(x);
+            if (w > 0 && (double)w >= least) put_in_list(token_of(key_of(x), lo + i));
+        });
+        if (finish_list(false, whole)) return;
     }
 
     // ---- the last token that top-k and top-p keep: those from `last` on stay
     u64 last = (u64)(MINUS_INFINITY_KEY + 1) << 32;
     // Narrows a cut down to that token: of the tokens in the cut's step the first ones until before + theirs reach the goal.
-    auto narrow = [&](bool by_weight, float scale, u64 count_goal, double weight_goal) {
+    auto narrow = [&](bool by_weight, float scale, Cut cut, u64 count_goal, double weight_goal) {
         u64 before = by_weight ? cut.weight_before : cut.count_before, inside = cut.count;
         unsigned high_key = 0, low_key = 0;                          // of the step's tokens, once it has been refined
         bool by_step = true;
@@ -369,17 +502,16 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         };
         while (inside > LIST) {
             if (by_step) {                                           // the step's tokens are those of a run of keys
-                u64 a = 0, b = 0;
-                for (int i = tid; i < n; i += THREADS) {
-                    const float x = at(i);
+                unsigned a = 0, b = 0;
+                for_all([&](float x, int i) {
                     const unsigned key = key_of(x);
                     if (is_inside(x, token_of(key, lo + i))) {
-                        a = key > a ? key : a;
-                        b = ~key > (unsigned)b ? ~key : b;
+                        a = max(a, key);
+                        b = max(b, ~key);
                     }
-                }
-                block_join<true>(a, b, s);
-                exchange(a, b, true, all, front);
+                });
+                const u64 most_key = block_join<true>(a, s), most_other = block_join<true>(b, s);
+                exchange(most_key, most_other, true, all, front);
                 high_key = (unsigned)all[0];
                 low_key = ~(unsigned)all[1];
                 by_step = false;
@@ -387,39 +519,19 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
             if (high_key == low_key) break;
             const int shift = max(0, 32 - __clz(high_key - low_key) - 9);      // at most BINS steps of 2^shift keys
             cluster_barrier();                                       // the last histogram has been read
-            s.bin_count[tid] = 0;
-            s.bin_weight[tid] = 0;
+            clear_bins();
             __syncthreads();
-            for (int i = tid; i < n; i += THREADS) {
-                const float x = at(i);
+            for_all([&](float x, int i) {
                 const unsigned key = key_of(x);
-                if (!is_inside(x, token_of(key, lo + i))) continue;
-                atomicAdd(&s.bin_count[(high_key - key) >> shift], 1u);
-                if (by_weight) atomicAdd(&s.bin_weight[(high_key - key) >> shift], weight(x));
-            }
-            __syncthreads();
-            cluster_barrier();
-            u64 c = 0, w = 0;
-            for (unsigned q = 0; q < ctas; ++q) {
-                c += remote_load(remote(&s.bin_count[tid], q));
-                if (by_weight) w += remote_load64(remote(&s.bin_weight[tid], q));
-            }
-            u64 c_sum = c, w_sum = w;
-            block_scan(c_sum, w_sum, s);
-            if (tid == 0) s.found = BINS - 1;
-            __syncthreads();
-            if (by_weight ? (double)(before + w_sum) >= weight_goal : before + c_sum >= count_goal) atomicMin(&s.found, tid);
-            __syncthreads();
-            if (tid == s.found) {
-                s.weights[0] = by_weight ? w_sum - w : c_sum - c;
-                s.weights[1] = c;
-            }
-            __syncthreads();
-            before += s.weights[0];
-            inside = s.weights[1];
-            high_key -= (unsigned)s.found << shift;
-            if (high_key - low_key >> shift) low_key = high_key - ((1u << shift) - 1);
-            __syncthreads();
+                if (!is_inside(x, token_of(key, lo + i))) return;
+                if (by_weight) add_weight((high_key - key) >> shift, weight(x));
+                else atomicAdd(&s.bin_count[(high_key - key) >> shift], 1u);
+            });
+            const Cut inner = cut_at(by_weight, before, count_goal, 0.0, weight_goal);
+            before += by_weight ? inner.weight_before : inner.count_before;
+            inside = inner.count;
+            high_key -= (unsigned)inner.step << shift;
+            if ((high_key - low_key) >> shift) low_key = high_key - ((1u << shift) - 1);
         }
         u64 result = 0;
         if (inside > LIST) {                                         // equal ones: as many as it takes, the first in the order of the indices
@@ -430,25 +542,21 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
             auto counts = [&](int i) { return key_of(at(i)) == high_key && token_of(high_key, lo + i) >= last; };
             u64 mine = 0, unused = 0;
             for (int i = from; i < to; ++i) mine += counts(i);
-            u64 upto = mine, block = mine;
+            u64 upto = mine;
             block_scan(upto, unused, s);
-            unused = 0;
-            block_join<false>(block, unused, s);
-            exchange(block, 0, false, all, front);
-            upto += front[0];
+            exchange(block_join<false>(mine, s), 0, false, all, front);
+            upto += front;
             if (upto >= take && upto - mine < take) {                // one thread of the row's
-                u64 at_token = upto - mine;
+                u64 so_far = upto - mine;
                 for (int i = from; i < to; ++i)
-                    if (counts(i) && ++at_token == take) result = token_of(high_key, lo + i);
+                    if (counts(i) && ++so_far == take) result = token_of(high_key, lo + i);
             }
-            unused = 0;
-            block_join<true>(result, unused, s);
+            result = block_join<true>(result, s);
         } else {
-            for (int i = tid; i < n; i += THREADS) {
-                const float x = at(i);
+            for_all([&](float x, int i) {
                 const u64 token = token_of(key_of(x), lo + i);
                 if (is_inside(x, token)) put_in_list(token);
-            }
+            });
             cluster_barrier();
             if (rank == 0) {
                 const int listed = (int)s.listed, padded = power_of_two(listed);
@@ -468,95 +576,89 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
                     const u64 reach = before + (h ? sum - v[1] : sum - v[0] - v[1]);
                     mine += i < listed && (i == 0 || (by_weight ? (double)reach < weight_goal : reach < count_goal));
                 }
-                unused = 0;
-                block_join<false>(mine, unused, s);
-                result = s.list[max(1, (int)mine) - 1];
+                result = s.list[max(1, (int)block_join<false>(mine, s)) - 1];
                 if (tid == 0) s.listed = 0;
             }
         }
         exchange(result, 0, true, all, front);
         last = all[0];
     };
-    auto clear_bins = [&]() {
-        cluster_barrier();
-        s.bin_count[tid] = 0;
-        s.bin_weight[tid] = 0;
-        __syncthreads();
+    // a histogram over steps, from nothing
+    auto start_bins = [&]() {
+        if (counted) {
+            cluster_barrier();                                       // the last one has been read
+            clear_bins();
+            __syncthreads();
+        }
+        counted = true;
     };
     if (k_on) {
-        if (k > LIST) {                                              // else it is there already
-            for (int i = tid; i < n; i += THREADS) {
-                const float x = at(i);
-                if (x > -INFINITY) atomicAdd(&s.bin_count[step_of(x, count_scale)], 1u);
-            }
-            __syncthreads();
-            cut = cut_at(false, k, 0.0);
-        }
-        if (cut.count_before + cut.count >= (u64)k) narrow(false, count_scale, k, 0.0);      // else there are no more than k
-        if (p_on) clear_bins();
+        start_bins();
+        for_all([&](float x, int) {
+            if (x > -INFINITY) atomicAdd(&s.bin_count[step_of(x, count_scale)], 1u);
+        });
+        const Cut cut = cut_at(false, 0, k, 0.0, 0.0);
+        if (cut.count_before + cut.count >= (u64)k) narrow(false, count_scale, cut, k, 0.0);      // else there are no more than k
     }
     if (p_on) {
-        for (int i = tid; i < n; i += THREADS) {
-            const float x = at(i);
-            if (token_of(key_of(x), lo + i) < last) continue;
+        start_bins();
+        for_all([&](float x, int i) {
+            if (token_of(key_of(x), lo + i) < last) return;
             const u64 w = weight(x);
-            if (w == 0) continue;
-            const int b = step_of(x, weight_scale);
-            atomicAdd(&s.bin_count[b], 1u);
-            atomicAdd(&s.bin_weight[b], w);
-        }
-        __syncthreads();
-        cut = cut_at(true, 0, (double)p);
+            if (w > 0) add_weight(step_of(x, weight_scale), w);
+        });
+        const Cut cut = cut_at(true, 0, 0, (double)p, -1.0);
         if (cut.count_before + cut.count <= LIST) {
-            for (int i = tid; i < n; i += THREADS) {
-                const float x = at(i);
+            for_all([&](float x, int i) {
                 const u64 token = token_of(key_of(x), lo + i);
                 if (token >= last && step_of(x, weight_scale) <= cut.step && weight(x) > 0) put_in_list(token);
-            }
+            });
             finish_list(false, cut.weight_sum);
             return;
         }
-        narrow(true, weight_scale, 0, (double)p * (double)cut.weight_sum);
+        narrow(true, weight_scale, cut, 0, (double)p * (double)cut.weight_sum);
     }
 
-    // ---- the draw over the slices: a warp has a run of tokens, 32 at a time
+    // ---- the draw over the slices: a warp has a run of tokens
     const int run = ((n + WARPS - 1) / WARPS + 31) & ~31, from = min(n, warp * run), to = min(n, from + run);
     auto kept_weight = [&](int i) -> u64 {
-        const float x = i < to ? at(i) : NAN;
+        const float x = at(i);
         if (token_of(key_of(x), lo + i) < last) return 0;
         const u64 w = weight(x);
         return (double)w >= least ? w : 0;
     };
-    u64 mass = 0, unused = 0;
-    for (int i = from; i < to; i += 32) mass += kept_weight(i + lane);
-    u64 scan = mass;
-    block_scan(scan, unused, s);
-    const u64 before_warp = __shfl_sync(0xffffffffu, scan - mass, 0), upto_warp = __shfl_sync(0xffffffffu, scan, 31);
-    u64 block_mass = mass;
-    unused = 0;
-    block_join<false>(block_mass, unused, s);
-    exchange(block_mass, 0, false, all, front);
-    // the running sum has to pass u times the whole: at least 1, and at most the whole itself
-    const u64 total = all[0];
-    const double asked = (double)u * (double)total;
-    const u64 passed = asked > 0 ? (u64)asked + 1 : 1, goal = passed < total ? passed : total;
-    u64 upto = front[0] + before_warp;
-    if (goal > upto && goal <= front[0] + upto_warp) {
-        for (int i = from; i < to; i += 32) {
-            u64 w = kept_weight(i + lane);
+    u64 mass = 0;
+    for (int i = from + lane; i < to; i += 32) mass += kept_weight(i);
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const u64 x = __shfl_up_sync(0xffffffffu, w, o);
-                if (lane >= o) w += x;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, upto + w >= goal);
-            if (past) {
-                if (lane == 0) out[r] = lo + i + __ffs(past) - 1;
+    for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+    __syncthreads();
+    if (lane == 0) s.warp_b[warp] = mass;
+    __syncthreads();
+    u64 block_mass = 0;
+#pragma unroll
+    for (int q = 0; q < WARPS; ++q) block_mass += s.warp_b[q];
+    exchange(block_mass, 0, false, all, front);
+    const u64 goal = goal_of(all[0]);
+    if (goal <= front || goal > front + block_mass) return;
+    // it is in this CTA: the warp's run with the draw, a few tokens a thread
+    u64 upto = front;
+    int q = 0;
+    while (q < WARPS - 1 && upto + s.warp_b[q] < goal) upto += s.warp_b[q++];
+    const int first = min(n, q * run), end = min(n, first + run), each = (end - first + THREADS - 1) / THREADS;
+    const int mine_from = min(end, first + tid * each), mine_to = min(end, mine_from + each);
+    u64 mine = 0, unused = 0;
+    for (int i = mine_from; i < mine_to; ++i) mine += kept_weight(i);
+    u64 scan = mine;
+    block_scan(scan, unused, s);                                     // (it writes warp_b behind a barrier)
+    upto += scan - mine;
+    if (upto < goal && upto + mine >= goal)
+        for (int i = mine_from; i < mine_to; ++i) {
+            upto += kept_weight(i);
+            if (upto >= goal) {
+                out[r] = lo + i;
                 break;
             }
-            upto += __shfl_sync(0xffffffffu, w, 31);
         }
-    }
 }
 
 template <bool RESIDENT>
