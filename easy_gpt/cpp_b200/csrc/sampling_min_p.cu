@@ -15,7 +15,7 @@
 // A row is a cluster's, up to 16 CTAs with a slice of it each in shared memory, so that it is read once however often it is passed over.
 // What most rows come to is a short list: the k largest, or what min-p or top-p leave.  The tokens that can be among those, at most 1,024, go to the
 // first CTA, which puts them in order and has all three cuts and the draw among them.  With top-k they are those that are not below the k-th
-// largest of the threads' own maxima; with min-p its threshold says it; with top-p alone a histogram over 512 equal steps below the largest logit, of
+// largest of the maxima of at least 2 k groups of tokens; with min-p its threshold says it; with top-p alone a histogram over 512 equal steps below the largest logit, of
 // counts and weights.  A row that keeps more finds the last token of top-k's and top-p's runs by such histograms, refined until a step's tokens
 // are a short list (or all equal); then every CTA sums what is kept of its slice, and the one in whose part the draw falls finds it.
 //
@@ -26,9 +26,9 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = 1024, SHORT = 128, MOST_CTAS = 16;
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = 1024, SHORT = 128, MOST_CTAS = 16, GROUPS = 1024;
 constexpr int LIMBS = 3, LIMB_BITS = 14;                             // of a weight, at most 2^42: sums of 2^17 of them stay below 2^32
-constexpr int SLICE = 20480, MOST_SLICE = 51200;                     // logits of a slice: two CTAs an SM, and what fits at all
+constexpr int SLICE = 20480, MOST_SLICE = 50176;                     // logits of a slice: two CTAs an SM, and what fits at all
 constexpr double ONE = 4398046511104.0;                              // 2^42: with 2^20 tokens sums stay below 2^62
 constexpr int MOST_TOKENS = 1 << 20;
 constexpr float COUNT_RANGE = 32.f, WEIGHT_RANGE = 30.f;             // what a histogram's steps span below the largest logit; of weights in units of T
@@ -65,6 +65,8 @@ __device__ __forceinline__ unsigned remote(const void* mine, unsigned rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
     return a;
 }
+__device__ __forceinline__ void remote_store(unsigned at, u64 a, u64 b) { asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(at), "l"(a), "l"(b) : "memory"); }
+__device__ __forceinline__ void remote_store(unsigned at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 __device__ __forceinline__ void remote_store(unsigned at, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
 __device__ __forceinline__ unsigned remote_load(unsigned at) {
     unsigned v;
@@ -80,29 +82,21 @@ __device__ __forceinline__ unsigned remote_add(unsigned at, unsigned n) {
 // 2^(i / 64), filled in by the first threads
 constexpr int POWERS = 64;
 
-template <int N, typename T, typename F>
-__device__ __forceinline__ T sum_of_loads(unsigned ctas, F load) {
-    T sum = 0, v[N];
-    for (unsigned q0 = 0; q0 < ctas; q0 += N) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = q0 + i < ctas ? load(q0 + i) : 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) sum += v[i];
-    }
-    return sum;
-}
-
 struct Shared {
     double power[POWERS];
     __align__(16) u64 slot[2][MOST_CTAS][2];                                       // what the CTAs tell each other, in turn
     u64 warp_a[WARPS], warp_b[WARPS];
-    u64 list[LIST], weights[LIST];
+    u64 list[LIST];
+    __align__(16) u64 weights[LIST];                                 // of the list; a histogram's sums over the CTAs, count and weight a step
+    float group_most[GROUPS];
     unsigned bin_weight[LIMBS][BINS], bin_count[BINS];
     unsigned listed;
     int found;
     float floats[WARPS];
-    u64 pair[2];
+    u64 pair[4];
 };
+
+static_assert(sizeof(Shared) + MOST_SLICE * 4 <= 227 * 1024, "shared memory of a CTA");
 
 // the sum (or the maximum) over the CTA
 template <bool MAX>
@@ -139,16 +133,21 @@ __device__ __forceinline__ void block_scan(u64& a, u64& b, Shared& s) {
     b += __shfl_sync(0xffffffffu, y, 0);
 }
 
-// descending, n a power of two
+// Descending, n a power of two up to 2 THREADS.  A thread has a pair of every stage; pairs no more than 32 apart are within a warp's 64 places, and
+// stages of those need no barrier of the CTA.
 __device__ __forceinline__ void sort_descending(u64* list, int n) {
+    const int i = threadIdx.x;
+    __syncthreads();
     for (int size = 2; size <= n; size *= 2)
         for (int step = size / 2; step > 0; step /= 2) {
-            __syncthreads();
-            for (int i = threadIdx.x; i < n / 2; i += THREADS) {
+            if (i < n / 2) {
                 const int a = 2 * i - (i & (step - 1)), b = a + step;
                 const u64 x = list[a], y = list[b];
                 if ((x < y) == ((a & size) == 0)) list[a] = y, list[b] = x;
             }
+            const int next = step > 1 ? step / 2 : size;             // the next stage's step
+            if (step > 32 || next > 32) __syncthreads();
+            else __syncwarp();
         }
     __syncthreads();
 }
@@ -186,37 +185,36 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;\n" ::: "memory");
         __syncthreads();
     }
-    // f(x, i) for the thread's tokens, four at a time
-    auto for_all = [&](auto f) {
+    // f(x, i) for the thread's tokens of from .. to - 1 (a multiple of 4), `threads` of them sharing these; several at a time, so that
+    // their chains of operations overlap.  Tokens below `least_logit` may be left out.
+    auto for_some = [&](int from, int to, int thread, int threads, float least_logit, auto f) {
         if constexpr (RESIDENT) {
-            for (int q = tid; q < n / 4; q += THREADS) {
-                const float4 v = reinterpret_cast<const float4*>(slice_s)[q];
-                f(v.x, 4 * q);
-                f(v.y, 4 * q + 1);
-                f(v.z, 4 * q + 2);
-                f(v.w, 4 * q + 3);
+            for (int i = from + 4 * thread; i + 3 < to; i += 4 * threads) {
+                const float4 v = *reinterpret_cast<const float4*>(slice_s + i);
+                if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) < least_logit) continue;
+                f(v.x, i);
+                f(v.y, i + 1);
+                f(v.z, i + 2);
+                f(v.w, i + 3);
             }
-            for (int i = n / 4 * 4 + tid; i < n; i += THREADS) f(slice_s[i], i);
+            for (int i = from + (to - from) / 4 * 4 + thread; i < to; i += threads) f(slice_s[i], i);
         } else {
-            for (int i = tid; i < n; i += THREADS) f(__ldg(row + i), i);
+            for (int i = from + thread; i < to; i += threads) f(__ldg(row + i), i);
         }
     };
+    auto for_all = [&](float least_logit, auto f) { for_some(0, n, tid, THREADS, least_logit, f); };
     auto at = [&](int i) { return RESIDENT ? slice_s[i] : __ldg(row + i); };
 
     int turn = 0;
     // every CTA's pair, after a barrier: what the CTAs in front of this one have (front), and all of them
     auto exchange = [&](u64 a, u64 b, bool max, u64 (&all)[2], u64& front) {
-        if (tid < (int)ctas) {
-            const unsigned to = remote(&s.slot[turn][rank][0], tid);
-            remote_store(to, a);
-            remote_store(to + 8, b);
-        }
+        if (tid < (int)ctas) remote_store(remote(&s.slot[turn][rank][0], tid), a, b);
         cluster_barrier();
         all[0] = all[1] = front = 0;
 #pragma unroll
         for (unsigned c = 0; c < MOST_CTAS; ++c) {
+            if (c >= ctas) break;
             const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&s.slot[turn][c][0]);
-            if (c >= ctas) continue;
             all[0] = max ? (v.x > all[0] ? v.x : all[0]) : all[0] + v.x;
             all[1] = max ? (v.y > all[1] ? v.y : all[1]) : all[1] + v.y;
             if (c < rank) front += v.x;
@@ -225,18 +223,28 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     };
     u64 all[2], front;
 
-    // ---- the largest logit, and every thread's
-    float mine_most = -INFINITY;                                     // NaN is passed over
-    for_all([&](float x, int) { mine_most = fmaxf(mine_most, x); });
-    float most = mine_most;
+    // ---- the largest logit; with top-k that of groups of 1 to 32 threads too, which every CTA gets
+    const bool k_on = k > 0 && k < vocab, p_on = p > 0.f && p < 1.f, m_on = least > 0.0;
+    float most = -INFINITY;                                          // NaN is passed over
+    for_all(-INFINITY, [&](float x, int) { most = fmaxf(most, x); });
+    int width = 32;
+    while (width > 1 && (int)ctas * THREADS / width < 2 * min(k, GROUPS)) width /= 2;
+    const int groups = (int)ctas * THREADS / width;
+    const bool grouped = k_on && groups >= 2 * k && groups <= GROUPS;
+    float group = most;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    for (int o = 1; o < 32; o *= 2) {
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (2 * o == width) group = most;
+    }
     if (lane == 0) s.floats[warp] = most;
     __syncthreads();
     most = s.floats[lane & (WARPS - 1)];
 #pragma unroll
     for (int o = WARPS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+    if (grouped && tid % width == 0)
+        for (unsigned q = 0; q < ctas; ++q) remote_store(remote(&s.group_most[(rank * THREADS + tid) / width], q), group);
     exchange(key_of(most), 0, true, all, front);
     const unsigned top = (unsigned)all[0];
     const float largest = value_of(top);
@@ -246,7 +254,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     }
     if (!(T > 0.f)) {                                                // the first of the largest
         u64 best = 0;
-        for_all([&](float x, int i) {
+        for_all(largest, [&](float x, int i) {
             const u64 token = x == largest ? token_of(top, lo + i) : 0;
             best = token > best ? token : best;
         });
@@ -262,8 +270,6 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     const double top_value = (double)largest;
     const float no_weight = NO_WEIGHT * T;
     auto weight = [&](float x) -> u64 {
-        if (x == largest) return (u64)ONE;                           // +inf too
-        if (!(x > -INFINITY) || largest == INFINITY || largest - x > no_weight) return 0;
         constexpr double WHOLE = 6755399441055744.0;                 // 1.5 2^52
         const double y = ((double)x - top_value) * per_step, shifted = y + WHOLE;
         const int whole = __double2loint(shifted);                   // n
@@ -272,9 +278,12 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         const double scaled = __hiloint2double(__double2hiint(power) + ((whole >> 6) + 42 << 20), __double2loint(power));
         const double series = fma(fma(fma(z, 1.0 / 24, 1.0 / 6), z, 0.5), z * z, z);
         const double w = fma(scaled, series, scaled) + WHOLE;        // exp(z) = 1 + series
-        return (u64)__double_as_longlong(w) & 0x7ffffffffffffull;
+        const u64 found = (u64)__double_as_longlong(w) & 0x7ffffffffffffull;
+        // (no branches, so that several tokens' chains overlap) with +inf the largest, +inf alone has a weight; NaN and -inf have none
+        const bool none = !(x > -INFINITY) || largest == INFINITY || largest - x > no_weight;
+        return x == largest ? (u64)ONE : none ? 0 : found;
     };
-    const bool k_on = k > 0 && k < vocab, p_on = p > 0.f && p < 1.f, m_on = least > 0.0;
+    const float weighty = largest < INFINITY ? largest - no_weight * 1.0001f - 1e-5f * fabsf(largest) : largest;      // nothing below it has a weight
 
     // ---- the short list, in the first CTA
     auto put_in_list = [&](u64 token) {
@@ -383,7 +392,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         if (rank == 0) {
             const unsigned listed = s.listed;
             done = listed <= LIST;
-            if (tid < (int)ctas) remote_store(remote(&s.slot[turn][0][0], tid), done);
+            if (tid < (int)ctas) remote_store(remote(&s.slot[turn][0][0], tid), (u64)done);
             asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
             if (done) draw_from_list((int)listed, by_k, whole);
             asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
@@ -415,22 +424,24 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     auto cut_at = [&](bool by_weight, u64 before, u64 goal, double share, double weight_goal) {
         __syncthreads();
         cluster_barrier();
-        const u64 c = sum_of_loads<8, unsigned>(ctas, [&](unsigned q) { return remote_load(remote(&s.bin_count[tid], q)); });
-        u64 w = 0;
-        if (by_weight) {
+        {   // every CTA adds up its share of the steps, a lane a CTA's part of a step, and each of these lanes tells one CTA the sum
+            const int step = (int)rank * (BINS / (int)ctas) + tid / (int)ctas, of = tid % (int)ctas;
+            u64 count = remote_load(remote(&s.bin_count[step], of)), weight = 0;
+            if (by_weight) {
+                unsigned v[LIMBS];
 #pragma unroll
-            for (int h = 0; h < LIMBS; ++h) {
-                u64 sum = 0;                                         // a limb's sums over 16 CTAs pass 32 bits
-                unsigned v[8];
-                for (unsigned q0 = 0; q0 < ctas; q0 += 8) {
+                for (int h = 0; h < LIMBS; ++h) v[h] = remote_load(remote(&s.bin_weight[h][step], of));
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = q0 + i < ctas ? remote_load(remote(&s.bin_weight[h][tid], q0 + i)) : 0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sum += v[i];
-                }
-                w += sum << (LIMB_BITS * h);
+                for (int h = 0; h < LIMBS; ++h) weight += (u64)v[h] << (LIMB_BITS * h);
             }
+            for (unsigned o = 1; o < ctas; o *= 2) {
+                count += __shfl_xor_sync(0xffffffffu, count, o);
+                weight += __shfl_xor_sync(0xffffffffu, weight, o);
+            }
+            remote_store(remote(&s.weights[2 * step], of), count, weight);
         }
+        cluster_barrier();                                           // the histograms may be cleared now
+        const u64 c = s.weights[2 * tid], w = s.weights[2 * tid + 1];
         u64 c_sum = c, w_sum = w;
         block_scan(c_sum, w_sum, s);
         if (tid == BINS - 1) s.pair[0] = w_sum;
@@ -441,47 +452,67 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         if (by_weight ? w_sum > 0 && (double)(before + w_sum) >= weight_goal : before + c_sum >= goal) atomicMin(&s.found, tid);
         __syncthreads();
         if (tid == s.found) {
-            s.weights[0] = c_sum - c;
-            s.weights[1] = c;
-            s.weights[2] = w_sum - w;
+            s.pair[1] = c_sum - c;
+            s.pair[2] = c;
+            s.pair[3] = w_sum - w;
         }
         __syncthreads();
-        const Cut cut = {s.found, s.weights[0], s.weights[1], s.weights[2], weight_sum};
+        const Cut cut = {s.found, s.pair[1], s.pair[2], s.pair[3], weight_sum};
         __syncthreads();
         return cut;
     };
     const float count_scale = BINS / COUNT_RANGE, weight_scale = BINS / (WEIGHT_RANGE * T);
 
     // ---- what is kept as a short list
-    bool counted = false;                                            // the histograms have been used
-    if (k_on && vocab <= LIST && 4 * k > THREADS) {
-        for_all([&](float x, int i) {
+    if (k_on && vocab <= LIST && !grouped) {
+        for_all(-INFINITY, [&](float x, int i) {
             if (x > -INFINITY) put_in_list(token_of(key_of(x), lo + i));
         });
         finish_list(true, 0);
         return;
-    } else if (k_on && k <= LIST && 4ll * k <= (long long)ctas * THREADS) {
-        // the k-th largest of the threads' maxima is no larger than the k-th largest logit
-        if (mine_most > -INFINITY) atomicAdd(&s.bin_count[step_of(mine_most, count_scale)], 1u);
-        counted = true;
-        const Cut cut = cut_at(false, 0, k, 0.0, 0.0);
-        if (cut.count_before + cut.count >= (u64)k) {
-            for_all([&](float x, int i) {
-                if (x > -INFINITY && step_of(x, count_scale) <= cut.step) put_in_list(token_of(key_of(x), lo + i));
-            });
-            if (finish_list(true, 0)) return;
+    }
+    if (grouped) {
+        // the k-th largest of the groups' maxima is no larger than the k-th largest logit; it is one of at most GROUPS numbers that every CTA has
+        float border = -INFINITY;
+        if (groups <= THREADS) {                                     // the one with k - 1 in front of it
+            if (tid < groups) {
+                const float mine = s.group_most[tid];
+                int place = 0;
+                for (int j = 0; j < groups; j += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(s.group_most + j);
+                    place += (v.x > mine || (v.x == mine && j < tid)) + (v.y > mine || (v.y == mine && j + 1 < tid)) + (v.z > mine || (v.z == mine && j + 2 < tid)) +
+                             (v.w > mine || (v.w == mine && j + 3 < tid));
+                }
+                if (place == k - 1) s.floats[0] = mine;
+            }
+            __syncthreads();
+            border = s.floats[0];
+        } else {                                                     // the lower end of the step with it
+            for (int j = tid; j < groups; j += THREADS) atomicAdd(&s.bin_count[step_of(s.group_most[j], count_scale)], 1u);
+            __syncthreads();
+            u64 c = s.bin_count[tid], unused = 0;
+            s.bin_count[tid] = 0;
+            const u64 mine = c;
+            block_scan(c, unused, s);
+            if (c >= (u64)k && c - mine < (u64)k) s.found = tid;
+            __syncthreads();
+            border = s.found == BINS - 1 ? -INFINITY : largest == INFINITY ? largest : largest - (float)(s.found + 1) / count_scale * 1.0001f - 1e-5f * fabsf(largest);
         }
+        for_all(border, [&](float x, int i) {
+            if (x >= border && x > -INFINITY) put_in_list(token_of(key_of(x), lo + i));
+        });
+        if (finish_list(true, 0)) return;
     } else if (!k_on && (m_on || (vocab <= LIST && !p_on))) {
         u64 whole = 0;
         if (p_on) {
             u64 sum = 0;
-            for_all([&](float x, int) { sum += weight(x); });
+            for_all(weighty, [&](float x, int) { sum += weight(x); });
             exchange(block_join<false>(sum, s), 0, false, all, front);
             whole = all[0];
         }
         // what is far below min-p's border (by more than a float's rounding moves it) needs no weight
         const float border = m_on ? largest + T * (logf(fminf(min_p[r], 1.f)) - 1e-3f) - 1e-5f * fabsf(largest) : -INFINITY;
-        for_all([&](float x, int i) {
+        for_all(border, [&](float x, int i) {
             if (x < border || !(x > -INFINITY)) return;
             const u64 w = weight(x);
             if (w > 0 && (double)w >= least) put_in_list(token_of(key_of(x), lo + i));
@@ -503,7 +534,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         while (inside > LIST) {
             if (by_step) {                                           // the step's tokens are those of a run of keys
                 unsigned a = 0, b = 0;
-                for_all([&](float x, int i) {
+                for_all(-INFINITY, [&](float x, int i) {
                     const unsigned key = key_of(x);
                     if (is_inside(x, token_of(key, lo + i))) {
                         a = max(a, key);
@@ -518,10 +549,9 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
             }
             if (high_key == low_key) break;
             const int shift = max(0, 32 - __clz(high_key - low_key) - 9);      // at most BINS steps of 2^shift keys
-            cluster_barrier();                                       // the last histogram has been read
-            clear_bins();
+            clear_bins();                                            // every CTA has read the last ones
             __syncthreads();
-            for_all([&](float x, int i) {
+            for_all(value_of(low_key), [&](float x, int i) {
                 const unsigned key = key_of(x);
                 if (!is_inside(x, token_of(key, lo + i))) return;
                 if (by_weight) add_weight((high_key - key) >> shift, weight(x));
@@ -553,13 +583,26 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
             }
             result = block_join<true>(result, s);
         } else {
-            for_all([&](float x, int i) {
+            for_all(by_step ? -INFINITY : value_of(low_key), [&](float x, int i) {
                 const u64 token = token_of(key_of(x), lo + i);
                 if (is_inside(x, token)) put_in_list(token);
             });
             cluster_barrier();
-            if (rank == 0) {
-                const int listed = (int)s.listed, padded = power_of_two(listed);
+            const int listed = (int)s.listed;
+            if (rank == 0 && listed <= SHORT) {                      // places by counting: four threads a token
+                const int e = tid / 4, part = tid % 4;
+                if (tid < listed) s.weights[tid] = by_weight ? weight(value_of((unsigned)(s.list[tid] >> 32))) : 1;
+                __syncthreads();
+                const u64 token = e < listed ? s.list[e] : 0;
+                u64 ahead = 0;
+                for (int j = part; j < listed; j += 4) ahead += s.list[j] > token ? s.weights[j] : 0;
+#pragma unroll
+                for (int o = 1; o < 4; o *= 2) ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+                const bool kept = e < listed && (ahead == 0 || (by_weight ? (double)(before + ahead) < weight_goal : before + ahead < count_goal));
+                result = ~block_join<true>(kept ? ~token : 0, s);    // the last of those
+                if (tid == 0) s.listed = 0;
+            } else if (rank == 0) {
+                const int padded = power_of_two(listed);
                 for (int i = listed + tid; i < padded; i += THREADS) s.list[i] = 0;
                 sort_descending(s.list, padded);
                 u64 v[2];
@@ -583,33 +626,24 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         exchange(result, 0, true, all, front);
         last = all[0];
     };
-    // a histogram over steps, from nothing
-    auto start_bins = [&]() {
-        if (counted) {
-            cluster_barrier();                                       // the last one has been read
-            clear_bins();
-            __syncthreads();
-        }
-        counted = true;
-    };
     if (k_on) {
-        start_bins();
-        for_all([&](float x, int) {
+        for_all(-INFINITY, [&](float x, int) {
             if (x > -INFINITY) atomicAdd(&s.bin_count[step_of(x, count_scale)], 1u);
         });
         const Cut cut = cut_at(false, 0, k, 0.0, 0.0);
         if (cut.count_before + cut.count >= (u64)k) narrow(false, count_scale, cut, k, 0.0);      // else there are no more than k
+        clear_bins();
+        __syncthreads();
     }
     if (p_on) {
-        start_bins();
-        for_all([&](float x, int i) {
+        for_all(weighty, [&](float x, int i) {
             if (token_of(key_of(x), lo + i) < last) return;
             const u64 w = weight(x);
             if (w > 0) add_weight(step_of(x, weight_scale), w);
         });
         const Cut cut = cut_at(true, 0, 0, (double)p, -1.0);
         if (cut.count_before + cut.count <= LIST) {
-            for_all([&](float x, int i) {
+            for_all(weighty, [&](float x, int i) {
                 const u64 token = token_of(key_of(x), lo + i);
                 if (token >= last && step_of(x, weight_scale) <= cut.step && weight(x) > 0) put_in_list(token);
             });
@@ -620,15 +654,14 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     }
 
     // ---- the draw over the slices: a warp has a run of tokens
-    const int run = ((n + WARPS - 1) / WARPS + 31) & ~31, from = min(n, warp * run), to = min(n, from + run);
-    auto kept_weight = [&](int i) -> u64 {
-        const float x = at(i);
-        if (token_of(key_of(x), lo + i) < last) return 0;
+    const int run = ((n + WARPS - 1) / WARPS + 127) & ~127, from = min(n, warp * run), to = min(n, from + run);
+    const u64 least_weight = least > 0.0 ? (u64)ceil(least) : 0;
+    auto kept_weight = [&](float x, int i) -> u64 {
         const u64 w = weight(x);
-        return (double)w >= least ? w : 0;
+        return token_of(key_of(x), lo + i) >= last && w >= least_weight ? w : 0;
     };
     u64 mass = 0;
-    for (int i = from + lane; i < to; i += 32) mass += kept_weight(i);
+    for_some(from, to, lane, 32, fmaxf(weighty, value_of((unsigned)(last >> 32))), [&](float x, int i) { mass += kept_weight(x, i); });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
     __syncthreads();
@@ -647,13 +680,13 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     const int first = min(n, q * run), end = min(n, first + run), each = (end - first + THREADS - 1) / THREADS;
     const int mine_from = min(end, first + tid * each), mine_to = min(end, mine_from + each);
     u64 mine = 0, unused = 0;
-    for (int i = mine_from; i < mine_to; ++i) mine += kept_weight(i);
+    for (int i = mine_from; i < mine_to; ++i) mine += kept_weight(at(i), i);
     u64 scan = mine;
     block_scan(scan, unused, s);                                     // (it writes warp_b behind a barrier)
     upto += scan - mine;
     if (upto < goal && upto + mine >= goal)
         for (int i = mine_from; i < mine_to; ++i) {
-            upto += kept_weight(i);
+            upto += kept_weight(at(i), i);
             if (upto >= goal) {
                 out[r] = lo + i;
                 break;
