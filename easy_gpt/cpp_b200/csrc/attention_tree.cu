@@ -47,8 +47,8 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     const int last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;    // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
-    if (part >= parts) return;
-    const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
+    // a part behind the last one has no tiles, but its share of the output
+    const int begin = tile0 + (int)((long long)tiles * min(part, parts) / parts), stop = tile0 + (int)((long long)tiles * min(part + 1, parts) / parts);
 
     // ---- the tree: parents of the nodes up to the tile's last one, and every row's first cached key
     for (int i = tid; i <= last_node && i < STAGED_NODES; i += THREADS) ups[i] = tree::parent_of(p, e, i);
@@ -186,66 +186,49 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
             }
         }
     }
+    // where a row's results go
+    auto line_of = [&](int row) {
+        return static_cast<T*>(p.out) + (size_t)(e.first + (row0 + row) / group) * p.ldo + (size_t)(kvh * group + (row0 + row) % group) * D;
+    };
+    if (p.max_parts == 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (4 * ty + i >= count) continue;
+            T* const line = line_of(4 * ty + i);
+            const float inv = l[i] > 0.f ? 1.f / l[i] : l[i];
+#pragma unroll
+            for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    if (4 * tx + 64 * c + x < D) line[4 * tx + 64 * c + x] = from_f32<T>(acc[i][c][x] * inv);
+        }
+        return;
+    }
+    __syncthreads();                                                 // q, keys and values have been read
+    float* const o_s = q_s;
+    float* const ml_s = k_s;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int row = 4 * ty + i;
-        if (row >= count) continue;
-        const int node = (row0 + row) / group, head = kvh * group + (row0 + row) % group;
-        const float inv = parts > 1 ? 1.f : l[i] > 0.f ? 1.f / l[i] : 0.f;
-        const size_t line = (size_t)(e.first + node) * p.num_heads + head, slot = (size_t)part * p.rows * p.num_heads + line;
 #pragma unroll
         for (int c = 0; c < COLS; ++c)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int d = 4 * tx + 64 * c + x;
-                if (d >= D) continue;
-                if (parts > 1) p.partial_o[slot * D + d] = acc[i][c][x];
-                else static_cast<T*>(p.out)[(size_t)(e.first + node) * p.ldo + (size_t)head * D + d] = from_f32<T>(acc[i][c][x] * inv);
-            }
-        if (parts > 1 && tx == 0) *reinterpret_cast<float2*>(p.partial_ml + slot * 2) = make_float2(m[i], l[i]);
+            *reinterpret_cast<float4*>(o_s + (4 * ty + i) * L::LD + 4 * tx + 64 * c) = make_float4(acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]);
+        if (tx == 0) *reinterpret_cast<float2*>(ml_s + 2 * (4 * ty + i)) = make_float2(m[i], l[i]);
     }
-}
-
-// Adds the parts of a (row, head) up, in their order: a warp a line of the output, lanes over its columns.
-template <typename T>
-__global__ void __launch_bounds__(THREADS) attention_tree_merge_kernel(const Params p, int row_tile, int key_tile) {
-    pdl_enter();
-    const int r = blockIdx.y, group = p.num_heads / p.num_kv_heads, lane = threadIdx.x & 31;
-    const Entry e = tree::sound(p, p.entry_starts[r], p.entry_starts[r + 1], p.context[r]);
-    const int first = tree::first_key(p, e);
-    const long long lines = (long long)e.n * p.num_heads;
-    for (long long line = (long long)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5); line < lines; line += (long long)gridDim.x * (THREADS / 32)) {
-        const int node = (int)(line / p.num_heads), head = (int)(line % p.num_heads);
-        const int tile = (node * group + head % group) / row_tile, count = min(row_tile, e.n * group - tile * row_tile);
-        const int end = e.context + (tile * row_tile + count - 1) / group + 1;
-        const int parts = tree::parts_of(p, (end - 1) / key_tile - first / key_tile + 1);
-        if (parts <= 1) continue;
-        const size_t at = (size_t)e.first * p.num_heads + line, stride = (size_t)p.rows * p.num_heads;
-        float top = -INFINITY, total = 0.f;
-        for (int i = 0; i < parts; ++i) top = fmaxf(top, __ldcg(p.partial_ml + (at + i * stride) * 2));
-        for (int i = 0; i < parts; ++i) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.partial_ml + (at + i * stride) * 2));
-            total += ml.x == -INFINITY ? 0.f : exp2f(ml.x - top) * ml.y;
-        }
-        const float inv = total > 0.f ? 1.f / total : 0.f;
-        for (int d = lane; d < p.head_dim; d += 32) {
-            float sum = 0.f;
-            for (int i = 0; i < parts; ++i) {
-                const float m = __ldcg(p.partial_ml + (at + i * stride) * 2);
-                if (m != -INFINITY) sum = fmaf(exp2f(m - top), __ldcg(p.partial_o + (at + i * stride) * p.head_dim + d), sum);
-            }
-            static_cast<T*>(p.out)[(size_t)(e.first + node) * p.ldo + (size_t)head * p.head_dim + d] = from_f32<T>(sum * inv);
-        }
-    }
+    tree::add_parts<THREADS>(o_s, L::LD, ml_s, count, DMAX, parts, [&](int row, int d, float4 v) {
+        T* const line = line_of(row);
+        if (d < D) line[d] = from_f32<T>(v.x);
+        if (d + 1 < D) line[d + 1] = from_f32<T>(v.y);
+        if (d + 2 < D) line[d + 2] = from_f32<T>(v.z);
+        if (d + 3 < D) line[d + 3] = from_f32<T>(v.w);
+    });
 }
 
 template <typename T, int DMAX>
 int launch(cudaStream_t stream, const Params& p, int tiles) {
-    const int bytes = Layout<DMAX>::FLOATS * 4;
-    const cudaError_t set = cudaFuncSetAttribute(attention_tree_kernel<T, DMAX>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set != cudaSuccess) return (int)set;
-    eg_pdl_launch(attention_tree_kernel<T, DMAX>, dim3(p.max_parts, p.num_kv_heads, tiles), dim3(THREADS), bytes, stream, p);
-    return eg_launch_status();
+    constexpr int bytes = Layout<DMAX>::FLOATS * 4;
+    static unsigned long long seen = 0;
+    if (const int code = tree::prepare_kernel(attention_tree_kernel<T, DMAX>, bytes, seen)) return code;
+    return tree::launch_clusters(attention_tree_kernel<T, DMAX>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, p);
 }
 
 }  // namespace
@@ -261,27 +244,27 @@ EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries,
     const bool tiled = dtype == EG_BF16 && aligned && page_size % 16 == 0 && (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256);
     const int row_tile = !tiled ? ROWS : lines <= 16 ? 16 : lines <= 32 ? 32 : 64;
     const long long units = entries * ((lines + row_tile - 1) / row_tile) * num_kv_heads, key_tiles = ((long long)max_context + 63) / 64;
-    const long long places = (long long)sm_count * (tiled ? 3 : 2);
-    long long parts = (places + units - 1) / units;
-    if (parts > key_tiles / 2) parts = key_tiles / 2;
+    // as many parts as fill the SMs once, a power of two, of two key tiles at least; a cluster has to find room among the 16 SMs and more of a GPC
+    const int ctas = !tiled ? (head_dim <= 128 ? 2 : 1) : head_dim <= 64 ? 3 : head_dim == 128 ? 2 : 1;
+    int parts = 1;
+    while (parts < (ctas > 1 ? tree::MAX_PARTS : tree::MAX_PARTS / 2) && units * parts * 2 <= (long long)sm_count * ctas && key_tiles >= parts * 4) parts *= 2;
     plan[0] = tiled ? row_tile : 0;
-    plan[1] = (int)(parts < 1 ? 1 : parts > 128 ? 128 : parts);
+    plan[1] = parts;
     plan[2] = 2;
     return 0;
 }
 
 // q: [rows, ldq], out: [rows, ldo] of num_heads * head_dim columns; k_cache, v_cache: [num_pages][num_kv_heads][page_size][head_dim] with the same strides (in
 // elements); block_table: [entries, table_pages] with row stride table_stride; entry_starts: [entries + 1]; context: [entries]; parents: [rows].  A tile's keys
-// are cut into up to max_parts parts of at least part_tiles times 64 keys: partial_o takes max_parts * rows * num_heads * head_dim floats, partial_ml
-// max_parts * rows * num_heads * 2 (neither is used with max_parts 1).
+// are cut into up to max_parts (1, 2, 4, 8 or 16) parts of at least part_tiles times 64 keys.
 EG_API int eg_attention_tree(cudaStream_t stream, int dtype, const void* q, long long ldq, const void* k_cache, const void* v_cache, long long page_stride,
                              long long head_stride, const int* block_table, int table_stride, int table_pages, int num_pages, const int* entry_starts, const int* context,
                              const int* parents, void* out, long long ldo, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int window,
-                             float scale, int row_tile, int max_parts, int part_tiles, float* partial_o, float* partial_ml, int* status) {
+                             float scale, int row_tile, int max_parts, int part_tiles, int* status) {
     if (entries <= 0 || rows <= 0) return 0;
     if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads || num_kv_heads > 65535 || head_dim < 1 || head_dim > 256 || page_size < 1 || num_pages < 1 ||
-        table_pages < 0 || entries > 65535 || max_parts < 1 || part_tiles < 1 || (max_parts > 1 && (!partial_o || !partial_ml)) || !status || (dtype != EG_F32 && dtype != EG_BF16) ||
-        part_tiles > 1 << 20 || (row_tile != 0 && row_tile != 16 && row_tile != 32 && row_tile != 64))
+        table_pages < 0 || max_parts < 1 || max_parts > tree::MAX_PARTS || (max_parts & (max_parts - 1)) || part_tiles < 1 || part_tiles > 1 << 20 || !status ||
+        (dtype != EG_F32 && dtype != EG_BF16) || (row_tile != 0 && row_tile != 16 && row_tile != 32 && row_tile != 64))
         return (int)cudaErrorInvalidValue;
     if (row_tile && (dtype != EG_BF16 || (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) || page_size % 16 || (uintptr_t)q % 4 || ldq % 2 ||
                      (uintptr_t)out % 4 || ldo % 2 || (uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || page_stride % 8 || head_stride % 8))
@@ -290,17 +273,9 @@ EG_API int eg_attention_tree(cudaStream_t stream, int dtype, const void* q, long
     const long long tiles = (long long)rows * (num_heads / num_kv_heads) / tile_rows + entries; // at most: every entry's last tile may be a short one
     if (tiles > 65535 || (long long)rows * num_heads > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const Params p = {q, ldq, k_cache, v_cache, page_stride, head_stride, block_table, table_stride, table_pages, num_pages, entry_starts, context, parents, out, ldo,
-                      rows, entries, num_heads, num_kv_heads, head_dim, page_size, window, scale, max_parts, part_tiles * (64 / tile_keys), partial_o, partial_ml, status};
-    int code;
-    if (row_tile)
-        code = tree::launch_mma(stream, p, row_tile, (int)tiles);
-    else if (dtype == EG_F32)
-        code = head_dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);
-    else
-        code = head_dim <= 64 ? launch<bf16, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<bf16, 128>(stream, p, (int)tiles) : launch<bf16, 256>(stream, p, (int)tiles);
-    if (code || max_parts == 1) return code;
-    const dim3 grid((unsigned)min((long long)1024, ((long long)rows * num_heads + THREADS / 32 - 1) / (THREADS / 32)), entries);
-    if (dtype == EG_F32) eg_pdl_launch(attention_tree_merge_kernel<float>, grid, dim3(THREADS), 0, stream, p, tile_rows, tile_keys);
-    else eg_pdl_launch(attention_tree_merge_kernel<bf16>, grid, dim3(THREADS), 0, stream, p, tile_rows, tile_keys);
-    return eg_launch_status();
+                      rows, entries, num_heads, num_kv_heads, head_dim, page_size, window, scale, max_parts, part_tiles * (64 / tile_keys), status};
+    if (row_tile) return tree::launch_mma(stream, p, row_tile, (int)tiles);
+    if (dtype == EG_F32)
+        return head_dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);
+    return head_dim <= 64 ? launch<bf16, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<bf16, 128>(stream, p, (int)tiles) : launch<bf16, 256>(stream, p, (int)tiles);
 }

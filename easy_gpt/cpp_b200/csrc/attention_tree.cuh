@@ -6,9 +6,9 @@
 // and itself; with a window only those whose position is above its own minus the window.
 //
 // A row of the kernels is a (node, query head of the KV head's group): row i of an entry and KV head is head i % group of node i / group.
-// Rows are cut into tiles of ROWS, tiles are numbered through over the entries, and a tile's keys are cut into parts, each a unit of work:
-// its partial result (unnormalised output, reference, sum; base 2) goes to scratch memory and a merge kernel adds the parts up in order.  A
-// tile with one part is written at once.
+// Rows are cut into tiles, tiles are numbered through over the entries, and a tile's keys are cut into up to 16 parts, a CTA each.  The CTAs
+// of a tile are a thread-block cluster: their partial results (unnormalised output, reference, sum; base 2) stay in their shared memory, where the
+// cluster adds them up in the order of the parts, every CTA a share of the output.
 #pragma once
 #include "common.cuh"
 
@@ -30,8 +30,6 @@ struct Params {
     int rows, entries, num_heads, num_kv_heads, head_dim, page_size, window;
     float scale;
     int max_parts, part_tiles;       // a tile's keys are cut into min(max_parts, key tiles / part_tiles) parts, one at least
-    float* partial_o;                // [parts][rows * heads][head_dim]
-    float* partial_ml;               // [parts][rows * heads][2]
     int* status;
 };
 
@@ -49,15 +47,15 @@ __device__ __forceinline__ Entry sound(const Params& p, int first, int end, int 
     return e;
 }
 
-// A node's parent; one that cannot be is none, and a status bit.
-__device__ __forceinline__ int parent_of(const Params& p, const Entry& e, int i) {
-    const int up = p.parents[e.first + i];
+// Node i's parent as the metadata has it; one that cannot be is none, and a status bit.
+__device__ __forceinline__ int sound_parent(const Params& p, int i, int up) {
     if (up < -1 || up >= i) {
         atomicOr(p.status, EG_STATUS_BAD_TREE);
         return -1;
     }
     return up;
 }
+__device__ __forceinline__ int parent_of(const Params& p, const Entry& e, int i) { return sound_parent(p, i, p.parents[e.first + i]); }
 
 // The entry whose tile number `tile` is, counting ceil(n * group / row_tile) tiles an entry, and the tile's number within it; false: there
 // is none.  For a whole warp: 32 entries at a time, in one trip to memory.
@@ -95,5 +93,97 @@ __device__ __forceinline__ int parts_of(const Params& p, int key_tiles) { return
 
 // The kernel in attention_tree_mma.cu (16, 32 or 64 rows a CTA, key tiles of 64).  Its caller has checked what it takes.
 int launch_mma(cudaStream_t stream, const Params& p, int row_tile, int tiles);
+
+// ---- the parts of a tile, one CTA of the cluster each
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ unsigned remote(const void* mine, unsigned rank) {
+    unsigned a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((unsigned)__cvta_generic_to_shared(mine)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float2 remote_load2(unsigned at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ float4 remote_load4(unsigned at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+    return v;
+}
+constexpr int MAX_PARTS = 16;
+
+// Adds the cluster's parts up.  Every CTA has `o` (rows of `ld` floats, unnormalised) and `ml` (reference and sum a row; -inf and 0 where it has seen
+// nothing) in shared memory, written before the call; put(row, column, four values) takes the result.  A row takes part whose sum is not 0, in whatever
+// part; all CTAs of the cluster call this, and none leaves it before its shared memory has been read.
+template <int THREADS, typename Put>
+__device__ __forceinline__ void add_parts(const float* o, int ld, const float* ml, int rows, int columns, int parts, Put put) {
+    unsigned rank, ctas;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    cluster_barrier();
+    const int quads = columns / 4;
+    for (int i = (int)rank * THREADS + (int)threadIdx.x; i < rows * quads; i += (int)ctas * THREADS) {
+        const int row = i / quads, d = i % quads * 4;
+        float2 w[MAX_PARTS];
+#pragma unroll
+        for (int q = 0; q < MAX_PARTS; ++q) w[q] = q < parts ? remote_load2(remote(ml + 2 * row, q)) : make_float2(-INFINITY, 0.f);
+        float top = -INFINITY, total = 0.f;
+#pragma unroll
+        for (int q = 0; q < MAX_PARTS; ++q) top = fmaxf(top, w[q].x);
+#pragma unroll
+        for (int q = 0; q < MAX_PARTS; ++q) {
+            w[q].x = w[q].x == -INFINITY ? 0.f : exp2f(w[q].x - top);
+            total = fmaf(w[q].x, w[q].y, total);
+        }
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int q0 = 0; q0 < MAX_PARTS; q0 += 4) {
+            float4 v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = q0 + q < parts ? remote_load4(remote(o + row * ld + d, q0 + q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                sum.x = fmaf(w[q0 + q].x, v[q].x, sum.x);
+                sum.y = fmaf(w[q0 + q].x, v[q].y, sum.y);
+                sum.z = fmaf(w[q0 + q].x, v[q].z, sum.z);
+                sum.w = fmaf(w[q0 + q].x, v[q].w, sum.w);
+            }
+        }
+        const float inv = total > 0.f ? 1.f / total : total;          // nothing seen: 0; NaN stays
+        put(row, d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+    }
+    cluster_barrier();
+}
+
+// A launch whose CTAs along x are clusters, behind the kernel in front as a programmatic dependent.
+template <class... P, class... A>
+static inline int launch_clusters(void (*kernel)(P...), dim3 grid, int threads, size_t bytes, cudaStream_t stream, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = grid.x;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);       // its error is the launch status
+    return eg_launch_status();
+}
+template <class K> static inline int prepare_kernel(K kernel, int bytes, unsigned long long& seen) {
+    int device;
+    if (!eg_first_on_device(seen, device)) return 0;
+    cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (set == cudaSuccess) set = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (set == cudaSuccess) eg_done_on_device(seen, device);
+    return (int)set;
+}
 
 }  // namespace tree

@@ -27,7 +27,7 @@ struct Layout {
     static constexpr int STAGES = HD <= 64 ? 4 : HD == 128 ? 3 : 3;
     static constexpr bool Q_IN_SMEM = HD == 256;                                    // a row's fragments would take 64 registers
     static constexpr int Q_BYTES = Q_IN_SMEM ? ROWS * HD * 2 : 0;
-    static constexpr int MERGE_LD = HD + 8, MERGE_BYTES = WK == 1 ? 0 : 4 * 16 * (MERGE_LD + 2) * 4;
+    static constexpr int MERGE_LD = HD + 8, MERGE_BYTES = 4 * 16 * (MERGE_LD + 4) * 4;
     static constexpr int RING_BYTES = STAGES * STAGE_BYTES > MERGE_BYTES ? STAGES * STAGE_BYTES : MERGE_BYTES;
     static constexpr int SMEM = Q_BYTES + RING_BYTES;
     __device__ static __forceinline__ int offset(int row, int chunk) { return (row * CHUNKS + (chunk ^ (row & SWZ))) * 16; }
@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     const int row0 = within * ROWS, count = min(ROWS, e.n * group - row0), last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
-    if (part >= parts) return;
-    const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
+    // a part behind the last one has no tiles, but its share of the output
+    const int begin = tile0 + (int)((long long)tiles * min(part, parts) / parts), stop = tile0 + (int)((long long)tiles * min(part + 1, parts) / parts);
     const int* const table = p.block_table + (size_t)r * p.table_stride;
     const bf16* const q = static_cast<const bf16*>(p.q);
 
@@ -94,34 +94,11 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
             cp_async_16(ks + L::TILE_BYTES + L::offset(row, my_chunk), static_cast<const bf16*>(p.v_cache) + from, valid);
         }
     };
+    // ---- the tree: parents of the nodes up to the tile's last one, and every row's first cached key
+    // (what the next trip to memory brings is asked for before anything waits for it: block table, a parent a thread, rows of q)
     int ahead[LOOKUPS];
     look_up(begin, ahead);
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        int now[LOOKUPS];
-#pragma unroll
-        for (int i = 0; i < LOOKUPS; ++i) now[i] = ahead[i];
-        look_up(begin + s + 1, ahead);
-        if (begin + s < stop) load(begin + s, now);
-        cp_async_commit();
-    }
-
-    // ---- the tree: parents of the nodes up to the tile's last one, and every row's first cached key
-    for (int i = tid; i <= last_node && i < STAGED_NODES; i += THREADS) ups[i] = tree::parent_of(p, e, i);
-    if (tid == 0) latest = 0;
-    auto up_of = [&](int i) { return i < STAGED_NODES ? ups[i] : tree::parent_of(p, e, i); };
-    if (p.window > 0) {
-        __syncthreads();
-        if (tid < count) {
-            int depth = 0;
-            for (int i = up_of((row0 + tid) / group); i >= 0; i = up_of(i)) ++depth;
-            lowest[tid] = (int)max(0ll, (long long)e.context + depth - p.window + 1);
-            atomicMax(&latest, lowest[tid]);
-        }
-    } else if (tid < count) {
-        lowest[tid] = 0;
-    }
-
+    const int parent = tid <= last_node ? p.parents[e.first + tid] : -1;
     // ---- the rows of q as A fragments
     auto q_row = [&](int row) { return q + (size_t)(e.first + (row0 + row) / group) * p.ldq + (size_t)(kvh * group + (row0 + row) % group) * HD; };
     uint32_t qf[L::Q_IN_SMEM ? 1 : HD / 16][4];
@@ -143,6 +120,31 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
             qf[k][3] = b < count ? *reinterpret_cast<const uint32_t*>(qb + d + 8) : 0u;
         }
     }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+        int now[LOOKUPS];
+#pragma unroll
+        for (int i = 0; i < LOOKUPS; ++i) now[i] = ahead[i];
+        look_up(begin + s + 1, ahead);
+        if (begin + s < stop) load(begin + s, now);
+        cp_async_commit();
+    }
+    if (tid <= last_node) ups[tid] = tree::sound_parent(p, tid, parent);
+    for (int i = THREADS + tid; i <= last_node && i < STAGED_NODES; i += THREADS) ups[i] = tree::parent_of(p, e, i);
+    if (tid == 0) latest = 0;
+    auto up_of = [&](int i) { return i < STAGED_NODES ? ups[i] : tree::parent_of(p, e, i); };
+    if (p.window > 0) {
+        __syncthreads();
+        if (tid < count) {
+            int depth = 0;
+            for (int i = up_of((row0 + tid) / group); i >= 0; i = up_of(i)) ++depth;
+            lowest[tid] = (int)max(0ll, (long long)e.context + depth - p.window + 1);
+            atomicMax(&latest, lowest[tid]);
+        }
+    } else if (tid < count) {
+        lowest[tid] = 0;
+    }
+
     const float scale_log2 = p.scale * 1.4426950408889634f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, acc[HD / 8][4];
 #pragma unroll
@@ -306,64 +308,75 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
-    // what a row (of the tile), two columns of it, come to
-    auto put = [&](int row, int d, float x, float y) {
-        const size_t node = e.first + (row0 + row) / group, head = kvh * group + (row0 + row) % group;
-        if (parts > 1) *reinterpret_cast<float2*>(p.partial_o + (((size_t)part * p.rows + node) * p.num_heads + head) * HD + d) = make_float2(x, y);
-        else *reinterpret_cast<uint32_t*>(static_cast<bf16*>(p.out) + node * p.ldo + head * HD + d) = pack_bf16(x, y);
-    };
-    auto put_ml = [&](int row, float m, float l) {
-        const size_t node = e.first + (row0 + row) / group, head = kvh * group + (row0 + row) % group;
-        *reinterpret_cast<float2*>(p.partial_ml + (((size_t)part * p.rows + node) * p.num_heads + head) * 2) = make_float2(m, l);
-    };
     cp_async_wait<0>();
-    if constexpr (WK == 1) {
+    auto line_of = [&](int row) {                                    // where a row's results go
+        return static_cast<bf16*>(p.out) + (size_t)(e.first + (row0 + row) / group) * p.ldo + (size_t)(kvh * group + (row0 + row) % group) * HD;
+    };
+    auto put4 = [&](int row, int d, float4 v) {
+        uint32_t* const at = reinterpret_cast<uint32_t*>(line_of(row) + d);
+        at[0] = pack_bf16(v.x, v.y);
+        at[1] = pack_bf16(v.z, v.w);
+    };
+    if (WK == 1 && p.max_parts == 1) {
         const int a = wr * 16 + gid, b = a + 8;
-        const float i0 = parts > 1 ? 1.f : l0 > 0.f ? 1.f / l0 : l0, i1 = parts > 1 ? 1.f : l1 > 0.f ? 1.f / l1 : l1;
+        const float i0 = l0 > 0.f ? 1.f / l0 : l0, i1 = l1 > 0.f ? 1.f / l1 : l1;
 #pragma unroll
         for (int j = 0; j < HD / 8; ++j) {
-            if (a < count) put(a, 8 * j + 2 * tig, acc[j][0] * i0, acc[j][1] * i0);
-            if (b < count) put(b, 8 * j + 2 * tig, acc[j][2] * i1, acc[j][3] * i1);
+            if (a < count) *reinterpret_cast<uint32_t*>(line_of(a) + 8 * j + 2 * tig) = pack_bf16(acc[j][0] * i0, acc[j][1] * i0);
+            if (b < count) *reinterpret_cast<uint32_t*>(line_of(b) + 8 * j + 2 * tig) = pack_bf16(acc[j][2] * i1, acc[j][3] * i1);
         }
-        if (parts > 1 && tig == 0) {
-            if (a < count) put_ml(a, m0, l0);
-            if (b < count) put_ml(b, m1, l1);
-        }
+        return;
+    }
+    // ---- the warps that share rows, in the order of their keys, then the parts
+    __syncthreads();
+    float* const o_s = reinterpret_cast<float*>(ring);               // a line a warp and row
+    float* const ml_s = o_s + 4 * 16 * L::MERGE_LD;
+    float* const row_ml = ml_s + 2 * 4 * 16;                         // of the warps together
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) {
+        *reinterpret_cast<float2*>(o_s + (warp * 16 + gid) * L::MERGE_LD + 8 * j + 2 * tig) = make_float2(acc[j][0], acc[j][1]);
+        *reinterpret_cast<float2*>(o_s + (warp * 16 + gid + 8) * L::MERGE_LD + 8 * j + 2 * tig) = make_float2(acc[j][2], acc[j][3]);
+    }
+    if (tig == 0) {
+        *reinterpret_cast<float2*>(ml_s + 2 * (warp * 16 + gid)) = make_float2(m0, l0);
+        *reinterpret_cast<float2*>(ml_s + 2 * (warp * 16 + gid + 8)) = make_float2(m1, l1);
+    }
+    if constexpr (WK == 1) {
+        tree::add_parts<THREADS>(o_s, L::MERGE_LD, ml_s, count, HD, parts, put4);
     } else {
-        // the warps that share rows, in the order of their keys
         __syncthreads();
-        float* const o_s = reinterpret_cast<float*>(ring);
-        float* const ml_s = o_s + 4 * 16 * L::MERGE_LD;
-#pragma unroll
-        for (int j = 0; j < HD / 8; ++j) {
-            *reinterpret_cast<float2*>(o_s + (warp * 16 + gid) * L::MERGE_LD + 8 * j + 2 * tig) = make_float2(acc[j][0], acc[j][1]);
-            *reinterpret_cast<float2*>(o_s + (warp * 16 + gid + 8) * L::MERGE_LD + 8 * j + 2 * tig) = make_float2(acc[j][2], acc[j][3]);
-        }
-        if (tig == 0) {
-            ml_s[(warp * 16 + gid) * 2] = m0;
-            ml_s[(warp * 16 + gid) * 2 + 1] = l0;
-            ml_s[(warp * 16 + gid + 8) * 2] = m1;
-            ml_s[(warp * 16 + gid + 8) * 2 + 1] = l1;
-        }
-        __syncthreads();
-        for (int i = tid; i < ROWS * (HD / 2); i += THREADS) {
-            const int row = i / (HD / 2), d = i % (HD / 2) * 2;
-            if (row >= count) break;
-            const int line0 = (row / 16 * WK) * 16 + row % 16;
-            float top = -INFINITY, total = 0.f, x = 0.f, y = 0.f;
+        for (int i = tid; i < ROWS * (HD / 4); i += THREADS) {
+            const int row = i / (HD / 4), d = i % (HD / 4) * 4, line0 = row / 16 * WK * 16 + row % 16;
+            float top = -INFINITY, total = 0.f;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < WK; ++w) top = fmaxf(top, ml_s[(line0 + 16 * w) * 2]);
 #pragma unroll
             for (int w = 0; w < WK; ++w) {
-                const float m = ml_s[(line0 + 16 * w) * 2], c = m == -INFINITY ? 0.f : exp2_fast(m - top);
-                const float2 o = *reinterpret_cast<const float2*>(o_s + (line0 + 16 * w) * L::MERGE_LD + d);
-                total = fmaf(c, ml_s[(line0 + 16 * w) * 2 + 1], total);
-                x = fmaf(c, o.x, x);
-                y = fmaf(c, o.y, y);
+                const float2 ml = *reinterpret_cast<const float2*>(ml_s + (line0 + 16 * w) * 2);
+                const float c = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
+                const float4 o = *reinterpret_cast<const float4*>(o_s + (line0 + 16 * w) * L::MERGE_LD + d);
+                total = fmaf(c, ml.y, total);
+                sum = make_float4(fmaf(c, o.x, sum.x), fmaf(c, o.y, sum.y), fmaf(c, o.z, sum.z), fmaf(c, o.w, sum.w));
             }
-            const float inv = parts > 1 ? 1.f : total > 0.f ? 1.f / total : total;
-            put(row, d, x * inv, y * inv);
-            if (parts > 1 && d == 0) put_ml(row, top, total);
+            if (p.max_parts == 1) {
+                const float inv = total > 0.f ? 1.f / total : total;
+                if (row < count) put4(row, d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+            } else {                                                 // into its own line: nobody else reads this quad
+                *reinterpret_cast<float4*>(o_s + line0 * L::MERGE_LD + d) = sum;
+                if (d == 0) *reinterpret_cast<float2*>(row_ml + 2 * row) = make_float2(top, total);
+            }
+        }
+        if (p.max_parts > 1) {
+            // the lines of a row group lie WK * 16 apart
+            if constexpr (WK == 4) tree::add_parts<THREADS>(o_s, L::MERGE_LD, row_ml, count, HD, parts, put4);
+            else {
+                __syncthreads();
+                for (int i = tid; i < 16 * (HD / 4); i += THREADS)   // the second group's to behind the first's
+                    *reinterpret_cast<float4*>(o_s + (16 + i / (HD / 4)) * L::MERGE_LD + i % (HD / 4) * 4) =
+                        *reinterpret_cast<const float4*>(o_s + (32 + i / (HD / 4)) * L::MERGE_LD + i % (HD / 4) * 4);
+                tree::add_parts<THREADS>(o_s, L::MERGE_LD, row_ml, count, HD, parts, put4);
+            }
         }
     }
 }
@@ -371,10 +384,9 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
 template <int HD, int WR>
 int launch(cudaStream_t stream, const Params& p, int tiles) {
     constexpr int bytes = Layout<HD, WR>::SMEM;
-    const cudaError_t set = cudaFuncSetAttribute(attention_tree_mma_kernel<HD, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (set != cudaSuccess) return (int)set;
-    eg_pdl_launch(attention_tree_mma_kernel<HD, WR>, dim3(p.max_parts, p.num_kv_heads, tiles), dim3(THREADS), bytes, stream, p);
-    return eg_launch_status();
+    static unsigned long long seen = 0;
+    if (const int code = tree::prepare_kernel(attention_tree_mma_kernel<HD, WR>, bytes, seen)) return code;
+    return tree::launch_clusters(attention_tree_mma_kernel<HD, WR>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, p);
 }
 
 }  // namespace

@@ -100,7 +100,7 @@ class _Signatures:
     eg_sample = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_sample_min_p = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_attention_tree = [c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
-                         c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]
+                         c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p]
     eg_attention_tree_plan = [c_int] * 10 + [c_void_p]
     eg_tree_accept = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_cache_keep = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_void_p, c_int, c_int,
@@ -977,13 +977,10 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             dtype, (q.data_ptr() | out.data_ptr() | (q.stride(0) | out.stride(0)) * q.element_size()) % 4 == 0
             and (k_cache.data_ptr() | v_cache.data_ptr() | (k_cache.stride(0) | k_cache.stride(1)) * q.element_size()) % 16 == 0,
             T, entries, num_heads, num_kv_heads, head_dim, page_size, int(max_context)) if T and entries else (0, 1, 1)
-        scratch = torch.empty(parts * T * num_heads * (head_dim + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
-        partial_o = _ptr(scratch)
-        partial_ml = partial_o + parts * T * num_heads * head_dim * 4 if parts > 1 else None
         _check(library().eg_attention_tree(
             _stream(), dtype, _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), k_cache.stride(0), k_cache.stride(1), _ptr(block_table),
             block_table.stride(0), block_table.shape[1], k_cache.shape[0], _ptr(entry_starts), _ptr(context), _ptr(parents), _ptr(out), out.stride(0), T, entries,
-            num_heads, num_kv_heads, head_dim, page_size, int(window or 0), float(scale), row_tile, parts, part_tiles, partial_o, partial_ml, _ptr(status)), "attention_tree")
+            num_heads, num_kv_heads, head_dim, page_size, int(window or 0), float(scale), row_tile, parts, part_tiles, _ptr(status)), "attention_tree")
 
 
 def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch.Tensor, parents: torch.Tensor, path: torch.Tensor,

@@ -87,13 +87,13 @@ def test_launchers_refuse_sizes_they_do_not_take():
     assert [keep(size=1), keep(size=8), keep(pages=0), keep(heads=0), keep(page=0), keep(dim=0), keep(longest=0), keep(status=None), keep(entries=65536), keep(kv=at + 1),
             keep(layers=1 << 30)] == [1] * 11
 
-    def attend(dtype=kernels.BF16, rows=4, entries=1, heads=4, kv_heads=2, dim=64, page=16, pages=4, parts=1, tiles=1, scratch=at, status=at,
+    def attend(dtype=kernels.BF16, rows=4, entries=1, heads=4, kv_heads=2, dim=64, page=16, pages=4, parts=1, tiles=1, status=at,
                q=at, ldq=256, row_tile=0):
-        return lib.eg_attention_tree(None, dtype, q, ldq, at, at, 4096, 1024, at, 3, 3, pages, at, at, at, at, 256, rows, entries, heads, kv_heads, dim, page, 0, 0.125, row_tile, parts, tiles, scratch,
-                                     scratch, status)
+        return lib.eg_attention_tree(None, dtype, q, ldq, at, at, 4096, 1024, at, 3, 3, pages, at, at, at, at, 256, rows, entries, heads, kv_heads, dim, page, 0, 0.125, row_tile, parts, tiles,
+                                     status)
 
     assert [attend(rows=0), attend(entries=0)] == [0, 0]
-    assert [attend(dtype=2), attend(heads=3), attend(kv_heads=0), attend(dim=0), attend(dim=257), attend(page=0), attend(pages=0), attend(parts=0), attend(tiles=0), attend(parts=2, scratch=None),
-            attend(status=None), attend(entries=65536), attend(rows=1 << 30)] == [1] * 13
+    assert [attend(dtype=2), attend(heads=3), attend(kv_heads=0), attend(dim=0), attend(dim=257), attend(page=0), attend(pages=0), attend(parts=0), attend(tiles=0), attend(parts=3),
+            attend(parts=32), attend(status=None), attend(entries=65536), attend(rows=1 << 30)] == [1] * 14
     assert [attend(row_tile=8), attend(row_tile=16, dtype=kernels.F32), attend(row_tile=16, dim=80), attend(row_tile=64, page=24), attend(row_tile=32, q=at + 2),
             attend(row_tile=16, ldq=257)] == [1] * 6
