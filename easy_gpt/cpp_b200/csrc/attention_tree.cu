@@ -14,6 +14,7 @@ namespace {
 using tree::Entry;
 using tree::Params;
 
+constexpr int TC_LINES = 64;                                         // rows of an entry and KV head from which on the tcgen05 kernel takes them
 constexpr int ROWS = 64, KEYS = 32, THREADS = 256, STAGED_NODES = 1024;
 
 template <int DMAX>
@@ -47,8 +48,8 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     const int last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;    // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
-    // a part behind the last one has no tiles, but its share of the output
-    const int begin = tile0 + (int)((long long)tiles * min(part, parts) / parts), stop = tile0 + (int)((long long)tiles * min(part + 1, parts) / parts);
+    if (part >= parts) return;
+    const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
 
     // ---- the tree: parents of the nodes up to the tile's last one, and every row's first cached key
     for (int i = tid; i <= last_node && i < STAGED_NODES; i += THREADS) ups[i] = tree::parent_of(p, e, i);
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     auto line_of = [&](int row) {
         return static_cast<T*>(p.out) + (size_t)(e.first + (row0 + row) / group) * p.ldo + (size_t)(kvh * group + (row0 + row) % group) * D;
     };
-    if (p.max_parts == 1) {
+    if (parts == 1) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (4 * ty + i >= count) continue;
@@ -233,18 +234,30 @@ int launch(cudaStream_t stream, const Params& p, int tiles) {
 
 }  // namespace
 
-// How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (16, 32 or 64: the tensor-core kernel; 0: the 32-bit one),
-// plan[1] and plan[2] the max_parts and part_tiles of eg_attention_tree.  aligned: q, out and their rows start on 4-byte boundaries, the
-// caches, their pages and heads on 16-byte ones.  max_context: the most keys of an entry, as far as known.
+// How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (128: the tcgen05 kernel; 16, 32 or 64: the warp-level one;
+// 0: the 32-bit one),
+// plan[1] and plan[2] the max_parts and part_tiles of eg_attention_tree.  aligned: the caches, their pages and heads start on 16-byte boundaries, and
+// q, out and their rows on 16-byte (2) or 4-byte (1) ones.  max_context: the most keys of an entry, as far as known.
 EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count,
                                   int* plan) {
     if (rows < 1 || entries < 1 || num_kv_heads < 1 || num_heads % num_kv_heads || num_heads < 1 || page_size < 1 || sm_count < 1 || !plan) return (int)cudaErrorInvalidValue;
     const int group = num_heads / num_kv_heads;
     const long long lines = ((long long)rows * group + entries - 1) / entries;      // of an entry, on the average
     const bool tiled = dtype == EG_BF16 && aligned && page_size % 16 == 0 && (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256);
-    const int row_tile = !tiled ? ROWS : lines <= 16 ? 16 : lines <= 32 ? 32 : 64;
+    const bool wide = tiled && aligned > 1 && (head_dim == 64 || head_dim == 128) && group <= 128;
+    const int row_tile = !tiled ? ROWS : lines <= 16 ? 16 : lines <= 32 ? 32 : wide && lines > TC_LINES ? 128 : 64;
     const long long units = entries * ((lines + row_tile - 1) / row_tile) * num_kv_heads, key_tiles = ((long long)max_context + 63) / 64;
     // as many parts as fill the SMs once, a power of two, of two key tiles at least; a cluster has to find room among the 16 SMs and more of a GPC
+    if (row_tile == 128) {
+        const int nodes = 128 / group;
+        const long long tc_units = entries * (((long long)rows + entries * nodes - 1) / (entries * nodes)) * num_kv_heads;
+        int parts = 1;
+        while (parts < 8 && tc_units * parts < 6ll * sm_count && key_tiles >= parts * 8) parts *= 2;
+        plan[0] = 128;
+        plan[1] = parts;
+        plan[2] = (int)(key_tiles / (parts * 2) > 4 ? key_tiles / parts : 4);
+        return 0;
+    }
     const int ctas = !tiled ? (head_dim <= 128 ? 2 : 1) : head_dim <= 64 ? 3 : head_dim == 128 ? 2 : 1;
     int parts = 1;
     while (parts < (ctas > 1 ? tree::MAX_PARTS : tree::MAX_PARTS / 2) && units * parts * 2 <= (long long)sm_count * ctas && key_tiles >= parts * 4) parts *= 2;
@@ -263,17 +276,21 @@ EG_API int eg_attention_tree(cudaStream_t stream, int dtype, const void* q, long
                              float scale, int row_tile, int max_parts, int part_tiles, int* status) {
     if (entries <= 0 || rows <= 0) return 0;
     if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads || num_kv_heads > 65535 || head_dim < 1 || head_dim > 256 || page_size < 1 || num_pages < 1 ||
-        table_pages < 0 || max_parts < 1 || max_parts > tree::MAX_PARTS || (max_parts & (max_parts - 1)) || part_tiles < 1 || part_tiles > 1 << 20 || !status ||
-        (dtype != EG_F32 && dtype != EG_BF16) || (row_tile != 0 && row_tile != 16 && row_tile != 32 && row_tile != 64))
+        table_pages < 0 || !(scale > 0.f) || scale > 3e38f || max_parts < 1 || max_parts > tree::MAX_PARTS || (max_parts & (max_parts - 1)) || part_tiles < 1 || part_tiles > 1 << 20 || !status ||
+        (dtype != EG_F32 && dtype != EG_BF16) || (row_tile != 0 && row_tile != 16 && row_tile != 32 && row_tile != 64 && row_tile != 128))
         return (int)cudaErrorInvalidValue;
     if (row_tile && (dtype != EG_BF16 || (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) || page_size % 16 || (uintptr_t)q % 4 || ldq % 2 ||
                      (uintptr_t)out % 4 || ldo % 2 || (uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || page_stride % 8 || head_stride % 8))
+        return (int)cudaErrorInvalidValue;
+    if (row_tile == 128 && ((head_dim != 64 && head_dim != 128) || num_heads / num_kv_heads > 128 || (uintptr_t)q % 16 || ldq % 8 || (uintptr_t)out % 16 || ldo % 8 ||
+                            page_stride % head_dim || head_stride % head_dim || page_stride <= 0 || head_stride <= 0))
         return (int)cudaErrorInvalidValue;
     const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
     const long long tiles = (long long)rows * (num_heads / num_kv_heads) / tile_rows + entries; // at most: every entry's last tile may be a short one
     if (tiles > 65535 || (long long)rows * num_heads > 0x7fffffff) return (int)cudaErrorInvalidValue;
     const Params p = {q, ldq, k_cache, v_cache, page_stride, head_stride, block_table, table_stride, table_pages, num_pages, entry_starts, context, parents, out, ldo,
                       rows, entries, num_heads, num_kv_heads, head_dim, page_size, window, scale, max_parts, part_tiles * (64 / tile_keys), status};
+    if (row_tile == 128) return tree::launch_tc(stream, p);
     if (row_tile) return tree::launch_mma(stream, p, row_tile, (int)tiles);
     if (dtype == EG_F32)
         return head_dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);

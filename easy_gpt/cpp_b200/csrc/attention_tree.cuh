@@ -93,6 +93,9 @@ __device__ __forceinline__ int parts_of(const Params& p, int key_tiles) { return
 
 // The kernel in attention_tree_mma.cu (16, 32 or 64 rows a CTA, key tiles of 64).  Its caller has checked what it takes.
 int launch_mma(cudaStream_t stream, const Params& p, int row_tile, int tiles);
+// The kernel in attention_tree_tc.cu (128 rows a CTA, or as many as whole nodes have; key tiles of 64).  Its caller has checked what it takes, but for the
+// size of the tensor maps.
+int launch_tc(cudaStream_t stream, const Params& p);
 
 // ---- the parts of a tile, one CTA of the cluster each
 __device__ __forceinline__ void cluster_barrier() {
@@ -117,15 +120,15 @@ constexpr int MAX_PARTS = 16;
 
 // Adds the cluster's parts up.  Every CTA has `o` (rows of `ld` floats, unnormalised) and `ml` (reference and sum a row; -inf and 0 where it has seen
 // nothing) in shared memory, written before the call; put(row, column, four values) takes the result.  A row takes part whose sum is not 0, in whatever
-// part; all CTAs of the cluster call this, and none leaves it before its shared memory has been read.
+// part.  The cluster's first `parts` CTAs call this, and none of them leaves it before its shared memory has been read; the others have left the
+// kernel, which the barriers do not wait for.
 template <int THREADS, typename Put>
 __device__ __forceinline__ void add_parts(const float* o, int ld, const float* ml, int rows, int columns, int parts, Put put) {
-    unsigned rank, ctas;
+    unsigned rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
     cluster_barrier();
     const int quads = columns / 4;
-    for (int i = (int)rank * THREADS + (int)threadIdx.x; i < rows * quads; i += (int)ctas * THREADS) {
+    for (int i = (int)rank * THREADS + (int)threadIdx.x; i < rows * quads; i += parts * THREADS) {
         const int row = i / quads, d = i % quads * 4;
         float2 w[MAX_PARTS];
 #pragma unroll

@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     const int row0 = within * ROWS, count = min(ROWS, e.n * group - row0), last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
-    // a part behind the last one has no tiles, but its share of the output
-    const int begin = tile0 + (int)((long long)tiles * min(part, parts) / parts), stop = tile0 + (int)((long long)tiles * min(part + 1, parts) / parts);
+    if (part >= parts) return;
+    const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
     const int* const table = p.block_table + (size_t)r * p.table_stride;
     const bf16* const q = static_cast<const bf16*>(p.q);
 
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
         at[0] = pack_bf16(v.x, v.y);
         at[1] = pack_bf16(v.z, v.w);
     };
-    if (WK == 1 && p.max_parts == 1) {
+    if (WK == 1 && parts == 1) {
         const int a = wr * 16 + gid, b = a + 8;
         const float i0 = l0 > 0.f ? 1.f / l0 : l0, i1 = l1 > 0.f ? 1.f / l1 : l1;
 #pragma unroll
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
                 total = fmaf(c, ml.y, total);
                 sum = make_float4(fmaf(c, o.x, sum.x), fmaf(c, o.y, sum.y), fmaf(c, o.z, sum.z), fmaf(c, o.w, sum.w));
             }
-            if (p.max_parts == 1) {
+            if (parts == 1) {
                 const float inv = total > 0.f ? 1.f / total : total;
                 if (row < count) put4(row, d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
             } else {                                                 // into its own line: nobody else reads this quad
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
                 if (d == 0) *reinterpret_cast<float2*>(row_ml + 2 * row) = make_float2(top, total);
             }
         }
-        if (p.max_parts > 1) {
+        if (parts > 1) {
             // the lines of a row group lie WK * 16 apart
             if constexpr (WK == 4) tree::add_parts<THREADS>(o_s, L::MERGE_LD, row_ml, count, HD, parts, put4);
             else {

@@ -11,6 +11,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import math
 import os
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional
@@ -938,9 +939,19 @@ def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
 SAMPLE_MAX_VOCAB = 1 << 20
 
 
+def _tree_alignment(q, k_cache, v_cache, out) -> int:
+    """What attention_tree_plan calls aligned: 2 rows of q and out on 16-byte boundaries, 1 on 4-byte ones, 0 neither or caches that are not."""
+    es, pages, heads = q.element_size(), k_cache.stride(0), k_cache.stride(1)
+    rows = q.data_ptr() | out.data_ptr() | (q.stride(0) | out.stride(0)) * es
+    if (k_cache.data_ptr() | v_cache.data_ptr() | (pages | heads) * es) % 16 or rows % 4:
+        return 0
+    return 1 if rows % 16 or pages % k_cache.shape[3] or heads % k_cache.shape[3] or not pages or not heads else 2
+
+
 @functools.lru_cache(maxsize=4096)
-def attention_tree_plan(dtype: int, aligned: bool, rows: int, entries: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_context: int):
-    """(rows of a CTA or 0 for the 32-bit kernel, the most parts a row tile's keys are cut into, the fewest times 64 keys of a part)."""
+def attention_tree_plan(dtype: int, aligned: int, rows: int, entries: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_context: int):
+    """(rows of a CTA: 128 the tcgen05 kernel, 16 to 64 the warp-level one, 0 the 32-bit one; the most parts a row tile's keys are cut into; the fewest
+    times 64 keys of a part)."""
     plan = (c_int * 3)()
     _need(library().eg_attention_tree_plan(dtype, aligned, rows, entries, num_heads, num_kv_heads, head_dim, page_size, max_context, sm_count(), plan) == 0, "sizes of a step")
     return tuple(plan)
@@ -970,12 +981,11 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
               and parents.is_contiguous(), "entry_starts [entries + 1], context [entries], contiguous parents")
         _need(k_cache.dim() == 4 and tuple(k_cache.shape[1:]) == (num_kv_heads, page_size, head_dim) and k_cache.shape == v_cache.shape
               and k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1 and k_cache.stride(2) == head_dim, "cache shape [pages, NKV, page_size, HD]")
-        _need(window is None or window > 0, "a window of one key at least")
+        _need((window is None or window > 0) and 0 < scale < math.inf, "a window of one key at least, a scale above 0")
         if max_context is None:
             max_context = block_table.shape[1] * page_size
         row_tile, parts, part_tiles = attention_tree_plan(
-            dtype, (q.data_ptr() | out.data_ptr() | (q.stride(0) | out.stride(0)) * q.element_size()) % 4 == 0
-            and (k_cache.data_ptr() | v_cache.data_ptr() | (k_cache.stride(0) | k_cache.stride(1)) * q.element_size()) % 16 == 0,
+            dtype, _tree_alignment(q, k_cache, v_cache, out),
             T, entries, num_heads, num_kv_heads, head_dim, page_size, int(max_context)) if T and entries else (0, 1, 1)
         _check(library().eg_attention_tree(
             _stream(), dtype, _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), k_cache.stride(0), k_cache.stride(1), _ptr(block_table),

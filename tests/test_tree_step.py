@@ -1,5 +1,6 @@
 """What the operators of a step over drafted trees refuse before anything is launched (no GPU): by their Python faces, and by the launchers alone."""
 import contextlib
+import math
 
 import pytest
 import torch
@@ -41,7 +42,7 @@ REFUSED = [
         dict(q=ROWS.float()), dict(q=ROWS.half(), out=ROWS.half(), k_cache=CACHE[:, 0].half(), v_cache=CACHE[:, 1].half()), dict(num_heads=3), dict(num_kv_heads=0), dict(num_heads=0), dict(head_dim=32),
         dict(head_dim=300), dict(block_table=i32(2, 3).long()), dict(block_table=i32(3, 2).t()), dict(block_table=i32(6)), dict(entry_starts=i32(2)), dict(context=i32(1)), dict(context=i32(4)[::2]),
         dict(parents=i32(11)), dict(parents=i32(20)[::2]), dict(out=ROWS[:4]), dict(out=ROWS[:, :255]), dict(v_cache=CACHE[:1, 1]), dict(k_cache=CACHE[:, 0].transpose(2, 3)), dict(k_cache=CACHE[0, 0]),
-        dict(status=i32(1).long()), dict(q=ROWS[:, :64]), dict(q=ROWS[0]), dict(window=-3), dict(window=0), dict(v_cache=CACHE[:, 1].float()))),
+        dict(status=i32(1).long()), dict(q=ROWS[:, :64]), dict(q=ROWS[0]), dict(window=-3), dict(window=0), dict(scale=0.0), dict(scale=-0.1), dict(scale=math.nan), dict(scale=math.inf), dict(v_cache=CACHE[:, 1].float()))),
     *(("sample_min_p", SAMPLE, w) for w in (
         dict(logits=torch.zeros((2, 8), dtype=torch.float64)), dict(logits=torch.zeros((8, 2)).t()), dict(logits=torch.zeros(8)), dict(temperature=NUMBERS.double()), dict(top_k=NUMBERS),
         dict(min_p=NUMBERS[:1]), dict(out=i32(2).long()), dict(logits=torch.zeros((2, 0))), dict(logits=torch.zeros((1, 1)).expand(2, (1 << 20) + 1)), dict(top_p=torch.zeros(4)[::2]))),
@@ -88,12 +89,12 @@ def test_launchers_refuse_sizes_they_do_not_take():
             keep(layers=1 << 30)] == [1] * 11
 
     def attend(dtype=kernels.BF16, rows=4, entries=1, heads=4, kv_heads=2, dim=64, page=16, pages=4, parts=1, tiles=1, status=at,
-               q=at, ldq=256, row_tile=0):
-        return lib.eg_attention_tree(None, dtype, q, ldq, at, at, 4096, 1024, at, 3, 3, pages, at, at, at, at, 256, rows, entries, heads, kv_heads, dim, page, 0, 0.125, row_tile, parts, tiles,
+               q=at, ldq=256, row_tile=0, scale=0.125):
+        return lib.eg_attention_tree(None, dtype, q, ldq, at, at, 4096, 1024, at, 3, 3, pages, at, at, at, at, 256, rows, entries, heads, kv_heads, dim, page, 0, scale, row_tile, parts, tiles,
                                      status)
 
     assert [attend(rows=0), attend(entries=0)] == [0, 0]
     assert [attend(dtype=2), attend(heads=3), attend(kv_heads=0), attend(dim=0), attend(dim=257), attend(page=0), attend(pages=0), attend(parts=0), attend(tiles=0), attend(parts=3),
             attend(parts=32), attend(status=None), attend(entries=65536), attend(rows=1 << 30)] == [1] * 14
-    assert [attend(row_tile=8), attend(row_tile=16, dtype=kernels.F32), attend(row_tile=16, dim=80), attend(row_tile=64, page=24), attend(row_tile=32, q=at + 2),
-            attend(row_tile=16, ldq=257)] == [1] * 6
+    assert [attend(row_tile=8), attend(row_tile=16, dtype=kernels.F32), attend(row_tile=16, dim=80), attend(row_tile=64, page=24), attend(row_tile=32, q=at + 2), attend(scale=0.0), attend(scale=-1.0), attend(row_tile=128, dim=32), attend(row_tile=128, q=at + 8),
+            attend(row_tile=16, ldq=257)] == [1] * 10
