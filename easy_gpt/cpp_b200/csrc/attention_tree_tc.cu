@@ -10,8 +10,8 @@
 // A row is a thread and a warp's rows exponentiate at the unit's rate (512 cycles a tile and SM, against 128 or 256 for the two products), so two
 // CTAs share an SM (256 columns of TMEM and less than half the shared memory each), one's exponents beside the other's products and waits.
 //
-// Warps: 0 loads, 1 allocates TMEM and issues the products (scores of a later tile before this one's output), 2 to 5 have the rows.  Keys and
-// values have rings of their own: a key stage is free when its scores are there.  A piece of a tile that no row sees, or whose page is none, is
+// Warps: 0 loads keys and 6 values, 1 allocates TMEM and issues the products (scores of a later tile before this one's output), 2 to 5 have the rows.
+// Keys and values have rings of their own, since a key stage is free long before the value stage of its tile: when its scores are there.  A piece of a tile that no row sees, or whose page is none, is
 // read from behind the last row of the cache map, which gives zeros.  Every wait is bounded; a role that gives up raises the CTA's abort flag, the
 // loader waits for its copies, and the CTA leaves as it always does.
 //
@@ -28,7 +28,7 @@ using namespace tc05;
 using tree::Entry;
 using tree::Params;
 
-constexpr int KEYS = 64, THREADS = 192, STAGED_NODES = 512;
+constexpr int KEYS = 64, THREADS = 224, STAGED_NODES = 512;
 constexpr float REFERENCE_SLACK = 8.f;
 
 template <int HD>
@@ -74,9 +74,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const int* const table = p.block_table + (size_t)r * p.table_stride;
     const int row_warps = (count + 31) / 32;
 
-    // ---- loader: a lane a box (64 columns of K or V, piece_rows keys) of every tile; its page is looked up a tile ahead
-    const int pieces = KEYS / maps.piece_rows, piece = lane % pieces, is_v = lane / pieces & 1, sub = lane / (2 * pieces);
-    const bool loads = warp == 0 && lane < 2 * pieces * S::SUBS;
+    // ---- loaders: a lane a box (64 columns, piece_rows keys) of every tile; its page is looked up a tile ahead
+    const bool is_v = warp == 6, loader = warp == 0 || is_v;
+    const int pieces = KEYS / maps.piece_rows, piece = lane % pieces, sub = lane / pieces;
+    const bool loads = loader && lane < pieces * S::SUBS;
     constexpr int NOT_NEEDED = -2;
     auto page_of = [&](int j) {
         const int key = (begin + j) * KEYS + piece * maps.piece_rows, slot = key / p.page_size;
@@ -84,6 +85,15 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         return slot < p.table_pages ? max(__ldg(table + slot), -1) : -1;
     };
     int page_ahead = loads ? page_of(0) : NOT_NEEDED;
+    // ---- rows: a thread's row of q and a node's parent are asked for in the same trip
+    const int quad = warp & 3, row = quad * 32 + lane;               // (of warps 2 to 5) a warp may touch the TMEM lanes 32 (warp % 4) ..
+    const bool has_rows = !loader && warp != 1 && quad < row_warps, valid = has_rows && row < count;
+    const int node = node0 + min(row, count - 1) / group, head = kvh * group + row % group;
+    uint4 q_row[HD / 8];
+    const uint4* const q_from = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + (size_t)(e.first + node) * p.ldq + (size_t)head * HD);
+#pragma unroll
+    for (int c = 0; c < HD / 8; ++c) q_row[c] = valid ? __ldg(q_from + c) : make_uint4(0, 0, 0, 0);
+    const int parent = has_rows && row <= last_node ? p.parents[e.first + row] : -1;
     if (threadIdx.x == 0) {
         mbar_init(&q_full, row_warps);
         for (int i = 0; i < STAGES; ++i) {
@@ -112,10 +122,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     // a row's result, its columns c0 .. c0 + 31
     bool rows_done = false;
     float row_scale = 1.f;
-    const int quad = warp & 3, row = quad * 32 + lane;               // (of warps 2 to 5) a warp may touch the TMEM lanes 32 (warp % 4) ..
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), o_lanes = lanes + S::O_COL;
-    const bool valid = row < count;
-    const int node = node0 + min(row, count - 1) / group, head = kvh * group + row % group;
     auto up_of = [&](int i) { return i < STAGED_NODES ? ups[i] : tree::parent_of(p, e, i); };
     int lowest = 0;
     // which of a key tile's keys the row sees
@@ -134,13 +141,17 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         return bits;
     };
 
-    if (warp == 0) {
+    if (loader) {
+        uint64_t* const full = is_v ? v_full : k_full;
+        uint64_t* const empty = is_v ? v_empty : k_empty;
+        const uint32_t ring = is_v ? v_ring : k_ring;
+        const CUtensorMap* const map = is_v ? &map_v : &map_k;
         int issued = 0;
         for (int j = 0; j < ntiles; ++j, ++issued) {
             const int st = j % STAGES, use = j / STAGES;
             const int page = page_ahead;
             if (loads) page_ahead = page_of(j + 1);
-            if (use > 0 && !__all_sync(0xffffffffu, lane > 1 || mbar_wait(lane ? &v_empty[st] : &k_empty[st], (use - 1) & 1, &abort_flag, p.status))) break;
+            if (use > 0 && !__all_sync(0xffffffffu, lane > 0 || mbar_wait(&empty[st], (use - 1) & 1, &abort_flag, p.status))) break;
             int at = maps.nowhere;
             if (loads && page != NOT_NEEDED) {
                 if (page < 0 || page >= p.num_pages) {
@@ -151,21 +162,13 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 }
             }
             __syncwarp();
-            if (lane == 0) {
-                mbar_expect_tx(&k_full[st], S::TILE_BYTES);
-                mbar_expect_tx(&v_full[st], S::TILE_BYTES);
-            }
+            if (lane == 0) mbar_expect_tx(&full[st], S::TILE_BYTES);
             __syncwarp();
-            if (loads)
-                tma_load_2d((is_v ? v_ring : k_ring) + st * S::TILE_BYTES + sub * S::SUB_BYTES + piece * maps.piece_rows * SUB_ROW_BYTES, is_v ? &map_v : &map_k,
-                            is_v ? &v_full[st] : &k_full[st], sub * 64, at);
+            if (loads) tma_load_2d(ring + st * S::TILE_BYTES + sub * S::SUB_BYTES + piece * maps.piece_rows * SUB_ROW_BYTES, map, &full[st], sub * 64, at);
         }
         // every copy has to land before the CTA gives up its shared memory, also when a role has given up
         if (lane == 0 && *(volatile int*)&abort_flag)
-            for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j) {
-                mbar_wait_plain(&k_full[j % STAGES], (j / STAGES) & 1);
-                mbar_wait_plain(&v_full[j % STAGES], (j / STAGES) & 1);
-            }
+            for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j) mbar_wait_plain(&full[j % STAGES], (j / STAGES) & 1);
     } else if (warp == 1) {
         if (lane == 0) {                                             // ---- the products
             const uint32_t idesc_s = idesc(KEYS, false), idesc_o = idesc(HD, true), hi = (uint32_t)(desc_k_major(0) >> 32);
@@ -205,23 +208,17 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 tc_commit(&v_empty[j % STAGES]);
             }
         }
-    } else if (quad < row_warps) {
+    } else if (has_rows) {
         // ---- the rows: q into shared memory, the tree, then a key tile at a time
-        const int row_threads = row_warps * 32, row_thread = quad * 32 + lane;
+        const int row_threads = row_warps * 32;
         auto rows_barrier = [&]() { asm volatile("bar.sync 1, %0;\n" ::"r"(row_threads) : "memory"); };
-        {
-            const uint4* const from = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + (size_t)(e.first + node) * p.ldq + (size_t)head * HD);
-            uint4 v[HD / 8];
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) v[c] = valid ? __ldg(from + c) : make_uint4(0, 0, 0, 0);
-            for (int i = row_thread; i <= last_node && i < STAGED_NODES; i += row_threads) ups[i] = tree::parent_of(p, e, i);
-#pragma unroll
-            for (int c = 0; c < HD / 8; ++c)
-                *reinterpret_cast<uint4*>(aligned + c / 8 * S::Q_SUB_BYTES + row * SUB_ROW_BYTES + ((c % 8) ^ (row & 7)) * 16) = v[c];
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full);
-        }
+        for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(aligned + c / 8 * S::Q_SUB_BYTES + row * SUB_ROW_BYTES + ((c % 8) ^ (row & 7)) * 16) = q_row[c];
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full);
+        if (row <= last_node) ups[row] = tree::sound_parent(p, row, parent);
+        for (int i = row_threads + row; i <= last_node && i < STAGED_NODES; i += row_threads) ups[i] = tree::parent_of(p, e, i);
         rows_barrier();
         if (p.window > 0) {
             int depth = 0;
