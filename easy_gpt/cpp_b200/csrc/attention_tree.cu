@@ -8,6 +8,7 @@
 // Which keys a row sees is decided by a select, never by adding: a hidden score may be anything.  A hidden value takes part as 0 * v, so
 // values that are not finite are put aside as zeros and added where they are seen.
 #include "attention_tree.cuh"
+#include "attention_tree_args.h"
 
 namespace {
 
@@ -267,32 +268,43 @@ EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries,
     return 0;
 }
 
-// q: [rows, ldq], out: [rows, ldo] of num_heads * head_dim columns; k_cache, v_cache: [num_pages][num_kv_heads][page_size][head_dim] with the same strides (in
-// elements); block_table: [entries, table_pages] with row stride table_stride; entry_starts: [entries + 1]; context: [entries]; parents: [rows].  A tile's keys
-// are cut into up to max_parts (1, 2, 4, 8 or 16) parts of at least part_tiles times 64 keys.
-EG_API int eg_attention_tree(cudaStream_t stream, int dtype, const void* q, long long ldq, const void* k_cache, const void* v_cache, long long page_stride,
-                             long long head_stride, const int* block_table, int table_stride, int table_pages, int num_pages, const int* entry_starts, const int* context,
-                             const int* parents, void* out, long long ldo, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int window,
-                             float scale, int row_tile, int max_parts, int part_tiles, int* status) {
-    if (entries <= 0 || rows <= 0) return 0;
-    if (num_kv_heads < 1 || num_heads < 1 || num_heads % num_kv_heads || num_kv_heads > 65535 || head_dim < 1 || head_dim > 256 || page_size < 1 || num_pages < 1 ||
-        table_pages < 0 || !(scale > 0.f) || scale > 3e38f || max_parts < 1 || max_parts > tree::MAX_PARTS || (max_parts & (max_parts - 1)) || part_tiles < 1 || part_tiles > 1 << 20 || !status ||
-        (dtype != EG_F32 && dtype != EG_BF16) || (row_tile != 0 && row_tile != 16 && row_tile != 32 && row_tile != 64 && row_tile != 128))
+// A tile's keys are cut into up to max_parts (1, 2, 4, 8 or 16) parts of at least part_tiles times 64 keys.
+EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* args) {
+    if (!args) return (int)cudaErrorInvalidValue;
+    const eg_attention_tree_args& a = *args;
+    if (a.entries <= 0 || a.rows <= 0) return 0;
+    constexpr long long INT = 0x7fffffff;
+    if ((a.dtype != EG_F32 && a.dtype != EG_BF16) || a.num_kv_heads < 1 || a.num_heads < 1 || a.num_heads > INT || a.num_heads % a.num_kv_heads || a.num_kv_heads > 65535 ||
+        a.head_dim < 1 || a.head_dim > 256 || a.page_size < 1 || a.page_size > INT || a.num_pages < 1 || a.num_pages > INT || a.table_pages < 0 || a.table_pages > INT ||
+        a.table_stride < 0 || a.table_stride > INT || a.entries > 65535 || a.rows > INT || a.rows * a.num_heads > INT || a.window < 0 || a.window > INT ||
+        !(a.scale > 0.0) || !(a.scale < 3e38) || !a.status)
         return (int)cudaErrorInvalidValue;
-    if (row_tile && (dtype != EG_BF16 || (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256) || page_size % 16 || (uintptr_t)q % 4 || ldq % 2 ||
-                     (uintptr_t)out % 4 || ldo % 2 || (uintptr_t)k_cache % 16 || (uintptr_t)v_cache % 16 || page_stride % 8 || head_stride % 8))
+    const int dim = (int)a.head_dim, group = (int)(a.num_heads / a.num_kv_heads);
+    // what the tensor-core kernels ask of addresses and strides
+    const long long rows_at = (long long)((uintptr_t)a.q | (uintptr_t)a.out) | (a.ldq | a.ldo) * 2;
+    const bool tiled = a.dtype == EG_BF16 && (((uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.page_stride | a.head_stride) & 7) == 0 && rows_at % 4 == 0;
+    const int aligned = !tiled ? 0 : rows_at % 16 || a.page_stride % dim || a.head_stride % dim || a.page_stride <= 0 || a.head_stride <= 0 ? 1 : 2;
+    int plan[3] = {(int)a.row_tile, (int)a.max_parts, (int)a.part_tiles};
+    if (a.row_tile < 0) {
+        const int code = eg_attention_tree_plan((int)a.dtype, aligned, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
+                                                (int)(a.max_context < 1 ? 1 : a.max_context > INT ? INT : a.max_context), eg_sm_count(), plan);
+        if (code) return code;
+    } else if ((a.row_tile && a.row_tile != 16 && a.row_tile != 32 && a.row_tile != 64 && a.row_tile != 128) || a.max_parts < 1 || a.max_parts > tree::MAX_PARTS ||
+               (a.max_parts & (a.max_parts - 1)) || a.part_tiles < 1 || a.part_tiles > 1 << 20) {
         return (int)cudaErrorInvalidValue;
-    if (row_tile == 128 && ((head_dim != 64 && head_dim != 128) || num_heads / num_kv_heads > 128 || (uintptr_t)q % 16 || ldq % 8 || (uintptr_t)out % 16 || ldo % 8 ||
-                            page_stride % head_dim || head_stride % head_dim || page_stride <= 0 || head_stride <= 0))
-        return (int)cudaErrorInvalidValue;
+    }
+    const int row_tile = plan[0];
+    if (row_tile && (!tiled || (dim != 32 && dim != 64 && dim != 128 && dim != 256) || a.page_size % 16)) return (int)cudaErrorInvalidValue;
+    if (row_tile == 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
     const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
-    const long long tiles = (long long)rows * (num_heads / num_kv_heads) / tile_rows + entries; // at most: every entry's last tile may be a short one
-    if (tiles > 65535 || (long long)rows * num_heads > 0x7fffffff) return (int)cudaErrorInvalidValue;
-    const Params p = {q, ldq, k_cache, v_cache, page_stride, head_stride, block_table, table_stride, table_pages, num_pages, entry_starts, context, parents, out, ldo,
-                      rows, entries, num_heads, num_kv_heads, head_dim, page_size, window, scale, max_parts, part_tiles * (64 / tile_keys), status};
+    const long long tiles = a.rows * group / tile_rows + a.entries;   // at most: every entry's last tile may be a short one
+    if (tiles > 65535) return (int)cudaErrorInvalidValue;
+    const Params p = {a.q, a.ldq, a.k_cache, a.v_cache, a.page_stride, a.head_stride, a.block_table, (int)a.table_stride, (int)a.table_pages, (int)a.num_pages,
+                      a.entry_starts, a.context, a.parents, a.out, a.ldo, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
+                      (int)a.window, (float)a.scale, plan[1], plan[2] * (64 / tile_keys), a.status};
     if (row_tile == 128) return tree::launch_tc(stream, p);
     if (row_tile) return tree::launch_mma(stream, p, row_tile, (int)tiles);
-    if (dtype == EG_F32)
-        return head_dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);
-    return head_dim <= 64 ? launch<bf16, 64>(stream, p, (int)tiles) : head_dim <= 128 ? launch<bf16, 128>(stream, p, (int)tiles) : launch<bf16, 256>(stream, p, (int)tiles);
+    if (a.dtype == EG_F32)
+        return dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);
+    return dim <= 64 ? launch<bf16, 64>(stream, p, (int)tiles) : dim <= 128 ? launch<bf16, 128>(stream, p, (int)tiles) : launch<bf16, 256>(stream, p, (int)tiles);
 }

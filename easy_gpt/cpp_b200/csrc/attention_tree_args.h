@@ -1,0 +1,22 @@
+/* What eg_attention_tree (attention_tree.cu) is given: one block of 8-byte fields, so that a caller in another language packs it in one go. */
+#ifndef EASY_GPT_ATTENTION_TREE_ARGS_H
+#define EASY_GPT_ATTENTION_TREE_ARGS_H
+
+typedef struct eg_attention_tree_args {
+    const void* q;                  /* [>= rows, ldq], num_heads * head_dim columns */
+    const void* k_cache;            /* [num_pages][num_kv_heads][page_size][head_dim], strides of pages and heads in elements */
+    const void* v_cache;            /* the same */
+    const int* block_table;         /* [entries, table_pages], row stride table_stride */
+    const int* entry_starts;        /* [entries + 1] */
+    const int* context;             /* [entries] */
+    const int* parents;             /* [rows] */
+    void* out;                      /* [>= rows, ldo] */
+    int* status;
+    long long dtype, ldq, ldo, page_stride, head_stride, table_stride, table_pages, num_pages, rows, entries, num_heads, num_kv_heads, head_dim, page_size;
+    long long window;               /* 0: none */
+    long long max_context;          /* the most keys an entry has, cached and its own, as far as known: how the work is split follows it */
+    long long row_tile, max_parts, part_tiles;      /* a plan (eg_attention_tree_plan); row_tile below 0: made by the call */
+    double scale;                   /* above 0 */
+} eg_attention_tree_args;
+
+#endif

@@ -134,6 +134,17 @@ static inline void eg_done_on_device(unsigned long long& seen, int device) {
     if (device >= 0) __atomic_fetch_or(&seen, 1ull << device, __ATOMIC_RELEASE);
 }
 
+// streaming multiprocessors of the current device
+static inline int eg_sm_count() {
+    static int counts[64] = {};
+    int device = 0, n = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return 148;
+    if (device >= 0 && device < 64 && (n = __atomic_load_n(&counts[device], __ATOMIC_RELAXED)) > 0) return n;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) return 148;
+    if (device >= 0 && device < 64) __atomic_store_n(&counts[device], n, __ATOMIC_RELAXED);
+    return n;
+}
+
 static inline int eg_launch_status() { return (int)cudaGetLastError(); }
 
 #ifdef EG_NEEDS_TENSOR_MAPS

@@ -5,6 +5,8 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include "../attention_tree_args.h"
+
 extern "C" {
 // activation.cu
 int eg_swiglu(cudaStream_t stream, int dtype, const void* gate_up, int ld, void* out, int ldo, int tokens, int inter);
@@ -228,7 +230,7 @@ int eg_attention_prefill_tcgen05_sigmoid_reach(void);
 // attention_tcgen05.cu
 int eg_attention_prefill_tcgen05_sigmoid(cudaStream_t stream, const void* q, long long ldq, int total_tokens, const void* k_cache, const void* v_cache, const int* block_table, int table_stride, const int* positions, const int* tiles, int num_tiles, void* out, long long ldo, int num_heads, int num_kv_heads, int head_dim, int page_size, long long page_stride, long long head_stride, int num_pages, float scale, const float* bias_table, int reach, const float* gate, long long ld_gate, int* status, int max_parts, int part_tiles, float* partial_o, float* partial_ml, int* queue);
 // attention_tree.cu
-int eg_attention_tree(cudaStream_t stream, int dtype, const void* q, long long ldq, const void* k_cache, const void* v_cache, long long page_stride, long long head_stride, const int* block_table, int table_stride, int table_pages, int num_pages, const int* entry_starts, const int* context, const int* parents, void* out, long long ldo, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int window, float scale, int row_tile, int max_parts, int part_tiles, int* status);
+int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* args);
 int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count, int* plan);
 // sampling_min_p.cu
 int eg_sample_min_p(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* out);

@@ -8,11 +8,11 @@ library cannot be built or loaded, importing it raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import math
 import os
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
@@ -100,8 +100,7 @@ class _Signatures:
     eg_wait_probe = [c_void_p, ctypes.c_uint, c_int, c_void_p, c_void_p]
     eg_sample = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_sample_min_p = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
-    eg_attention_tree = [c_void_p, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_longlong, c_longlong, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
-                         c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p]
+    eg_attention_tree = [c_void_p, ctypes.c_char_p]
     eg_attention_tree_plan = [c_int] * 10 + [c_void_p]
     eg_tree_accept = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_cache_keep = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_void_p, c_int, c_int,
@@ -174,18 +173,20 @@ def _cuda(*tensors) -> None:
             raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
 
 
-_here = contextlib.nullcontext()
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _on(*tensors):
-    """CUDA tensors of one device, and that device as the current one for the launch."""
-    device = tensors[0].device
+def _device_of(*tensors) -> int:
+    """The one CUDA device of the tensors."""
+    device = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
-            raise KernelError("kernels run on CUDA tensors only; there is no CPU path")
-        if t.device != device:
-            raise KernelError("tensors of one device")
-    return _here if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        if t.get_device() != device or device < 0:
+            raise KernelError("kernels run on CUDA tensors only, all of one device; there is no CPU path")
+    return device
+
+
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def embedding_gather(ids: torch.Tensor, table: torch.Tensor, residual: torch.Tensor, status: torch.Tensor) -> None:
@@ -918,43 +919,41 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor,
                                _ptr(top_k), _ptr(top_p), _ptr(uniform), _ptr(out)), "sample")
 
 
+SAMPLE_MAX_VOCAB = 1 << 20
+_F32, _I32 = torch.float32, torch.int32
+
+
 def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
                  uniform: torch.Tensor, out: torch.Tensor) -> None:
     """``sample`` with a further cut, and with its sums in 64 bits: per row temperature <= 0 -> greedy; else softmax(logits / T)
     cut by top_k (0 = off), then top_p (1 = off), then to the tokens with at least min_p times the largest one's probability
     (0 = off), drawn by inverse CDF in index order with uniform[r].  Ties go to the lower index; NaN is never kept; tokens of less
     than 2^-43 of the largest one's probability are never drawn; a row without a number above -inf gives 0."""
-    with _on(logits, temperature, top_k, top_p, min_p, uniform, out):
-        _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1, "float32 rows")
-        rows, vocab = logits.shape
-        _need(1 <= vocab <= SAMPLE_MAX_VOCAB, f"1 to {SAMPLE_MAX_VOCAB} logits a row")
-        _need(temperature.dtype == top_p.dtype == min_p.dtype == uniform.dtype == torch.float32 and top_k.dtype == out.dtype == torch.int32,
-              "float32 temperature/top_p/min_p/uniform, int32 top_k/out")
-        for t in (temperature, top_k, top_p, min_p, uniform, out):
-            _need(t.numel() >= rows and t.is_contiguous(), "one value per row, contiguous")
-        _check(library().eg_sample_min_p(_stream(), _ptr(logits), logits.stride(0), rows, vocab, _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                                         _ptr(min_p), _ptr(uniform), _ptr(out)), "sample_min_p")
+    device = _device_of(logits, temperature, top_k, top_p, min_p, uniform, out)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return sample_min_p(logits, temperature, top_k, top_p, min_p, uniform, out)
+    if logits.dim() != 2 or logits.dtype is not _F32:
+        raise KernelError("float32 rows")
+    (rows, vocab), (ld, step) = logits.shape, logits.stride()
+    if step != 1 or ld < 0 or not 1 <= vocab <= SAMPLE_MAX_VOCAB:
+        raise KernelError(f"rows of 1 to {SAMPLE_MAX_VOCAB} logits, side by side")
+    for t, dtype in ((temperature, _F32), (top_k, _I32), (top_p, _F32), (min_p, _F32), (uniform, _F32), (out, _I32)):
+        if t.dtype is not dtype or t.numel() < rows or not t.is_contiguous():
+            raise KernelError("float32 temperature/top_p/min_p/uniform, int32 top_k/out, one value per row, contiguous")
+    _check(library().eg_sample_min_p(_stream_of(device), logits.data_ptr(), ld, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+                                     min_p.data_ptr(), uniform.data_ptr(), out.data_ptr()), "sample_min_p")
 
 
-SAMPLE_MAX_VOCAB = 1 << 20
-
-
-def _tree_alignment(q, k_cache, v_cache, out) -> int:
-    """What attention_tree_plan calls aligned: 2 rows of q and out on 16-byte boundaries, 1 on 4-byte ones, 0 neither or caches that are not."""
-    es, pages, heads = q.element_size(), k_cache.stride(0), k_cache.stride(1)
-    rows = q.data_ptr() | out.data_ptr() | (q.stride(0) | out.stride(0)) * es
-    if (k_cache.data_ptr() | v_cache.data_ptr() | (pages | heads) * es) % 16 or rows % 4:
-        return 0
-    return 1 if rows % 16 or pages % k_cache.shape[3] or heads % k_cache.shape[3] or not pages or not heads else 2
-
-
-@functools.lru_cache(maxsize=4096)
 def attention_tree_plan(dtype: int, aligned: int, rows: int, entries: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_context: int):
     """(rows of a CTA: 128 the tcgen05 kernel, 16 to 64 the warp-level one, 0 the 32-bit one; the most parts a row tile's keys are cut into; the fewest
-    times 64 keys of a part)."""
+    times 64 keys of a part) that ``attention_tree`` goes by; aligned: 2 rows of q and out on 16-byte boundaries, 1 on 4-byte ones, 0 neither."""
     plan = (c_int * 3)()
     _need(library().eg_attention_tree_plan(dtype, aligned, rows, entries, num_heads, num_kv_heads, head_dim, page_size, max_context, sm_count(), plan) == 0, "sizes of a step")
     return tuple(plan)
+
+
+_pack_attention_tree = struct.Struct("=28qd").pack         # the fields of attention_tree_args.h
 
 
 def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, entry_starts: torch.Tensor,
@@ -962,35 +961,47 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                    window: Optional[int], scale: float, status: torch.Tensor, max_context: Optional[int] = None) -> None:
     """Attention of drafted trees over the paged cache.  Entry r's nodes are the rows entry_starts[r] .. entry_starts[r + 1] - 1 of q
     [>= T, >= NH*HD] and out [>= T, >= NH*HD] (rows behind the last entry's are left as they are), numbered from 0; parents[row] of
-    parents [T] is the number of a node's parent, lower than its own, or -1.  context[r] keys are cached before the step; node i's keys and values were stored at
-    cache position context[r] + i (and rotated at position context[r] + depth).  A node sees the cached keys, its ancestors and itself;
-    with a window, those of them whose position is above its own minus the window.  Caches [pages, NKV, page_size, HD], block_table
-    [entries, pages of a request], all int32 but q, out and the caches (float32 or bfloat16).  ``max_context``: the most keys an entry
-    has, cached and its own, as far as the caller knows (how the work is split follows it; by default what the block table has room for).
-    Bits of ``status``: 16 rows or a parent that cannot be (such rows are left, such a node has no parent), 2 a page that is none (its
-    keys are not seen)."""
-    with _on(q, k_cache, v_cache, block_table, entry_starts, context, parents, out, status):
-        T, entries, page_size, dtype = parents.numel(), block_table.shape[0], k_cache.shape[2], dtype_code(q.dtype)
-        _need(0 < num_kv_heads <= num_heads and num_heads % num_kv_heads == 0 and 0 < head_dim <= 256, "heads in whole groups, head sizes up to 256")
-        _need(q.dim() == 2 and out.dim() == 2 and q.stride(1) == 1 and out.stride(1) == 1 and q.dtype == out.dtype == k_cache.dtype == v_cache.dtype
-              and q.shape[1] >= num_heads * head_dim and out.shape[1] >= num_heads * head_dim and q.shape[0] >= T
-              and out.shape[0] >= T, "q/out/cache layout")
-        _need(block_table.dtype == entry_starts.dtype == context.dtype == parents.dtype == status.dtype == torch.int32 and block_table.dim() == 2
-              and (block_table.stride(1) == 1 or block_table.shape[1] <= 1), "int32 metadata")
-        _need(entry_starts.numel() == entries + 1 and context.numel() >= entries and entry_starts.is_contiguous() and context.is_contiguous()
-              and parents.is_contiguous(), "entry_starts [entries + 1], context [entries], contiguous parents")
-        _need(k_cache.dim() == 4 and tuple(k_cache.shape[1:]) == (num_kv_heads, page_size, head_dim) and k_cache.shape == v_cache.shape
-              and k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1 and k_cache.stride(2) == head_dim, "cache shape [pages, NKV, page_size, HD]")
-        _need((window is None or window > 0) and 0 < scale < math.inf, "a window of one key at least, a scale above 0")
-        if max_context is None:
-            max_context = block_table.shape[1] * page_size
-        row_tile, parts, part_tiles = attention_tree_plan(
-            dtype, _tree_alignment(q, k_cache, v_cache, out),
-            T, entries, num_heads, num_kv_heads, head_dim, page_size, int(max_context)) if T and entries else (0, 1, 1)
-        _check(library().eg_attention_tree(
-            _stream(), dtype, _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), k_cache.stride(0), k_cache.stride(1), _ptr(block_table),
-            block_table.stride(0), block_table.shape[1], k_cache.shape[0], _ptr(entry_starts), _ptr(context), _ptr(parents), _ptr(out), out.stride(0), T, entries,
-            num_heads, num_kv_heads, head_dim, page_size, int(window or 0), float(scale), row_tile, parts, part_tiles, _ptr(status)), "attention_tree")
+    parents [T] is the number of a node's parent, lower than its own, or -1.  context[r] keys are cached before the step; node i's keys
+    and values were stored at cache position context[r] + i (and rotated at position context[r] + depth).  A node sees the cached keys, its
+    ancestors and itself; with a window, those of them whose position is above its own minus the window.  Caches [pages, NKV, page_size,
+    HD], block_table [entries, pages of a request], all int32 but q, out and the caches (float32 or bfloat16).  scale is above 0.
+    ``max_context``: the most keys an entry has, cached and its own, as far as the caller knows (how the work is split follows it; by
+    default what the block table has room for).  Bits of ``status``: 16 rows or a parent that cannot be (such rows are left, such a node
+    has no parent), 2 a page that is none (its keys are not seen), 8 a bounded wait inside the kernel gave up."""
+    device = _device_of(q, k_cache, v_cache, block_table, entry_starts, context, parents, out, status)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return attention_tree(q, k_cache, v_cache, block_table, entry_starts, context, parents, out, num_heads, num_kv_heads, head_dim, window, scale, status,
+                                  max_context)
+    dtype, cache_shape, cache_stride = q.dtype, k_cache.shape, k_cache.stride()
+    code = dtype_code(dtype)
+    if out.dtype is not dtype or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+        raise KernelError("q, out and the caches of one dtype")
+    for t in (block_table, entry_starts, context, parents, status):
+        if t.dtype is not _I32:
+            raise KernelError("int32 metadata")
+    if not 0 < num_kv_heads <= num_heads or num_heads % num_kv_heads or not 0 < head_dim <= 256:
+        raise KernelError("heads in whole groups, head sizes up to 256")
+    if len(cache_shape) != 4 or cache_shape[1] != num_kv_heads or cache_shape[3] != head_dim or v_cache.shape != cache_shape or v_cache.stride() != cache_stride \
+            or cache_stride[3] != 1 or cache_stride[2] != head_dim:
+        raise KernelError("cache shape [pages, NKV, page_size, HD], equal strides, whole rows")
+    rows, q_shape, out_shape = parents.numel(), q.shape, out.shape
+    if len(q_shape) != 2 or len(out_shape) != 2 or q_shape[0] < rows or out_shape[0] < rows or q_shape[1] < num_heads * head_dim or out_shape[1] < num_heads * head_dim:
+        raise KernelError("q and out [>= T, >= NH*HD]")
+    (ldq, q_step), (ldo, out_step) = q.stride(), out.stride()
+    if q_step != 1 or out_step != 1 or block_table.dim() != 2:
+        raise KernelError("rows of q and out side by side, a block table [entries, pages]")
+    (entries, table_pages), (table_stride, table_step) = block_table.shape, block_table.stride()
+    if (table_step != 1 and table_pages > 1) or entry_starts.numel() != entries + 1 or context.numel() < entries or not entry_starts.is_contiguous() \
+            or not context.is_contiguous() or not parents.is_contiguous() or status.numel() < 1:
+        raise KernelError("block table rows, entry_starts [entries + 1], context [entries], parents [T], all contiguous")
+    if (window is not None and window <= 0) or not 0 < scale < math.inf:
+        raise KernelError("a window of one key at least, a scale above 0")
+    page_size = cache_shape[2]
+    _check(library().eg_attention_tree(_stream_of(device), _pack_attention_tree(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), entry_starts.data_ptr(), context.data_ptr(), parents.data_ptr(), out.data_ptr(),
+        status.data_ptr(), code, ldq, ldo, cache_stride[0], cache_stride[1], table_stride, table_pages, cache_shape[0], rows, entries, num_heads, num_kv_heads, head_dim,
+        page_size, window or 0, table_pages * page_size if max_context is None else max_context, -1, 1, 1, scale)), "attention_tree")
 
 
 def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch.Tensor, parents: torch.Tensor, path: torch.Tensor,
@@ -999,16 +1010,22 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch
     (``argmax`` or a sample of the row's logits), entry_starts and parents as in ``attention_tree``; all int32.  From node 0 of every entry
     (its last known token) the walk goes to the first child with the token that the model answered, and on.  path [entries, P]: the walk's
     nodes (at most P), then -1; accepted [entries]: how many they are; emitted [entries, P]: the model's answer at each, which is the entry's
-    new tokens (the last one is drafted by nobody), then -1.  An entry without rows accepts 0."""
-    with _on(tokens, targets, entry_starts, parents, path, accepted, emitted, status):
-        entries, rows = entry_starts.numel() - 1, tokens.numel()
-        for t in (tokens, targets, entry_starts, parents, path, accepted, emitted, status):
-            _need(t.dtype == torch.int32 and t.is_contiguous(), "contiguous int32 tensors")
-        _need(entries >= 0 and targets.numel() == rows and parents.numel() >= rows, "one target and one parent per token, entry_starts [entries + 1]")
-        _need(path.dim() == 2 and path.shape[0] == entries and path.shape[1] >= 1 and emitted.shape == path.shape and accepted.numel() >= entries,
-              "path and emitted [entries, P], accepted [entries]")
-        _check(library().eg_tree_accept(_stream(), _ptr(tokens), _ptr(targets), _ptr(entry_starts), _ptr(parents), entries, rows, path.shape[1], _ptr(path),
-                                        _ptr(accepted), _ptr(emitted), _ptr(status)), "tree_accept")
+    new tokens (the last one is drafted by nobody), then -1.  An entry without rows accepts 0.  Bit 16 of ``status``: rows or a parent that
+    cannot be."""
+    device = _device_of(tokens, targets, entry_starts, parents, path, accepted, emitted, status)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return tree_accept(tokens, targets, entry_starts, parents, path, accepted, emitted, status)
+    for t in (tokens, targets, entry_starts, parents, path, accepted, emitted, status):
+        if t.dtype is not _I32 or not t.is_contiguous():
+            raise KernelError("contiguous int32 tensors")
+    entries, rows, shape = entry_starts.numel() - 1, tokens.numel(), path.shape
+    if entries < 0 or targets.numel() != rows or parents.numel() < rows or status.numel() < 1:
+        raise KernelError("one target and one parent per token, entry_starts [entries + 1]")
+    if len(shape) != 2 or shape[0] != entries or shape[1] < 1 or emitted.shape != shape or accepted.numel() < entries:
+        raise KernelError("path and emitted [entries, P], accepted [entries]")
+    _check(library().eg_tree_accept(_stream_of(device), tokens.data_ptr(), targets.data_ptr(), entry_starts.data_ptr(), parents.data_ptr(), entries, rows, shape[1],
+                                    path.data_ptr(), accepted.data_ptr(), emitted.data_ptr(), status.data_ptr()), "tree_accept")
 
 
 def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, context: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor,
@@ -1018,19 +1035,27 @@ def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, context: torch.Tenso
     group's pool), through block_table [entries, pages of a request]; context, path [entries, P] and accepted as in ``tree_accept``.
     Bits of ``status``: 16 a path that does not ascend, or accepted outside 0 .. P (nothing of that request is moved), 2 a page that is none
     (that row is not moved)."""
-    with _on(kv, block_table, context, path, accepted, status):
-        _need(kv.dim() == 6 and kv.shape[2] == 2 and kv.element_size() in (2, 4) and (kv.shape[5] == 1 or kv.stride(5) == 1)
-              and (kv.shape[4] == 1 or kv.stride(4) == kv.shape[5]), "kv [layers, pages, 2, NKV, page_size, HD] of 2 or 4 bytes, whole rows")
-        for t in (block_table, context, path, accepted, status):
-            _need(t.dtype == torch.int32, "int32 metadata")
-        entries = path.shape[0]
-        _need(path.dim() == 2 and path.is_contiguous() and path.shape[1] >= 1 and accepted.numel() >= entries and context.numel() >= entries
-              and accepted.is_contiguous() and context.is_contiguous(), "path [entries, P], accepted and context [entries]")
-        _need(block_table.dim() == 2 and block_table.shape[0] >= entries and (block_table.stride(1) == 1 or block_table.shape[1] <= 1), "block table")
-        layers, pages, _, kv_heads, page_size, head_dim = kv.shape
-        _check(library().eg_cache_keep(_stream(), _ptr(kv), kv.element_size(), layers, pages, kv_heads, page_size, head_dim, kv.stride(0), kv.stride(1), kv.stride(2),
-                                       kv.stride(3), _ptr(block_table), block_table.stride(0), block_table.shape[1], _ptr(context), _ptr(path), _ptr(accepted),
-                                       entries, path.shape[1], _ptr(status)), "cache_keep")
+    device = _device_of(kv, block_table, context, path, accepted, status)
+    if device != _current_device():
+        with torch.cuda.device(device):
+            return cache_keep(kv, block_table, context, path, accepted, status)
+    for t in (context, path, accepted, status):
+        if t.dtype is not _I32 or not t.is_contiguous():
+            raise KernelError("contiguous int32 context, path, accepted and status")
+    shape, path_shape, table_shape, element_size = kv.shape, path.shape, block_table.shape, kv.element_size()
+    if len(shape) != 6 or shape[2] != 2 or element_size not in (2, 4):
+        raise KernelError("kv [layers, pages, 2, NKV, page_size, HD] of 2 or 4 bytes")
+    layers, pages, _, kv_heads, page_size, head_dim = shape
+    layer_stride, page_stride, plane_stride, head_stride, row_stride, step = kv.stride()
+    if (step != 1 and head_dim > 1) or (row_stride != head_dim and page_size > 1):
+        raise KernelError("kv's pages in whole rows")
+    if len(path_shape) != 2 or path_shape[1] < 1 or accepted.numel() < path_shape[0] or context.numel() < path_shape[0] or status.numel() < 1:
+        raise KernelError("path [entries, P], accepted and context [entries]")
+    if block_table.dtype is not _I32 or len(table_shape) != 2 or table_shape[0] < path_shape[0] or (block_table.stride(1) != 1 and table_shape[1] > 1):
+        raise KernelError("an int32 block table [entries, pages]")
+    _check(library().eg_cache_keep(_stream_of(device), kv.data_ptr(), element_size, layers, pages, kv_heads, page_size, head_dim, layer_stride, page_stride, plane_stride,
+                                   head_stride, block_table.data_ptr(), block_table.stride(0), table_shape[1], context.data_ptr(), path.data_ptr(), accepted.data_ptr(),
+                                   path_shape[0], path_shape[1], status.data_ptr()), "cache_keep")
 
 
 def wait_probe(limit: int, threads: int, status: torch.Tensor) -> int:

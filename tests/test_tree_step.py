@@ -1,5 +1,4 @@
 """What the operators of a step over drafted trees refuse before anything is launched (no GPU): by their Python faces, and by the launchers alone."""
-import contextlib
 import math
 
 import pytest
@@ -18,10 +17,10 @@ def on_the_host(monkeypatch):
     def reached():
         raise Reached
 
-    monkeypatch.setattr(kernels, "_on", lambda *tensors: contextlib.nullcontext())
+    monkeypatch.setattr(kernels, "_device_of", lambda *tensors: 0)
+    monkeypatch.setattr(kernels, "_current_device", lambda: 0)
     monkeypatch.setattr(kernels, "library", reached)
-    monkeypatch.setattr(kernels, "attention_tree_plan", lambda *sizes: (16, 1, 1))
-    monkeypatch.setattr(kernels, "_stream", lambda: 0)
+    monkeypatch.setattr(kernels, "_stream_of", lambda device: 0)
 
 
 def i32(*shape):
@@ -88,13 +87,28 @@ def test_launchers_refuse_sizes_they_do_not_take():
     assert [keep(size=1), keep(size=8), keep(pages=0), keep(heads=0), keep(page=0), keep(dim=0), keep(longest=0), keep(status=None), keep(entries=65536), keep(kv=at + 1),
             keep(layers=1 << 30)] == [1] * 11
 
-    def attend(dtype=kernels.BF16, rows=4, entries=1, heads=4, kv_heads=2, dim=64, page=16, pages=4, parts=1, tiles=1, status=at,
-               q=at, ldq=256, row_tile=0, scale=0.125):
-        return lib.eg_attention_tree(None, dtype, q, ldq, at, at, 4096, 1024, at, 3, 3, pages, at, at, at, at, 256, rows, entries, heads, kv_heads, dim, page, 0, scale, row_tile, parts, tiles,
-                                     status)
+    def attend(dtype=kernels.BF16, rows=4, entries=1, heads=4, kv_heads=2, dim=64, page=16, pages=4, parts=1, tiles=1, status=at, q=at, ldq=256, row_tile=0, scale=0.125,
+               window=0, table_pages=3, cache=at):
+        return lib.eg_attention_tree(None, kernels._pack_attention_tree(q, cache, cache, at, at, at, at, at, status, dtype, ldq, 256, 4096, 1024, 3, table_pages, pages, rows, entries, heads,
+                                                                        kv_heads, dim, page, window, 100, row_tile, parts, tiles, scale))
 
     assert [attend(rows=0), attend(entries=0)] == [0, 0]
-    assert [attend(dtype=2), attend(heads=3), attend(kv_heads=0), attend(dim=0), attend(dim=257), attend(page=0), attend(pages=0), attend(parts=0), attend(tiles=0), attend(parts=3),
-            attend(parts=32), attend(status=None), attend(entries=65536), attend(rows=1 << 30)] == [1] * 14
-    assert [attend(row_tile=8), attend(row_tile=16, dtype=kernels.F32), attend(row_tile=16, dim=80), attend(row_tile=64, page=24), attend(row_tile=32, q=at + 2), attend(scale=0.0), attend(scale=-1.0), attend(row_tile=128, dim=32), attend(row_tile=128, q=at + 8),
-            attend(row_tile=16, ldq=257)] == [1] * 10
+    assert lib.eg_attention_tree(None, None) == 1
+    for wrong in (dict(dtype=2), dict(heads=3), dict(kv_heads=0), dict(dim=0), dict(dim=257), dict(page=0), dict(pages=0), dict(parts=0), dict(tiles=0), dict(parts=3), dict(parts=32), dict(status=0),
+                  dict(entries=65536), dict(rows=1 << 30), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(window=-1), dict(table_pages=-1), dict(row_tile=8),
+                  dict(row_tile=16, dtype=kernels.F32), dict(row_tile=16, dim=80), dict(row_tile=64, page=24), dict(row_tile=32, q=at + 2), dict(row_tile=16, ldq=257),
+                  dict(row_tile=16, cache=at + 8), dict(row_tile=128, dim=32), dict(row_tile=128, q=at + 8), dict(row_tile=128, dim=128, ldq=260), dict(row_tile=128, heads=258)):
+        assert attend(**wrong) == 1, wrong
+
+
+def test_plans():
+    """From sizes alone: few rows on the warp-level kernel, many on tcgen05, what neither takes on the 32-bit one; more parts the fewer units there are."""
+    plan = kernels.attention_tree_plan
+    assert plan(kernels.F32, 2, 8, 1, 14, 2, 64, 16, 500)[0] == plan(kernels.BF16, 2, 8, 1, 14, 2, 80, 16, 500)[0] == plan(kernels.BF16, 2, 8, 1, 14, 2, 64, 24, 500)[0] == 0
+    assert plan(kernels.BF16, 0, 8, 1, 14, 2, 64, 16, 500)[0] == 0
+    assert [plan(kernels.BF16, 2, n, 1, 14, 2, 64, 16, 500)[0] for n in (1, 2, 4, 64)] == [16, 16, 32, 128]
+    assert plan(kernels.BF16, 1, 64, 1, 14, 2, 64, 16, 500)[0] == plan(kernels.BF16, 2, 64, 1, 14, 2, 32, 16, 500)[0] == 64
+    for aligned in (0, 1, 2):
+        for nodes in (1, 9, 64, 300):
+            parts = [plan(kernels.BF16, aligned, nodes * entries, entries, 28, 4, 128, 64, 32768)[1] for entries in (1, 4, 16, 64, 256)]
+            assert parts == sorted(parts, reverse=True) and all(p in (1, 2, 4, 8, 16) for p in parts) and parts[-1] == 1 or aligned == 2
