@@ -3,10 +3,12 @@
 //
 // A CTA takes 64 rows (node, query head) of an entry and KV head and a part of the keys, 32 at a time, in shared memory as float32; 256
 // threads have 4 rows x 2 keys of the scores and 4 rows x (head size / 16) columns of the output each.  Sums, reference and exponents are
-// 32-bit, the reference is the running maximum.
+// 32-bit, the reference is the running maximum.  Where rows of float32 are whole 16-byte pieces, the next tile comes by
+// asynchronous copies while this one is worked on; else a tile is read and converted when it is its turn.  Bound by the multiply-adds, and with few
+// keys a part by the trips to memory in front of the first tile.
 //
-// Which keys a row sees is decided by a select, never by adding: a hidden score may be anything.  A hidden value takes part as 0 * v, so
-// values that are not finite are put aside as zeros and added where they are seen.
+// Which keys a row sees is decided by a select, never by adding: a hidden score may be anything.  A hidden value takes part as 0 * v; where
+// there are values that are not finite, every row leaves out those that it does not see.
 #include "attention_tree.cuh"
 #include "attention_tree_args.h"
 
@@ -17,28 +19,30 @@ using tree::Params;
 
 constexpr int TC_LINES = 64;                                         // rows of an entry and KV head from which on the tcgen05 kernel takes them
 constexpr int ROWS = 64, KEYS = 32, THREADS = 256, STAGED_NODES = 1024;
+constexpr int LISTED = 16;                                           // key tiles whose places in the cache are looked up at a time
 
 template <int DMAX>
 struct Layout {
     static constexpr int LD = DMAX + 4;                              // floats of a row: eight rows' quads meet no bank twice
     static constexpr int P_LD = KEYS + 4;
-    static constexpr int FLOATS = ROWS * LD + 2 * KEYS * LD + ROWS * P_LD;
+    static constexpr int STAGE = 2 * KEYS * LD;                      // keys, then values
+    static constexpr int FLOATS = ROWS * LD + 2 * STAGE + ROWS * P_LD;
 };
 
-template <typename T, int DMAX>
-__global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p) {
+// ASYNC: float32 in whole 16-byte pieces, two stages of keys and values.
+template <typename T, int DMAX, bool ASYNC>
+__global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_kernel(const Params p) {
     using L = Layout<DMAX>;
     constexpr int COLS = DMAX / 64;                                  // quads of output columns a thread has
     extern __shared__ __align__(16) float smem[];
     float* const q_s = smem;
-    float* const k_s = q_s + ROWS * L::LD;
-    float* const v_s = k_s + KEYS * L::LD;
-    float* const p_s = v_s + KEYS * L::LD;
+    float* const ring = q_s + ROWS * L::LD;
+    float* const p_s = ring + 2 * L::STAGE;
     __shared__ int ups[STAGED_NODES];
-    __shared__ unsigned seen[ROWS];                                  // of a key tile, by row: a bit a key
+    __shared__ unsigned seen[ROWS];                                  // of a key tile that needs it, by row: a bit a key
     __shared__ int lowest[ROWS];                                     // a row's first cached key
-    __shared__ long long key_row[KEYS];                              // where a key's row lies in the cache; -1: there is none
-    __shared__ unsigned keys_there;
+    __shared__ int latest;                                           // the largest of those
+    __shared__ long long key_row[LISTED * KEYS];                     // where a key's row lies in the cache; -1: nowhere
     pdl_enter();
     const int part = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
     const int group = p.num_heads / p.num_kv_heads;
@@ -52,28 +56,92 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     if (part >= parts) return;
     const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
 
-    // ---- the tree: parents of the nodes up to the tile's last one, and every row's first cached key
+    bool hole = false;                                               // a page that is none has been met
+    auto list_keys = [&](int tile) {                                 // the places of tiles tile .. tile + LISTED - 1
+        for (int i = tid; i < LISTED * KEYS; i += THREADS) {
+            const int at = tile * KEYS + i, slot = at / p.page_size;
+            long long row = -1;
+            if (tile + i / KEYS < stop && at >= first && at < end) {
+                const int page = slot < p.table_pages ? p.block_table[(size_t)r * p.table_stride + slot] : -1;
+                if (page < 0 || page >= p.num_pages) {
+                    hole = true;
+                    atomicOr(p.status, EG_STATUS_BAD_PAGE);
+                } else {
+                    row = page * p.page_stride + kvh * p.head_stride + (long long)(at % p.page_size) * D;
+                }
+            }
+            key_row[i] = row;
+        }
+    };
+    auto stage_of = [&](int tile) { return ring + (ASYNC ? (tile - begin) & 1 : 0) * L::STAGE; };
+    auto load = [&](int tile) {
+        float* const k_s = stage_of(tile);
+        const long long* const rows = key_row + (tile - begin) % LISTED * KEYS;
+        if constexpr (ASYNC) {
+            constexpr int PIECES = DMAX / 4;
+#pragma unroll 4
+            for (int i = tid; i < KEYS * PIECES; i += THREADS) {
+                const int key = i / PIECES, d = i % PIECES * 4;
+                const long long row = rows[key];
+                const bool there = row >= 0 && d < D;
+                const size_t from = there ? (size_t)(row + d) : 0;
+                const unsigned to = (unsigned)__cvta_generic_to_shared(k_s + key * L::LD + d);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(static_cast<const float*>(p.k_cache) + from), "r"(there ? 16 : 0));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to + 4 * KEYS * L::LD), "l"(static_cast<const float*>(p.v_cache) + from),
+                             "r"(there ? 16 : 0));
+            }
+        } else {
+#pragma unroll 8
+            for (int i = tid; i < KEYS * DMAX; i += THREADS) {
+                const int key = i / DMAX, d = i % DMAX;
+                const long long row = rows[key];
+                float k = 0.f, v = 0.f;
+                if (d < D && row >= 0) {
+                    k = to_f32<T>(static_cast<const T*>(p.k_cache)[row + d]);
+                    v = to_f32<T>(static_cast<const T*>(p.v_cache)[row + d]);
+                }
+                k_s[key * L::LD + d] = k;
+                k_s[(KEYS + key) * L::LD + d] = v;
+            }
+        }
+    };
+    // ---- the rows of q
+    if constexpr (ASYNC) {
+        for (int i = tid; i < ROWS * (DMAX / 4); i += THREADS) {
+            const int row = i / (DMAX / 4), d = i % (DMAX / 4) * 4, node = (row0 + row) / group, head = kvh * group + (row0 + row) % group;
+            const bool there = row < count && d < D;
+            const size_t from = there ? (size_t)(e.first + node) * p.ldq + (size_t)head * D + d : 0;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"((unsigned)__cvta_generic_to_shared(q_s + row * L::LD + d)),
+                         "l"(static_cast<const float*>(p.q) + from), "r"(there ? 16 : 0));
+        }
+    } else {
+#pragma unroll 8
+        for (int i = tid; i < ROWS * DMAX; i += THREADS) {
+            const int row = i / DMAX, d = i % DMAX, node = (row0 + row) / group, head = kvh * group + (row0 + row) % group;
+            float x = 0.f;
+            if (row < count && d < D) x = to_f32<T>(static_cast<const T*>(p.q)[(size_t)(e.first + node) * p.ldq + (size_t)head * D + d]);
+            q_s[row * L::LD + d] = x;
+        }
+    }
+    list_keys(begin);
     for (int i = tid; i <= last_node && i < STAGED_NODES; i += THREADS) ups[i] = tree::parent_of(p, e, i);
+    if (tid == 0) latest = 0;
     __syncthreads();
+    if (ASYNC) {
+        load(begin);
+        asm volatile("cp.async.commit_group;\n" ::);
+    }
+    // ---- every row's first cached key
     auto up_of = [&](int i) { return i < STAGED_NODES ? ups[i] : tree::parent_of(p, e, i); };
     if (tid < ROWS) {
         int low = 0;
         if (p.window > 0 && tid < count) {
             int depth = 0;
             for (int i = up_of((row0 + tid) / group); i >= 0; i = up_of(i)) ++depth;
-            low = max(0ll, (long long)e.context + depth - p.window + 1);
+            low = (int)max(0ll, (long long)e.context + depth - p.window + 1);
+            atomicMax(&latest, low);
         }
         lowest[tid] = low;
-    }
-    // ---- the rows of q
-    for (int i = tid; i < ROWS * DMAX; i += THREADS) {
-        const int row = i / DMAX, d = i % DMAX;
-        float x = 0.f;
-        if (row < count && d < D) {
-            const int node = (row0 + row) / group, head = kvh * group + (row0 + row) % group;
-            x = to_f32<T>(static_cast<const T*>(p.q)[(size_t)(e.first + node) * p.ldq + (size_t)head * D + d]);
-        }
-        q_s[row * L::LD + d] = x;
     }
     const int tx = tid & 15, ty = tid >> 4;                          // keys tx, tx + 16; rows 4 ty ..; columns 4 tx + 64 c ..
     const float scale_log2 = p.scale * 1.4426950408889634f;
@@ -87,47 +155,53 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     }
     for (int tile = begin; tile < stop; ++tile) {
         const int key0 = tile * KEYS;
-        __syncthreads();                                             // the last tile has been read
-        if (tid < KEYS) {
-            const int at = key0 + tid, slot = at / p.page_size;
-            long long row = -1;
-            if (at >= first && at < end) {
-                const int page = slot < p.table_pages ? p.block_table[(size_t)r * p.table_stride + slot] : -1;
-                if (page < 0 || page >= p.num_pages) atomicOr(p.status, EG_STATUS_BAD_PAGE);
-                else row = page * p.page_stride + kvh * p.head_stride + (long long)(at % p.page_size) * D;
+        if constexpr (ASYNC) {
+            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+            __syncthreads();                                         // this tile is there, the last one has been read
+            if (tile + 1 < stop) {
+                if ((tile + 1 - begin) % LISTED == 0) {
+                    list_keys(tile + 1);
+                    __syncthreads();
+                }
+                load(tile + 1);
             }
-            key_row[tid] = row;
-            const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
-            if (tid == 0) keys_there = there;
-        }
-        __syncthreads();
-        bool odd = false;                                            // a value that is not finite
-        for (int i = tid; i < KEYS * DMAX; i += THREADS) {
-            const int key = i / DMAX, d = i % DMAX;
-            const long long row = key_row[key];
-            float k = 0.f, v = 0.f;
-            if (d < D && row >= 0) {
-                k = to_f32<T>(static_cast<const T*>(p.k_cache)[row + d]);
-                v = to_f32<T>(static_cast<const T*>(p.v_cache)[row + d]);
+            asm volatile("cp.async.commit_group;\n" ::);
+        } else {
+            __syncthreads();
+            if (tile > begin && (tile - begin) % LISTED == 0) {
+                list_keys(tile);
+                __syncthreads();
             }
-            odd |= !isfinite(v);
-            k_s[key * L::LD + d] = k;
-            v_s[key * L::LD + d] = v;
+            load(tile);
+            __syncthreads();
         }
-        if (tid < ROWS) {
-            unsigned bits = 0;
-            if (tid < count) {
-                const int low = max(lowest[tid], key0), high = min(e.context, key0 + KEYS);      // the cached keys that it sees
-                if (low < high) bits = 0xffffffffu >> (KEYS - (high - low)) << (low - key0);
-                int left = p.window > 0 ? p.window : 0x7fffffff;
-                for (int i = (row0 + tid) / group; i >= 0 && e.context + i >= key0 && left > 0; i = up_of(i), --left)
-                    if (e.context + i < key0 + KEYS) bits |= 1u << (e.context + i - key0);
+        const float* const k_s = stage_of(tile);
+        const float* const v_s = k_s + KEYS * L::LD;
+        // ---- a tile that reaches into the tree, over a window's edge or onto a page that is none (of this run of tiles): which keys a row sees
+        bool masked = key0 + KEYS > e.context || key0 < max(first, latest), odd = false;
+        masked = __syncthreads_or(masked || hole);
+        if (masked) {
+            if (tid < ROWS) {
+                unsigned bits = 0;
+                if (tid < count) {
+                    const int low = max(max(lowest[tid], first), key0), high = min(e.context, key0 + KEYS);      // the cached keys that it sees
+                    if (low < high) bits = 0xffffffffu >> (KEYS - (high - low)) << (low - key0);
+                    int left = p.window > 0 ? p.window : 0x7fffffff;
+                    for (int i = (row0 + tid) / group; i >= 0 && e.context + i >= key0 && left > 0; i = up_of(i), --left)
+                        if (e.context + i < key0 + KEYS) bits |= 1u << (e.context + i - key0);
+                    for (int key = 0; key < KEYS; ++key) {           // on pages that are there
+                        const int slot = (key0 + key) / p.page_size, page = slot < p.table_pages ? p.block_table[(size_t)r * p.table_stride + slot] : -1;
+                        if ((bits >> key & 1) && (page < 0 || page >= p.num_pages)) bits &= ~(1u << key);
+                    }
+                }
+                seen[tid] = bits;
             }
-            seen[tid] = bits & keys_there;
+            for (int i = tid; i < KEYS * DMAX; i += THREADS) odd |= !isfinite(v_s[i / DMAX * L::LD + i % DMAX]);
+            odd = __syncthreads_or(odd);
         }
-        odd = __syncthreads_or(odd);
         // ---- scores
         float s[4][2] = {};
+#pragma unroll 8
         for (int d = 0; d < DMAX; d += 4) {
             float4 a[4], b[2];
 #pragma unroll
@@ -141,7 +215,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const unsigned bits = seen[4 * ty + i];
+            const unsigned bits = masked ? seen[4 * ty + i] : ~0u;
             float top = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -170,22 +244,37 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
         }
         __syncwarp();                                                // a row's weights come from its own half warp
         // ---- output
-        for (int key = 0; key < KEYS; ++key) {
-            float w[4];
+        if (!odd) {
+#pragma unroll 2
+            for (int key = 0; key < KEYS; key += 4) {
+                float4 w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = p_s[(4 * ty + i) * L::P_LD + key];
+                for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(p_s + (4 * ty + i) * L::P_LD + key);
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-                float4 v = *reinterpret_cast<const float4*>(v_s + key * L::LD + 4 * tx + 64 * c);
+                for (int c = 0; c < COLS; ++c) {
+                    float4 v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (odd && !(seen[4 * ty + i] >> key & 1)) continue;
-                    acc[i][c][0] = fmaf(w[i], v.x, acc[i][c][0]);
-                    acc[i][c][1] = fmaf(w[i], v.y, acc[i][c][1]);
-                    acc[i][c][2] = fmaf(w[i], v.z, acc[i][c][2]);
-                    acc[i][c][3] = fmaf(w[i], v.w, acc[i][c][3]);
+                    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const float4*>(v_s + (key + x) * L::LD + 4 * tx + 64 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[i][c][0] = fmaf(w[i].w, v[3].x, fmaf(w[i].z, v[2].x, fmaf(w[i].y, v[1].x, fmaf(w[i].x, v[0].x, acc[i][c][0]))));
+                        acc[i][c][1] = fmaf(w[i].w, v[3].y, fmaf(w[i].z, v[2].y, fmaf(w[i].y, v[1].y, fmaf(w[i].x, v[0].y, acc[i][c][1]))));
+                        acc[i][c][2] = fmaf(w[i].w, v[3].z, fmaf(w[i].z, v[2].z, fmaf(w[i].y, v[1].z, fmaf(w[i].x, v[0].z, acc[i][c][2]))));
+                        acc[i][c][3] = fmaf(w[i].w, v[3].w, fmaf(w[i].z, v[2].w, fmaf(w[i].y, v[1].w, fmaf(w[i].x, v[0].w, acc[i][c][3]))));
+                    }
                 }
             }
+        } else {
+            for (int key = 0; key < KEYS; ++key)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!(seen[4 * ty + i] >> key & 1)) continue;
+                    const float w = p_s[(4 * ty + i) * L::P_LD + key];
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[i][c][x] = fmaf(w, v_s[key * L::LD + 4 * tx + 64 * c + x], acc[i][c][x]);
+                }
         }
     }
     // where a row's results go
@@ -208,7 +297,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     }
     __syncthreads();                                                 // q, keys and values have been read
     float* const o_s = q_s;
-    float* const ml_s = k_s;
+    float* const ml_s = ring;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -225,12 +314,16 @@ __global__ void __launch_bounds__(THREADS) attention_tree_kernel(const Params p)
     });
 }
 
-template <typename T, int DMAX>
+template <typename T, int DMAX, bool ASYNC>
 int launch(cudaStream_t stream, const Params& p, int tiles) {
     constexpr int bytes = Layout<DMAX>::FLOATS * 4;
     static unsigned long long seen = 0;
-    if (const int code = tree::prepare_kernel(attention_tree_kernel<T, DMAX>, bytes, seen)) return code;
-    return tree::launch_clusters(attention_tree_kernel<T, DMAX>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, p);
+    if (const int code = tree::prepare_kernel(attention_tree_kernel<T, DMAX, ASYNC>, bytes, seen)) return code;
+    return tree::launch_clusters(attention_tree_kernel<T, DMAX, ASYNC>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, p);
+}
+template <typename T, bool ASYNC>
+int launch_any(cudaStream_t stream, const Params& p, int tiles) {
+    return p.head_dim <= 64 ? launch<T, 64, ASYNC>(stream, p, tiles) : p.head_dim <= 128 ? launch<T, 128, ASYNC>(stream, p, tiles) : launch<T, 256, ASYNC>(stream, p, tiles);
 }
 
 }  // namespace
@@ -304,7 +397,7 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
                       (int)a.window, (float)a.scale, plan[1], plan[2] * (64 / tile_keys), a.status};
     if (row_tile == 128) return tree::launch_tc(stream, p);
     if (row_tile) return tree::launch_mma(stream, p, row_tile, (int)tiles);
-    if (a.dtype == EG_F32)
-        return dim <= 64 ? launch<float, 64>(stream, p, (int)tiles) : dim <= 128 ? launch<float, 128>(stream, p, (int)tiles) : launch<float, 256>(stream, p, (int)tiles);
-    return dim <= 64 ? launch<bf16, 64>(stream, p, (int)tiles) : dim <= 128 ? launch<bf16, 128>(stream, p, (int)tiles) : launch<bf16, 256>(stream, p, (int)tiles);
+    if (a.dtype == EG_BF16) return launch_any<bf16, false>(stream, p, (int)tiles);
+    const bool pieces = (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.ldq | a.page_stride | a.head_stride | a.head_dim) & 3) == 0;
+    return pieces ? launch_any<float, true>(stream, p, (int)tiles) : launch_any<float, false>(stream, p, (int)tiles);
 }
