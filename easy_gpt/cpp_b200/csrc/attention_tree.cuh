@@ -128,31 +128,30 @@ __device__ __forceinline__ void add_parts(const float* o, int ld, const float* m
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     cluster_barrier();
     const int quads = columns / 4;
+    constexpr int AT_ONCE = 8;                                       // parts whose numbers are asked for together
     for (int i = (int)rank * THREADS + (int)threadIdx.x; i < rows * quads; i += parts * THREADS) {
         const int row = i / quads, d = i % quads * 4;
-        float2 w[MAX_PARTS];
-#pragma unroll
-        for (int q = 0; q < MAX_PARTS; ++q) w[q] = q < parts ? remote_load2(remote(ml + 2 * row, q)) : make_float2(-INFINITY, 0.f);
         float top = -INFINITY, total = 0.f;
-#pragma unroll
-        for (int q = 0; q < MAX_PARTS; ++q) top = fmaxf(top, w[q].x);
-#pragma unroll
-        for (int q = 0; q < MAX_PARTS; ++q) {
-            w[q].x = w[q].x == -INFINITY ? 0.f : exp2f(w[q].x - top);
-            total = fmaf(w[q].x, w[q].y, total);
-        }
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q0 = 0; q0 < parts; q0 += AT_ONCE) {
+            float2 w[AT_ONCE];
+            float4 v[AT_ONCE];
 #pragma unroll
-        for (int q0 = 0; q0 < MAX_PARTS; q0 += 4) {
-            float4 v[4];
+            for (int q = 0; q < AT_ONCE; ++q) w[q] = q0 + q < parts ? remote_load2(remote(ml + 2 * row, q0 + q)) : make_float2(-INFINITY, 0.f);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = q0 + q < parts ? remote_load4(remote(o + row * ld + d, q0 + q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int q = 0; q < AT_ONCE; ++q) v[q] = q0 + q < parts ? remote_load4(remote(o + row * ld + d, q0 + q)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float now = top;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                sum.x = fmaf(w[q0 + q].x, v[q].x, sum.x);
-                sum.y = fmaf(w[q0 + q].x, v[q].y, sum.y);
-                sum.z = fmaf(w[q0 + q].x, v[q].z, sum.z);
-                sum.w = fmaf(w[q0 + q].x, v[q].w, sum.w);
+            for (int q = 0; q < AT_ONCE; ++q) now = fmaxf(now, w[q].x);
+            const float ref = now == -INFINITY ? 0.f : now, keep = exp2f(top - ref);
+            top = now;
+            total *= keep;
+            sum = make_float4(sum.x * keep, sum.y * keep, sum.z * keep, sum.w * keep);
+#pragma unroll
+            for (int q = 0; q < AT_ONCE; ++q) {
+                const float c = w[q].x == -INFINITY ? 0.f : exp2f(w[q].x - ref);
+                total = fmaf(c, w[q].y, total);
+                sum = make_float4(fmaf(c, v[q].x, sum.x), fmaf(c, v[q].y, sum.y), fmaf(c, v[q].z, sum.z), fmaf(c, v[q].w, sum.w));
             }
         }
         const float inv = total > 0.f ? 1.f / total : total;          // nothing seen: 0; NaN stays
