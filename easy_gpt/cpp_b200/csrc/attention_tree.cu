@@ -328,7 +328,7 @@ int launch_any(cudaStream_t stream, const Params& p, int tiles) {
 
 }  // namespace
 
-// How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (128: the tcgen05 kernel; 16, 32 or 64: the warp-level one;
+// How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (128 or 256: the tcgen05 kernel; 16, 32 or 64: the warp-level one;
 // 0: the 32-bit one),
 // plan[1] and plan[2] the max_parts and part_tiles of eg_attention_tree.  aligned: the caches, their pages and heads start on 16-byte boundaries, and
 // q, out and their rows on 16-byte (2) or 4-byte (1) ones.  max_context: the most keys of an entry, as far as known.
@@ -382,20 +382,20 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
         const int code = eg_attention_tree_plan((int)a.dtype, aligned, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
                                                 (int)(a.max_context < 1 ? 1 : a.max_context > INT ? INT : a.max_context), eg_sm_count(), plan);
         if (code) return code;
-    } else if ((a.row_tile && a.row_tile != 16 && a.row_tile != 32 && a.row_tile != 64 && a.row_tile != 128) || a.max_parts < 1 || a.max_parts > tree::MAX_PARTS ||
+    } else if ((a.row_tile && a.row_tile != 16 && a.row_tile != 32 && a.row_tile != 64 && a.row_tile != 128 && a.row_tile != 256) || a.max_parts < 1 || a.max_parts > tree::MAX_PARTS ||
                (a.max_parts & (a.max_parts - 1)) || a.part_tiles < 1 || a.part_tiles > 1 << 20) {
         return (int)cudaErrorInvalidValue;
     }
     const int row_tile = plan[0];
     if (row_tile && (!tiled || (dim != 32 && dim != 64 && dim != 128 && dim != 256) || a.page_size % 16)) return (int)cudaErrorInvalidValue;
-    if (row_tile == 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
+    if (row_tile >= 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
     const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
     const long long tiles = a.rows * group / tile_rows + a.entries;   // at most: every entry's last tile may be a short one
     if (tiles > 65535) return (int)cudaErrorInvalidValue;
     const Params p = {a.q, a.ldq, a.k_cache, a.v_cache, a.page_stride, a.head_stride, a.block_table, (int)a.table_stride, (int)a.table_pages, (int)a.num_pages,
                       a.entry_starts, a.context, a.parents, a.out, a.ldo, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
                       (int)a.window, (float)a.scale, plan[1], plan[2] * (64 / tile_keys), a.status};
-    if (row_tile == 128) return tree::launch_tc(stream, p);
+    if (row_tile >= 128) return tree::launch_tc(stream, p, row_tile / 128);
     if (row_tile) return tree::launch_mma(stream, p, row_tile, (int)tiles);
     if (a.dtype == EG_BF16) return launch_any<bf16, false>(stream, p, (int)tiles);
     const bool pieces = (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.ldq | a.page_stride | a.head_stride | a.head_dim) & 3) == 0;

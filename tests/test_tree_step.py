@@ -97,7 +97,7 @@ def test_launchers_refuse_sizes_they_do_not_take():
     for wrong in (dict(dtype=2), dict(heads=3), dict(kv_heads=0), dict(dim=0), dict(dim=257), dict(page=0), dict(pages=0), dict(parts=0), dict(tiles=0), dict(parts=3), dict(parts=32), dict(status=0),
                   dict(entries=65536), dict(rows=1 << 30), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(window=-1), dict(table_pages=-1), dict(row_tile=8),
                   dict(row_tile=16, dtype=kernels.F32), dict(row_tile=16, dim=80), dict(row_tile=64, page=24), dict(row_tile=32, q=at + 2), dict(row_tile=16, ldq=257),
-                  dict(row_tile=16, cache=at + 8), dict(row_tile=128, dim=32), dict(row_tile=128, q=at + 8), dict(row_tile=128, dim=128, ldq=260), dict(row_tile=128, heads=258)):
+                  dict(row_tile=16, cache=at + 8), dict(row_tile=128, dim=32), dict(row_tile=128, q=at + 8), dict(row_tile=128, dim=128, ldq=260), dict(row_tile=128, heads=258), dict(row_tile=256, dim=32), dict(row_tile=512)):
         assert attend(**wrong) == 1, wrong
 
 

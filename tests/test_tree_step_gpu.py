@@ -125,6 +125,46 @@ def test_attention_tree_window(heads, window, kind, dtype):
     check(step, window)
 
 
+def run_plan(step, plan, window=None):
+    """The call with a plan given: (rows of a CTA, parts, key tiles of a part)."""
+    from easy_gpt.cpp_b200 import kernels
+
+    k = step.k
+    args = kernels._pack_attention_tree(step.q.data_ptr(), k.data_ptr(), step.v.data_ptr(), step.block_table.data_ptr(), step.starts.data_ptr(), step.context.data_ptr(), step.flat.data_ptr(),
+                                        step.out.data_ptr(), step.status.data_ptr(), kernels.dtype_code(step.dtype), step.q.stride(0), step.out.stride(0), k.stride(0), k.stride(1),
+                                        step.block_table.stride(0), step.block_table.shape[1], k.shape[0], step.flat.numel(), len(step.nodes), step.heads, step.kv_heads, step.dim, step.page,
+                                        window or 0, 0, *plan, step.dim ** -0.5)
+    assert kernels.library().eg_attention_tree(torch.cuda.current_stream().cuda_stream, args) == 0
+    return step.out
+
+
+@pytest.mark.parametrize("parts, part_tiles", [(1, 1), (2, 3), (8, 1), (16, 1)])
+@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("heads, window", [((14, 2, 64), None), ((14, 2, 64), 50), ((28, 4, 128), None), ((16, 1, 128), 200), ((3, 3, 64), 70), ((4, 2, 32), None), ((8, 1, 256), 33)])
+def test_attention_tree_every_kernel(heads, window, row_tile, parts, part_tiles):
+    """Every kernel and cut by name, whatever the rule would choose: one and two tiles of rows, an entry whose second tile is empty, parts without keys."""
+    if row_tile >= 128 and heads[2] not in (64, 128) or parts == 16 and heads[2] == 256:
+        pytest.skip("sizes that kernel does not take")
+    step = Step([*heads, row_tile], [1, 18, 19, 0, 36, 37, 100], [0, 1000, 63, 7, 640, 1, 333], *heads, 32)
+    got, want = run_plan(step, (row_tile, parts, part_tiles), window).double(), step.plain(window)
+    total = sum(step.nodes)
+    assert int(step.status) == 0 and torch.equal(got[total:], want[total:])
+    assert float(((got[:total] - want[:total]).norm(dim=1) / want[:total].norm(dim=1)).max()) <= tolerance(step.dtype, step.dim)
+
+
+@pytest.mark.parametrize("row_tile", [0, 16, 64, 128, 256])
+def test_attention_tree_every_kernel_hides_what_is_not_a_number(row_tile):
+    step = Step(6, [40, 20], [100, 700], 14, 2, 64, 16, kind="chain")
+    step.cache[step.table[0, 3], :, :, 8] = math.nan                  # entry 0's key 56: seen with a window of 50 by nodes up to depth 5
+    step.cache[step.table[1, 44], :, :, 15] = math.inf                # entry 1's node 19, the chain's last
+    got, want = run_plan(step, (row_tile, 4, 1), 50).double(), step.plain(50)
+    for i in range(60):
+        hidden = i > 5 if i < 40 else i != 59
+        assert bool(torch.isfinite(got[i]).all()) == hidden, i
+        if hidden:
+            assert float((got[i] - want[i]).norm() / want[i].norm()) <= tolerance(torch.bfloat16, 64)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (8, 1, 256)])
 @pytest.mark.parametrize("nodes", [1, 5, 64, 300])
