@@ -17,7 +17,6 @@ namespace {
 using tree::Entry;
 using tree::Params;
 
-constexpr int TC_LINES = 64;                                         // rows of an entry and KV head from which on the tcgen05 kernel takes them
 constexpr int ROWS = 64, KEYS = 32, THREADS = 256, STAGED_NODES = 1024;
 constexpr int LISTED = 16;                                           // key tiles whose places in the cache are looked up at a time
 
@@ -328,36 +327,36 @@ int launch_any(cudaStream_t stream, const Params& p, int tiles) {
 
 }  // namespace
 
-// How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (128 or 256: the tcgen05 kernel; 16, 32 or 64: the warp-level one;
-// 0: the 32-bit one),
-// plan[1] and plan[2] the max_parts and part_tiles of eg_attention_tree.  aligned: the caches, their pages and heads start on 16-byte boundaries, and
-// q, out and their rows on 16-byte (2) or 4-byte (1) ones.  max_context: the most keys of an entry, as far as known.
+// How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (128: the tcgen05 kernel; 16, 32 or 64: the warp-level one;
+// 0: the 32-bit one), plan[1] and plan[2] the max_parts and part_tiles of eg_attention_tree.  aligned: the caches, their pages and heads start on
+// 16-byte boundaries, and q, out and their rows on 16-byte (2) or 4-byte (1) ones.  max_context: the most keys of an entry, as far as known.
+//
+// A key tile of 64 takes a CTA 1 us on the tcgen05 kernel whatever its rows, and 1 us (16 rows of 64) to 2.6 us (64 rows of 128) on the warp-level one,
+// whose start and end are 2 us shorter: that one takes short contexts of few units where both would do (a chain of 8 at 500 keys 7.6 us against 9.4;
+// 64 requests of 16 nodes at 700 keys 46 against 21).  Parts: as many as keep one CTA an SM with three key tiles a part, or two CTAs with eight;
+// more of them cost more than they save (32 requests of 9 nodes at 1,000 keys in 1, 2, 4 and 8 parts 18.7, 16.2, 14.6 and 23.8 us; 64 requests of 16 at 700
+// in 1, 2 and 4 parts 21, 25 and 36), and clusters of 16 find little room.  Long contexts are cut into four in any case, for an even end (16 requests of up
+// to 32,768 keys, wide trees, in 1, 2, 4 and 8 parts 563, 460, 399 and 428).
 EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count,
                                   int* plan) {
     if (rows < 1 || entries < 1 || num_kv_heads < 1 || num_heads % num_kv_heads || num_heads < 1 || page_size < 1 || sm_count < 1 || !plan) return (int)cudaErrorInvalidValue;
     const int group = num_heads / num_kv_heads;
     const long long lines = ((long long)rows * group + entries - 1) / entries;      // of an entry, on the average
+    const long long key_tiles = ((long long)max_context + 63) / 64;
     const bool tiled = dtype == EG_BF16 && aligned && page_size % 16 == 0 && (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256);
     const bool wide = tiled && aligned > 1 && (head_dim == 64 || head_dim == 128) && group <= 128;
-    const int row_tile = !tiled ? ROWS : lines <= 16 ? 16 : lines <= 32 ? 32 : wide && lines > TC_LINES ? 128 : 64;
-    const long long units = entries * ((lines + row_tile - 1) / row_tile) * num_kv_heads, key_tiles = ((long long)max_context + 63) / 64;
-    // as many parts as fill the SMs once, a power of two, of two key tiles at least; a cluster has to find room among the 16 SMs and more of a GPC
-    if (row_tile == 128) {
-        const int nodes = 128 / group;
-        const long long tc_units = entries * (((long long)rows + entries * nodes - 1) / (entries * nodes)) * num_kv_heads;
-        int parts = 1;
-        while (parts < 8 && tc_units * parts < 6ll * sm_count && key_tiles >= parts * 8) parts *= 2;
-        plan[0] = 128;
-        plan[1] = parts;
-        plan[2] = (int)(key_tiles / (parts * 2) > 4 ? key_tiles / parts : 4);
-        return 0;
-    }
-    const int ctas = !tiled ? (head_dim <= 128 ? 2 : 1) : head_dim <= 64 ? 3 : head_dim == 128 ? 2 : 1;
+    const auto units_of = [&](long long tile) { return entries * ((lines + tile - 1) / tile) * num_kv_heads; };
+    int row_tile = !tiled ? 0 : lines <= 16 ? 16 : lines <= 32 ? 32 : 64;
+    if (wide && (key_tiles > 16 || units_of(64) * 8 > sm_count)) row_tile = 128;
+    else if (tiled && units_of(16) * 8 <= sm_count) row_tile = 16;
+    const long long units = units_of(row_tile == 128 ? 128 / group * group : row_tile ? row_tile : ROWS);
+    const int most = head_dim > 128 ? 8 : row_tile == 0 || row_tile == 128 ? 8 : 16;
     int parts = 1;
-    while (parts < (ctas > 1 ? tree::MAX_PARTS : tree::MAX_PARTS / 2) && units * parts * 2 <= (long long)sm_count * ctas && key_tiles >= parts * 4) parts *= 2;
-    plan[0] = tiled ? row_tile : 0;
+    while (parts < most && ((units * parts * 2 <= sm_count && key_tiles >= parts * (row_tile == 128 ? 6 : 2)) || (units * parts * 2 <= 2ll * sm_count && key_tiles >= parts * 16))) parts *= 2;
+    while (parts < 4 && key_tiles > parts * 64) parts *= 2;
+    plan[0] = row_tile;
     plan[1] = parts;
-    plan[2] = 2;
+    plan[2] = 1;
     return 0;
 }
 
@@ -382,20 +381,20 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
         const int code = eg_attention_tree_plan((int)a.dtype, aligned, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
                                                 (int)(a.max_context < 1 ? 1 : a.max_context > INT ? INT : a.max_context), eg_sm_count(), plan);
         if (code) return code;
-    } else if ((a.row_tile && a.row_tile != 16 && a.row_tile != 32 && a.row_tile != 64 && a.row_tile != 128 && a.row_tile != 256) || a.max_parts < 1 || a.max_parts > tree::MAX_PARTS ||
+    } else if ((a.row_tile && a.row_tile != 16 && a.row_tile != 32 && a.row_tile != 64 && a.row_tile != 128) || a.max_parts < 1 || a.max_parts > tree::MAX_PARTS ||
                (a.max_parts & (a.max_parts - 1)) || a.part_tiles < 1 || a.part_tiles > 1 << 20) {
         return (int)cudaErrorInvalidValue;
     }
     const int row_tile = plan[0];
     if (row_tile && (!tiled || (dim != 32 && dim != 64 && dim != 128 && dim != 256) || a.page_size % 16)) return (int)cudaErrorInvalidValue;
-    if (row_tile >= 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
+    if (row_tile == 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
     const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
     const long long tiles = a.rows * group / tile_rows + a.entries;   // at most: every entry's last tile may be a short one
     if (tiles > 65535) return (int)cudaErrorInvalidValue;
     const Params p = {a.q, a.ldq, a.k_cache, a.v_cache, a.page_stride, a.head_stride, a.block_table, (int)a.table_stride, (int)a.table_pages, (int)a.num_pages,
                       a.entry_starts, a.context, a.parents, a.out, a.ldo, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
                       (int)a.window, (float)a.scale, plan[1], plan[2] * (64 / tile_keys), a.status};
-    if (row_tile >= 128) return tree::launch_tc(stream, p, row_tile / 128);
+    if (row_tile == 128) return tree::launch_tc(stream, p);
     if (row_tile) return tree::launch_mma(stream, p, row_tile, (int)tiles);
     if (a.dtype == EG_BF16) return launch_any<bf16, false>(stream, p, (int)tiles);
     const bool pieces = (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.ldq | a.page_stride | a.head_stride | a.head_dim) & 3) == 0;

@@ -93,9 +93,9 @@ __device__ __forceinline__ int parts_of(const Params& p, int key_tiles) { return
 
 // The kernel in attention_tree_mma.cu (16, 32 or 64 rows a CTA, key tiles of 64).  Its caller has checked what it takes.
 int launch_mma(cudaStream_t stream, const Params& p, int row_tile, int tiles);
-// The kernel in attention_tree_tc.cu (one or two times 128 rows a CTA, or as many as whole nodes have; key tiles of 64).  Its caller has checked what it
-// takes, but for the size of the tensor maps.
-int launch_tc(cudaStream_t stream, const Params& p, int row_tiles);
+// The kernel in attention_tree_tc.cu (128 rows a CTA, or as many as whole nodes have; key tiles of 64).  Its caller has checked what it takes, but for the
+// size of the tensor maps.
+int launch_tc(cudaStream_t stream, const Params& p);
 
 // ---- the parts of a tile, one CTA of the cluster each
 __device__ __forceinline__ void cluster_barrier() {

@@ -7,13 +7,13 @@
 //   P = softmax  four warps, a row a thread: S out of TMEM, reference and sum in registers, P back over S as bfloat16 pairs
 //   O += P V     tcgen05.mma, P from TMEM, V by TMA, O in TMEM
 // The reference of the exponents follows a row's maximum lazily: it moves, and the row's O with it, only when the maximum has grown by 2^8.
-// A row is a thread and a warp's rows exponentiate at the unit's rate (512 cycles a tile and SM, as long as the two products of a head of 128 take), so
-// an SM has two tiles at a time, one's exponents beside the other's products and waits.  Either two CTAs share it (256 columns of TMEM and less than
-// half the shared memory each), or, where an entry's rows fill more than one tile, a CTA has two tiles (WGS 2): keys and values are then fetched once
-// for both, and their rings have more than twice the stages.
+// A row is a thread and a warp's rows exponentiate at the unit's rate (512 cycles a tile and SM, against 128 or 256 for the two products), so two
+// CTAs share an SM (256 columns of TMEM and less than half the shared memory each), one's exponents beside the other's products and waits.
 //
-// Warps: 0 loads keys and 6 values, 1 allocates TMEM and issues the scores' products and 7 the output's, 2 to 5 have the first tile's rows and 8 to 11 the
-// second's.  (One thread for both products: 3,800 cycles a key tile of two row tiles, with two threads ISSUE_NOW.)  Keys and values have rings of their own, since a key stage is free long before the value stage of its tile: when its scores are there.  A piece of a tile that no row sees, or whose page is none, is
+// Warps: 0 loads keys and 6 values, 1 allocates TMEM and issues the scores' products, 7 the output's, 2 to 5 have the rows.  (One thread for both products
+// was slower: 16 requests of up to 32,768 keys 464 us against 393.  So were two tiles of rows a CTA, 256 threads of rows that share keys and values: 520 to
+// 560, with the two exponentiating at the same time.)
+// Keys and values have rings of their own, since a key stage is free long before the value stage of its tile: when its scores are there.  A piece of a tile that no row sees, or whose page is none, is
 // read from behind the last row of the cache map, which gives zeros.  Every wait is bounded; a role that gives up raises the CTA's abort flag, the
 // loader waits for its copies, and the CTA leaves as it always does.
 //
@@ -30,56 +30,51 @@ using namespace tc05;
 using tree::Entry;
 using tree::Params;
 
-constexpr int KEYS = 64, STAGED_NODES = 512;
+constexpr int KEYS = 64, THREADS = 256, STAGED_NODES = 512;
 constexpr float REFERENCE_SLACK = 8.f;
 
-template <int HD, int WGS>
+template <int HD>
 struct Shape {
-    static constexpr int SUBS = HD / 64, THREADS = WGS == 1 ? 256 : 384;
-    static constexpr int K_STAGES = HD == 64 ? (WGS == 1 ? 5 : 10) : (WGS == 1 ? 2 : 5), V_STAGES = HD == 64 ? K_STAGES : (WGS == 1 ? 2 : 4);
-    static constexpr int SCORES = HD == 64 ? 3 : 2;                  // TMEM buffers of S and P, of a tile of rows
+    static constexpr int SUBS = HD / 64, STAGES = HD == 64 ? 5 : 2, SCORES = HD == 64 ? 3 : 2;      // stages of keys and of values, TMEM buffers of S and P
     static constexpr int Q_SUB_BYTES = BM * SUB_ROW_BYTES, SUB_BYTES = KEYS * SUB_ROW_BYTES, TILE_BYTES = SUBS * SUB_BYTES;
-    static constexpr int Q_BYTES = SUBS * Q_SUB_BYTES, SMEM = WGS * Q_BYTES + (K_STAGES + V_STAGES) * TILE_BYTES + 1024;
-    static constexpr int O_COL = WGS * SCORES * KEYS, TMEM_COLS = WGS * 256, OUT_LD = HD + 4;
-    static_assert(O_COL + WGS * HD <= TMEM_COLS, "TMEM columns");
-    static_assert(WGS * BM * OUT_LD * 4 <= SMEM - 1024, "a part's results in the tiles' place");
+    static constexpr int Q_BYTES = SUBS * Q_SUB_BYTES, SMEM = Q_BYTES + 2 * STAGES * TILE_BYTES + 1024;
+    static constexpr int O_COL = SCORES * KEYS, TMEM_COLS = 256, OUT_LD = HD + 4;
+    static_assert(O_COL + HD <= TMEM_COLS, "TMEM columns");
+    static_assert(BM * (OUT_LD + 2) * 4 <= SMEM - 1024, "a part's results in the tiles' place");
 };
 
 struct Maps {
-    int nodes, piece_rows, nowhere;                                  // nodes of a tile of rows; keys a box holds; the row behind the cache maps' last
+    int nodes, piece_rows, nowhere;                                  // nodes of a tile; keys a box holds; the row behind the cache maps' last
     long long page_rows, head_rows;
 };
 
-template <int HD, int WGS>
-__global__ void __launch_bounds__((Shape<HD, WGS>::THREADS), (WGS == 1 ? 2 : 1))
+template <int HD>
+__global__ void __launch_bounds__(THREADS, 2)
 attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p, const Maps maps) {
-    using S = Shape<HD, WGS>;
-    constexpr int SCORES = S::SCORES, K_STAGES = S::K_STAGES, V_STAGES = S::V_STAGES;
+    using S = Shape<HD>;
+    constexpr int STAGES = S::STAGES, SCORES = S::SCORES;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t q_full[WGS], k_full[K_STAGES], v_full[V_STAGES], k_empty[K_STAGES], v_empty[V_STAGES];
-    __shared__ __align__(8) uint64_t s_full[WGS * SCORES], p_full[WGS * SCORES], o_done[WGS * SCORES];
+    __shared__ __align__(8) uint64_t q_full, k_full[STAGES], v_full[STAGES], k_empty[STAGES], v_empty[STAGES], s_full[SCORES], p_full[SCORES], o_done[SCORES];
     __shared__ int ups[STAGED_NODES];
-    __shared__ float row_ml[2 * WGS * BM];
+    __shared__ float row_ml[2 * BM];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, latest, holes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.x, kvh = blockIdx.y;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
-    const uint32_t q_addr = base, k_ring = base + WGS * S::Q_BYTES, v_ring = k_ring + K_STAGES * S::TILE_BYTES;
+    const uint32_t q_addr = base, k_ring = base + S::Q_BYTES, v_ring = k_ring + STAGES * S::TILE_BYTES;
     unsigned char* const aligned = smem_raw + (base - smem_addr(smem_raw));
     pdl_enter();
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
-    if (!tree::find_tile(p, blockIdx.z, WGS * maps.nodes * group, r, e, within)) return;
-    const int node0 = within * WGS * maps.nodes, nodes = min(WGS * maps.nodes, e.n - node0), count = nodes * group, last_node = node0 + nodes - 1;
+    if (!tree::find_tile(p, blockIdx.z, maps.nodes * group, r, e, within)) return;
+    const int node0 = within * maps.nodes, nodes = min(maps.nodes, e.n - node0), count = nodes * group, last_node = node0 + nodes - 1;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
     if (part >= parts) return;
     const int begin = tile0 + (int)((long long)tiles * part / parts), ntiles = tile0 + (int)((long long)tiles * (part + 1) / parts) - begin;
     const int* const table = p.block_table + (size_t)r * p.table_stride;
-    // the rows of the two tiles, and the warps that have any
-    const int first_rows = min(nodes, maps.nodes) * group, second_rows = count - first_rows, first_warps = (first_rows + 31) / 32, second_warps = (second_rows + 31) / 32;
-    const int wgs = WGS == 1 || second_rows == 0 ? 1 : 2;
+    const int row_warps = (count + 31) / 32;
 
     // ---- loaders: a lane a box (64 columns, piece_rows keys) of every tile; its page is looked up a tile ahead
     const bool is_v = warp == 6, loader = warp == 0 || is_v;
@@ -93,34 +88,26 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     };
     int page_ahead = loads ? page_of(0) : NOT_NEEDED;
     // ---- rows: a thread's row of q and a node's parent are asked for in the same trip
-    const int g = WGS > 1 && warp >= 8 ? 1 : 0, quad = warp & 3, row = quad * 32 + lane;     // a warp may touch the TMEM lanes 32 (warp % 4) ..
-    const int my_rows = g ? second_rows : first_rows, my_warps = g ? second_warps : first_warps;
-    const bool has_rows = (g || (warp >= 2 && warp < 6)) && quad < my_warps, valid = has_rows && row < my_rows;
-    const int node = node0 + g * maps.nodes + min(row, max(my_rows, 1) - 1) / group, head = kvh * group + row % group;
+    const int quad = warp & 3, row = quad * 32 + lane;               // (of warps 2 to 5) a warp may touch the TMEM lanes 32 (warp % 4) ..
+    const bool has_rows = warp >= 2 && warp < 6 && quad < row_warps, valid = has_rows && row < count;
+    const int node = node0 + min(row, count - 1) / group, head = kvh * group + row % group;
     uint4 q_row[HD / 8];
     const uint4* const q_from = reinterpret_cast<const uint4*>(static_cast<const bf16*>(p.q) + (size_t)(e.first + node) * p.ldq + (size_t)head * HD);
 #pragma unroll
     for (int c = 0; c < HD / 8; ++c) q_row[c] = valid ? __ldg(q_from + c) : make_uint4(0, 0, 0, 0);
-    const int row_threads = (first_warps + (WGS > 1 ? second_warps : 0)) * 32, row_thread = (g ? first_warps * 32 : 0) + row;
-    const int parent = has_rows && row_thread <= last_node ? p.parents[e.first + row_thread] : -1;
+    const int parent = has_rows && row <= last_node ? p.parents[e.first + row] : -1;
     if (threadIdx.x == 0) {
-#pragma unroll
-        for (int w = 0; w < WGS; ++w) {
-            const int warps = max(1, w ? second_warps : first_warps);
-            mbar_init(&q_full[w], warps);
-            for (int i = 0; i < SCORES; ++i) {
-                mbar_init(&s_full[w * SCORES + i], 1);
-                mbar_init(&p_full[w * SCORES + i], warps);
-                mbar_init(&o_done[w * SCORES + i], 1);
-            }
-        }
-        for (int i = 0; i < K_STAGES; ++i) {
+        mbar_init(&q_full, row_warps);
+        for (int i = 0; i < STAGES; ++i) {
             mbar_init(&k_full[i], 1);
-            mbar_init(&k_empty[i], 1);
-        }
-        for (int i = 0; i < V_STAGES; ++i) {
             mbar_init(&v_full[i], 1);
+            mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < SCORES; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], row_warps);
+            mbar_init(&o_done[i], 1);
         }
         abort_flag = latest = holes = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -134,9 +121,10 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
+    // a row's result, its columns c0 .. c0 + 31
     bool rows_done = false;
     float row_scale = 1.f;
-    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(g * SCORES * KEYS), o_lanes = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(S::O_COL + g * HD);
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), o_lanes = lanes + S::O_COL;
     auto up_of = [&](int i) { return i < STAGED_NODES ? ups[i] : tree::parent_of(p, e, i); };
     int lowest = 0;
     // which of a key tile's keys the row sees
@@ -159,15 +147,13 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         uint64_t* const full = is_v ? v_full : k_full;
         uint64_t* const empty = is_v ? v_empty : k_empty;
         const uint32_t ring = is_v ? v_ring : k_ring;
-        const int stages = is_v ? V_STAGES : K_STAGES;
         const CUtensorMap* const map = is_v ? &map_v : &map_k;
-        int st = 0, use = 0;                                         // stage, and how often it has been used before
-        bool ok = true;
-        for (int j = 0; j < ntiles; ++j) {
+        int issued = 0;
+        for (int j = 0; j < ntiles; ++j, ++issued) {
+            const int st = j % STAGES, use = j / STAGES;
             const int page = page_ahead;
             if (loads) page_ahead = page_of(j + 1);
-            ok = use == 0 || __all_sync(0xffffffffu, lane > 0 || mbar_wait(&empty[st], (use - 1) & 1, &abort_flag, p.status));
-            if (!ok) break;
+            if (use > 0 && !__all_sync(0xffffffffu, lane > 0 || mbar_wait(&empty[st], (use - 1) & 1, &abort_flag, p.status))) break;
             int at = maps.nowhere;
             if (loads && page != NOT_NEEDED) {
                 if (page < 0 || page >= p.num_pages) {
@@ -181,80 +167,69 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (lane == 0) mbar_expect_tx(&full[st], S::TILE_BYTES);
             __syncwarp();
             if (loads) tma_load_2d(ring + st * S::TILE_BYTES + sub * S::SUB_BYTES + piece * maps.piece_rows * SUB_ROW_BYTES, map, &full[st], sub * 64, at);
-            if (++st == stages) st = 0, ++use;
         }
-        // every copy has to land before the CTA gives up its shared memory, also when a role has given up: the last copy of every stage
-        if (lane == 0 && (!ok || *(volatile int*)&abort_flag))
-            for (int i = 0; i < stages; ++i) {
-                const int uses = use + (i < st ? 1 : 0);
-                if (uses > 0) mbar_wait_plain(&full[i], (uses - 1) & 1);
-            }
+        // every copy has to land before the CTA gives up its shared memory, also when a role has given up
+        if (lane == 0 && *(volatile int*)&abort_flag)
+            for (int j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j) mbar_wait_plain(&full[j % STAGES], (j / STAGES) & 1);
     } else if (warp == 1) {
         if (lane == 0) {                                             // ---- S_j = Q K_j^T; descriptors differ in their low words
             const uint32_t product = idesc(KEYS, false), hi = (uint32_t)(desc_k_major(0) >> 32), q_lo = (uint32_t)desc_k_major(q_addr);
             uint32_t k_lo = (uint32_t)desc_k_major(k_ring);
-            bool ok = true;
-            for (int w = 0; w < wgs && ok; ++w) ok = mbar_wait(&q_full[w], 0, &abort_flag, p.status);
+            bool ok = mbar_wait(&q_full, 0, &abort_flag, p.status);
             int stage = 0, phase = 0, b = 0, b_phase = 1;            // of the key ring; of the score buffers
             for (int j = 0; j < ntiles && ok; ++j) {
-                ok = mbar_wait(&k_full[stage], phase, &abort_flag, p.status);
-                for (int w = 0; w < wgs && ok; ++w) {
-                    // S goes where S and P of SCORES tiles before were: the product that read that P must be done
-                    if (j >= SCORES) ok = mbar_wait(&o_done[w * SCORES + b], b_phase, &abort_flag, p.status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t a = q_lo + (uint32_t)((w * S::Q_BYTES) >> 4), d = tmem + (uint32_t)((w * SCORES + b) * KEYS);
+                // S goes where S and P of SCORES tiles before were: the product that read that P must be done
+                ok = mbar_wait(&k_full[stage], phase, &abort_flag, p.status) && (j < SCORES || mbar_wait(&o_done[b], b_phase, &abort_flag, p.status));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(b * KEYS);
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k) {
-                        const uint64_t x = desc_from(a + (uint32_t)((k / 4 * S::Q_SUB_BYTES + k % 4 * 32) >> 4), hi), y = desc_from(k_lo + (uint32_t)((k / 4 * S::SUB_BYTES + k % 4 * 32) >> 4), hi);
-                        if (k == 0) tc_mma<false>(d, x, y, product);
-                        else tc_mma<true>(d, x, y, product);
-                    }
-                    tc_commit(&s_full[w * SCORES + b]);
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint64_t x = desc_from(q_lo + (uint32_t)((k / 4 * S::Q_SUB_BYTES + k % 4 * 32) >> 4), hi);
+                    const uint64_t y = desc_from(k_lo + (uint32_t)((k / 4 * S::SUB_BYTES + k % 4 * 32) >> 4), hi);
+                    if (k == 0) tc_mma<false>(d, x, y, product);
+                    else tc_mma<true>(d, x, y, product);
                 }
-                if (ok) tc_commit(&k_empty[stage]);
+                tc_commit(&s_full[b]);
+                tc_commit(&k_empty[stage]);
                 k_lo += S::TILE_BYTES >> 4;
-                if (++stage == K_STAGES) stage = 0, phase ^= 1, k_lo -= (K_STAGES * S::TILE_BYTES) >> 4;
+                if (++stage == STAGES) stage = 0, phase ^= 1, k_lo -= (STAGES * S::TILE_BYTES) >> 4;
                 if (++b == SCORES) b = 0, b_phase ^= 1;
             }
         }
     } else if (warp == 7) {
         if (lane == 0) {                                             // ---- O += P_j V_j
-            const uint32_t product = idesc(HD, true), hi = (uint32_t)(desc_k_major(0) >> 32);
+            const uint32_t product = idesc(HD, true), hi = (uint32_t)(desc_k_major(0) >> 32), d = tmem + (uint32_t)S::O_COL;
             uint32_t v_lo = (uint32_t)desc_n_major(v_ring, S::SUB_BYTES);
             int stage = 0, phase = 0, b = 0, b_phase = 0;
-            bool ok = true;
-            for (int j = 0; j < ntiles && ok; ++j) {
-                ok = mbar_wait(&v_full[stage], phase, &abort_flag, p.status);
-                for (int w = 0; w < wgs && ok; ++w) {
-                    ok = mbar_wait(&p_full[w * SCORES + b], b_phase, &abort_flag, p.status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t weights = tmem + (uint32_t)((w * SCORES + b) * KEYS), d = tmem + (uint32_t)(S::O_COL + w * HD);
+            for (int j = 0; j < ntiles; ++j) {
+                if (!mbar_wait(&v_full[stage], phase, &abort_flag, p.status) || !mbar_wait(&p_full[b], b_phase, &abort_flag, p.status)) break;
+                tc_fence_after();
+                const uint32_t weights = tmem + (uint32_t)(b * KEYS);
 #pragma unroll
-                    for (int k = 0; k < KEYS / 16; ++k) {
-                        const uint64_t y = desc_from(v_lo + (uint32_t)((k * 2048) >> 4), hi);
-                        if (k == 0 && j == 0) tc_mma_a_tmem<false>(d, weights, y, product);
-                        else tc_mma_a_tmem<true>(d, weights + (uint32_t)(k * 8), y, product);
-                    }
-                    tc_commit(&o_done[w * SCORES + b]);
+                for (int k = 0; k < KEYS / 16; ++k) {
+                    const uint64_t y = desc_from(v_lo + (uint32_t)((k * 2048) >> 4), hi);
+                    if (k == 0 && j == 0) tc_mma_a_tmem<false>(d, weights, y, product);
+                    else tc_mma_a_tmem<true>(d, weights + (uint32_t)(k * 8), y, product);
                 }
-                if (ok) tc_commit(&v_empty[stage]);
+                tc_commit(&o_done[b]);
+                tc_commit(&v_empty[stage]);
                 v_lo += S::TILE_BYTES >> 4;
-                if (++stage == V_STAGES) stage = 0, phase ^= 1, v_lo -= (V_STAGES * S::TILE_BYTES) >> 4;
+                if (++stage == STAGES) stage = 0, phase ^= 1, v_lo -= (STAGES * S::TILE_BYTES) >> 4;
                 if (++b == SCORES) b = 0, b_phase ^= 1;
             }
         }
     } else if (has_rows) {
         // ---- the rows: q into shared memory, the tree, then a key tile at a time
+        const int row_threads = row_warps * 32;
         auto rows_barrier = [&]() { asm volatile("bar.sync 1, %0;\n" ::"r"(row_threads) : "memory"); };
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(aligned + g * S::Q_BYTES + c / 8 * S::Q_SUB_BYTES + row * SUB_ROW_BYTES + ((c % 8) ^ (row & 7)) * 16) = q_row[c];
+        for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(aligned + c / 8 * S::Q_SUB_BYTES + row * SUB_ROW_BYTES + ((c % 8) ^ (row & 7)) * 16) = q_row[c];
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&q_full[g]);
-        if (row_thread <= last_node && row_thread < STAGED_NODES) ups[row_thread] = tree::sound_parent(p, row_thread, parent);
-        for (int i = row_threads + row_thread; i <= last_node && i < STAGED_NODES; i += row_threads) ups[i] = tree::parent_of(p, e, i);
+        if (lane == 0) mbar_arrive(&q_full);
+        if (row <= last_node) ups[row] = tree::sound_parent(p, row, parent);
+        for (int i = row_threads + row; i <= last_node && i < STAGED_NODES; i += row_threads) ups[i] = tree::parent_of(p, e, i);
         rows_barrier();
         if (p.window > 0) {
             int depth = 0;
@@ -269,7 +244,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         bool ok = true, poison = false;                              // poison: values that are not finite have been met
         for (int j = 0; j < ntiles; ++j) {
             const int b = j % SCORES, key0 = (begin + j) * KEYS;
-            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[g * SCORES + b], (j / SCORES) & 1, &abort_flag, p.status));      // the warp stays together
+            ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], (j / SCORES) & 1, &abort_flag, p.status));      // the warp stays together
             if (!ok) break;
             tc_fence_after();
             float s[64];
@@ -292,9 +267,9 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             }
             // (a hole's values are zeros.  Every warp looks at the whole tile, so that none waits for another: a warp whose wait gave up would not come)
             if (key0 + KEYS > e.context || key0 < edge) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % V_STAGES], (j / V_STAGES) & 1, &abort_flag, p.status));
+                ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % STAGES], (j / STAGES) & 1, &abort_flag, p.status));
                 if (!ok) break;
-                unsigned char* const values = aligned + WGS * S::Q_BYTES + (K_STAGES + j % V_STAGES) * S::TILE_BYTES;
+                unsigned char* const values = aligned + S::Q_BYTES + (STAGES + j % STAGES) * S::TILE_BYTES;
                 bool odd = false;
                 for (int i = lane; i < S::TILE_BYTES / 16; i += 32) {
                     const uint4 v = *reinterpret_cast<const uint4*>(values + i * 16);
@@ -328,7 +303,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             }
             const float ref = m == -INFINITY ? 0.f : m;              // a row that has seen nothing: weights 0
             if (j > 0 && __any_sync(0xffffffffu, c != 1.f)) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&o_done[g * SCORES + (j - 1) % SCORES], ((j - 1) / SCORES) & 1, &abort_flag, p.status));
+                ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(j - 1) % SCORES], ((j - 1) / SCORES) & 1, &abort_flag, p.status));
                 if (!ok) break;
                 tc_fence_after();
 #pragma unroll
@@ -362,23 +337,17 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[g * SCORES + b]);
+            if (lane == 0) mbar_arrive(&p_full[b]);
         }
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[g * SCORES + (ntiles - 1) % SCORES], ((ntiles - 1) / SCORES) & 1, &abort_flag, p.status));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(ntiles - 1) % SCORES], ((ntiles - 1) / SCORES) & 1, &abort_flag, p.status));
         tc_fence_after();
         rows_done = ok;
         row_scale = parts > 1 ? 1.f : l > 0.f ? 1.f / l : l;         // nothing seen: 0; NaN stays
-        // a part's lines go where Q, K and V are, the second tile's behind the first's, once neither tile's products read those any more
-        // (every row warp comes here, also one whose wait gave up)
-        const int line_of_part = g ? first_rows + row : row;
-        if (WGS > 1 && parts > 1) rows_barrier();
-        if (valid) {
-            row_ml[2 * line_of_part] = rows_done ? m : -INFINITY;
-            row_ml[2 * line_of_part + 1] = rows_done ? l : 0.f;
-        }
+        row_ml[2 * row] = rows_done ? m : -INFINITY;
+        row_ml[2 * row + 1] = rows_done ? l : 0.f;
         if (rows_done) {
             bf16* const line = static_cast<bf16*>(p.out) + (size_t)(e.first + node) * p.ldo + (size_t)head * HD;
-            float* const part_line = reinterpret_cast<float*>(aligned) + line_of_part * S::OUT_LD;
+            float* const part_line = reinterpret_cast<float*>(aligned) + row * S::OUT_LD;
 #pragma unroll
             for (int c0 = 0; c0 < HD; c0 += 32) {
                 uint32_t o[32];
@@ -403,7 +372,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                         }
                     }
                 if (parts > 1) {
-                    if (!valid) continue;
 #pragma unroll
                     for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(part_line + c0 + x) = make_float4(v[x], v[x + 1], v[x + 2], v[x + 3]);
                 } else if (valid) {
@@ -421,26 +389,26 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     tc_fence_after();
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::TMEM_COLS) : "memory");
     if (parts > 1)
-        tree::add_parts<S::THREADS>(reinterpret_cast<const float*>(aligned), S::OUT_LD, row_ml, count, HD, parts, [&](int line, int d, float4 v) {
+        tree::add_parts<THREADS>(reinterpret_cast<const float*>(aligned), S::OUT_LD, row_ml, count, HD, parts, [&](int line, int d, float4 v) {
             uint2* const at = reinterpret_cast<uint2*>(static_cast<bf16*>(p.out) + (size_t)(e.first + node0 + line / group) * p.ldo +
                                                        (size_t)(kvh * group + line % group) * HD + d);
             *at = make_uint2(pack2(v.x, v.y), pack2(v.z, v.w));
         });
 }
 
-template <int HD, int WGS>
+template <int HD>
 int launch(cudaStream_t stream, const Params& p, const Maps& maps, const CUtensorMap& map_k, const CUtensorMap& map_v, int tiles) {
-    constexpr int bytes = Shape<HD, WGS>::SMEM;
+    constexpr int bytes = Shape<HD>::SMEM;
     static unsigned long long seen = 0;
-    if (const int code = tree::prepare_kernel(attention_tree_tc_kernel<HD, WGS>, bytes, seen)) return code;
-    return tree::launch_clusters(attention_tree_tc_kernel<HD, WGS>, dim3(p.max_parts, p.num_kv_heads, tiles), Shape<HD, WGS>::THREADS, bytes, stream, map_k, map_v, p, maps);
+    if (const int code = tree::prepare_kernel(attention_tree_tc_kernel<HD>, bytes, seen)) return code;
+    return tree::launch_clusters(attention_tree_tc_kernel<HD>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, map_k, map_v, p, maps);
 }
 
 }  // namespace
 
 namespace tree {
 
-int launch_tc(cudaStream_t stream, const Params& p, int row_tiles) {
+int launch_tc(cudaStream_t stream, const Params& p) {
     const int group = p.num_heads / p.num_kv_heads;
     Maps maps;
     maps.nodes = BM / group;
@@ -448,15 +416,13 @@ int launch_tc(cudaStream_t stream, const Params& p, int row_tiles) {
     maps.page_rows = p.page_stride / p.head_dim;
     maps.head_rows = p.head_stride / p.head_dim;
     const long long kv_rows = (long long)(p.num_pages - 1) * maps.page_rows + (long long)(p.num_kv_heads - 1) * maps.head_rows + p.page_size;
-    const long long tiles = (long long)p.rows / (row_tiles * maps.nodes) + p.entries;
+    const long long tiles = (long long)p.rows / maps.nodes + p.entries;
     if (kv_rows >= (1ll << 31) || tiles > 65535) return (int)cudaErrorInvalidValue;
     maps.nowhere = (int)kv_rows;
     CUtensorMap map_k, map_v;
     if (make_map(&map_k, p.k_cache, kv_rows, p.head_dim, p.head_dim, maps.piece_rows) || make_map(&map_v, p.v_cache, kv_rows, p.head_dim, p.head_dim, maps.piece_rows))
         return (int)cudaErrorInvalidValue;
-    if (row_tiles == 1)
-        return p.head_dim == 64 ? launch<64, 1>(stream, p, maps, map_k, map_v, (int)tiles) : launch<128, 1>(stream, p, maps, map_k, map_v, (int)tiles);
-    return p.head_dim == 64 ? launch<64, 2>(stream, p, maps, map_k, map_v, (int)tiles) : launch<128, 2>(stream, p, maps, map_k, map_v, (int)tiles);
+    return p.head_dim == 64 ? launch<64>(stream, p, maps, map_k, map_v, (int)tiles) : launch<128>(stream, p, maps, map_k, map_v, (int)tiles);
 }
 
 }  // namespace tree

@@ -139,11 +139,11 @@ def run_plan(step, plan, window=None):
 
 
 @pytest.mark.parametrize("parts, part_tiles", [(1, 1), (2, 3), (8, 1), (16, 1)])
-@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128, 256])
+@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
 @pytest.mark.parametrize("heads, window", [((14, 2, 64), None), ((14, 2, 64), 50), ((28, 4, 128), None), ((16, 1, 128), 200), ((3, 3, 64), 70), ((4, 2, 32), None), ((8, 1, 256), 33)])
 def test_attention_tree_every_kernel(heads, window, row_tile, parts, part_tiles):
-    """Every kernel and cut by name, whatever the rule would choose: one and two tiles of rows, an entry whose second tile is empty, parts without keys."""
-    if row_tile >= 128 and heads[2] not in (64, 128) or parts == 16 and heads[2] == 256:
+    """Every kernel and cut by name, whatever the rule would choose: entries of less than a tile of rows, of one and of several; parts without keys."""
+    if row_tile == 128 and heads[2] not in (64, 128) or parts == 16 and heads[2] == 256:
         pytest.skip("sizes that kernel does not take")
     step = Step([*heads, row_tile], [1, 18, 19, 0, 36, 37, 100], [0, 1000, 63, 7, 640, 1, 333], *heads, 32)
     got, want = run_plan(step, (row_tile, parts, part_tiles), window).double(), step.plain(window)
@@ -152,7 +152,7 @@ def test_attention_tree_every_kernel(heads, window, row_tile, parts, part_tiles)
     assert float(((got[:total] - want[:total]).norm(dim=1) / want[:total].norm(dim=1)).max()) <= tolerance(step.dtype, step.dim)
 
 
-@pytest.mark.parametrize("row_tile", [0, 16, 64, 128, 256])
+@pytest.mark.parametrize("row_tile", [0, 16, 64, 128])
 def test_attention_tree_every_kernel_hides_what_is_not_a_number(row_tile):
     step = Step(6, [40, 20], [100, 700], 14, 2, 64, 16, kind="chain")
     step.cache[step.table[0, 3], :, :, 8] = math.nan                  # entry 0's key 56: seen with a window of 50 by nodes up to depth 5
