@@ -343,7 +343,7 @@ EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries,
     const int group = num_heads / num_kv_heads;
     const long long lines = ((long long)rows * group + entries - 1) / entries;      // of an entry, on the average
     const long long key_tiles = ((long long)max_context + 63) / 64;
-    const bool tiled = dtype == EG_BF16 && aligned && page_size % 16 == 0 && (head_dim == 32 || head_dim == 64 || head_dim == 128 || head_dim == 256);
+    const bool tiled = dtype == EG_BF16 && aligned && page_size % 16 == 0 && head_dim % 8 == 0;
     const bool wide = tiled && aligned > 1 && (head_dim == 64 || head_dim == 128) && group <= 128;
     const auto units_of = [&](long long tile) { return entries * ((lines + tile - 1) / tile) * num_kv_heads; };
     int row_tile = !tiled ? 0 : lines <= 16 ? 16 : lines <= 32 ? 32 : 64;
@@ -378,15 +378,17 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
     const int aligned = !tiled ? 0 : rows_at % 16 || a.page_stride % dim || a.head_stride % dim || a.page_stride <= 0 || a.head_stride <= 0 ? 1 : 2;
     int plan[3] = {(int)a.row_tile, (int)a.max_parts, (int)a.part_tiles};
     if (a.row_tile < 0) {
+        // a window's worth of keys and the nodes, where that is less
+        const long long reach = a.window > 0 ? a.window + 2 * a.rows / a.entries : INT, most = a.max_context < reach ? a.max_context : reach, keys = most < 1 ? 1 : most > INT ? INT : most;
         const int code = eg_attention_tree_plan((int)a.dtype, aligned, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
-                                                (int)(a.max_context < 1 ? 1 : a.max_context > INT ? INT : a.max_context), eg_sm_count(), plan);
+                                                (int)keys, eg_sm_count(), plan);
         if (code) return code;
     } else if ((a.row_tile && a.row_tile != 16 && a.row_tile != 32 && a.row_tile != 64 && a.row_tile != 128) || a.max_parts < 1 || a.max_parts > tree::MAX_PARTS ||
                (a.max_parts & (a.max_parts - 1)) || a.part_tiles < 1 || a.part_tiles > 1 << 20) {
         return (int)cudaErrorInvalidValue;
     }
     const int row_tile = plan[0];
-    if (row_tile && (!tiled || (dim != 32 && dim != 64 && dim != 128 && dim != 256) || a.page_size % 16)) return (int)cudaErrorInvalidValue;
+    if (row_tile && (!tiled || dim % 8 || a.page_size % 16)) return (int)cudaErrorInvalidValue;
     if (row_tile == 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
     const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
     const long long tiles = a.rows * group / tile_rows + a.entries;   // at most: every entry's last tile may be a short one

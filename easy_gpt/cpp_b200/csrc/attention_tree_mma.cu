@@ -1,5 +1,5 @@
 // Attention over drafted trees and the paged cache (attention_tree.cuh says which keys a row sees) on the warp-level tensor cores: bfloat16,
-// heads of 32, 64, 128 and 256, pages of a multiple of 16 tokens, caches on 16-byte boundaries.
+// heads of a multiple of 8 up to 256 (columns up to 32, 64, 128 or 256 are zeros), pages of a multiple of 16 tokens, caches on 16-byte boundaries.
 //
 // A CTA of four warps takes 16, 32 or 64 rows (node, query head) of an entry and KV head, so that a key is read once for all of them, and a
 // part of the keys, 64 at a time through a ring of asynchronous copies.  With 64 rows a warp has 16 of them and all 64 keys; with 16 it has
@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
     const int* const table = p.block_table + (size_t)r * p.table_stride;
     const bf16* const q = static_cast<const bf16*>(p.q);
+    const int D = p.head_dim;
 
     // A thread copies the same chunk of rows THREADS / CHUNKS apart, of a tile's keys and values; its rows' quarters have a place in the cache
     // each, looked up a tile ahead of the copies.
@@ -84,14 +85,14 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
 #pragma unroll
         for (int c = 0; c < COPIES; ++c) {
             const int row = my_row + c * STEP, at = tile * KEYS + row, here = page[STEP >= 16 ? c : c * STEP / 16];
-            const bool needed = at >= first && at < end, valid = needed && here >= 0 && here < p.num_pages;
+            const bool needed = at >= first && at < end, valid = needed && here >= 0 && here < p.num_pages, copied = valid && my_chunk * 8 < D;
             if (needed && !valid) {
                 holes = true;
                 atomicOr(p.status, EG_STATUS_BAD_PAGE);
             }
-            const size_t from = valid ? (size_t)here * p.page_stride + (size_t)kvh * p.head_stride + (size_t)(at % p.page_size) * HD + my_chunk * 8 : 0;
-            cp_async_16(ks + L::offset(row, my_chunk), static_cast<const bf16*>(p.k_cache) + from, valid);
-            cp_async_16(ks + L::TILE_BYTES + L::offset(row, my_chunk), static_cast<const bf16*>(p.v_cache) + from, valid);
+            const size_t from = copied ? (size_t)here * p.page_stride + (size_t)kvh * p.head_stride + (size_t)(at % p.page_size) * D + my_chunk * 8 : 0;
+            cp_async_16(ks + L::offset(row, my_chunk), static_cast<const bf16*>(p.k_cache) + from, copied);
+            cp_async_16(ks + L::TILE_BYTES + L::offset(row, my_chunk), static_cast<const bf16*>(p.v_cache) + from, copied);
         }
     };
     // ---- the tree: parents of the nodes up to the tile's last one, and every row's first cached key
@@ -100,12 +101,12 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     look_up(begin, ahead);
     const int parent = tid <= last_node ? p.parents[e.first + tid] : -1;
     // ---- the rows of q as A fragments
-    auto q_row = [&](int row) { return q + (size_t)(e.first + (row0 + row) / group) * p.ldq + (size_t)(kvh * group + (row0 + row) % group) * HD; };
+    auto q_row = [&](int row) { return q + (size_t)(e.first + (row0 + row) / group) * p.ldq + (size_t)(kvh * group + (row0 + row) % group) * D; };
     uint32_t qf[L::Q_IN_SMEM ? 1 : HD / 16][4];
     if constexpr (L::Q_IN_SMEM) {
         for (int i = tid; i < ROWS * HD / 2; i += THREADS) {
             const int row = i / (HD / 2), pair = i % (HD / 2);
-            *reinterpret_cast<uint32_t*>(q_s + L::offset(row, pair / 4) + pair % 4 * 4) = row < count ? *reinterpret_cast<const uint32_t*>(q_row(row) + 2 * pair) : 0u;
+            *reinterpret_cast<uint32_t*>(q_s + L::offset(row, pair / 4) + pair % 4 * 4) = row < count && 2 * pair < D ? *reinterpret_cast<const uint32_t*>(q_row(row) + 2 * pair) : 0u;
         }
     } else {
         const int a = wr * 16 + gid, b = a + 8;
@@ -114,10 +115,11 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
             const int d = k * 16 + 2 * tig;
-            qf[k][0] = a < count ? *reinterpret_cast<const uint32_t*>(qa + d) : 0u;
-            qf[k][1] = b < count ? *reinterpret_cast<const uint32_t*>(qb + d) : 0u;
-            qf[k][2] = a < count ? *reinterpret_cast<const uint32_t*>(qa + d + 8) : 0u;
-            qf[k][3] = b < count ? *reinterpret_cast<const uint32_t*>(qb + d + 8) : 0u;
+            const bool low = d < D, high = d + 8 < D;
+            qf[k][0] = a < count && low ? *reinterpret_cast<const uint32_t*>(qa + d) : 0u;
+            qf[k][1] = b < count && low ? *reinterpret_cast<const uint32_t*>(qb + d) : 0u;
+            qf[k][2] = a < count && high ? *reinterpret_cast<const uint32_t*>(qa + d + 8) : 0u;
+            qf[k][3] = b < count && high ? *reinterpret_cast<const uint32_t*>(qb + d + 8) : 0u;
         }
     }
 #pragma unroll
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
 
     cp_async_wait<0>();
     auto line_of = [&](int row) {                                    // where a row's results go
-        return static_cast<bf16*>(p.out) + (size_t)(e.first + (row0 + row) / group) * p.ldo + (size_t)(kvh * group + (row0 + row) % group) * HD;
+        return static_cast<bf16*>(p.out) + (size_t)(e.first + (row0 + row) / group) * p.ldo + (size_t)(kvh * group + (row0 + row) % group) * D;
     };
     auto put4 = [&](int row, int d, float4 v) {
         uint32_t* const at = reinterpret_cast<uint32_t*>(line_of(row) + d);
@@ -322,6 +324,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
         const float i0 = l0 > 0.f ? 1.f / l0 : l0, i1 = l1 > 0.f ? 1.f / l1 : l1;
 #pragma unroll
         for (int j = 0; j < HD / 8; ++j) {
+            if (8 * j >= D) break;
             if (a < count) *reinterpret_cast<uint32_t*>(line_of(a) + 8 * j + 2 * tig) = pack_bf16(acc[j][0] * i0, acc[j][1] * i0);
             if (b < count) *reinterpret_cast<uint32_t*>(line_of(b) + 8 * j + 2 * tig) = pack_bf16(acc[j][2] * i1, acc[j][3] * i1);
         }
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
         *reinterpret_cast<float2*>(ml_s + 2 * (warp * 16 + gid + 8)) = make_float2(m1, l1);
     }
     if constexpr (WK == 1) {
-        tree::add_parts<THREADS>(o_s, L::MERGE_LD, ml_s, count, HD, parts, put4);
+        tree::add_parts<THREADS>(o_s, L::MERGE_LD, ml_s, count, D, parts, put4);
     } else {
         __syncthreads();
         for (int i = tid; i < ROWS * (HD / 4); i += THREADS) {
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
             }
             if (parts == 1) {
                 const float inv = total > 0.f ? 1.f / total : total;
-                if (row < count) put4(row, d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+                if (row < count && d < D) put4(row, d, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
             } else {                                                 // into its own line: nobody else reads this quad
                 *reinterpret_cast<float4*>(o_s + line0 * L::MERGE_LD + d) = sum;
                 if (d == 0) *reinterpret_cast<float2*>(row_ml + 2 * row) = make_float2(top, total);
@@ -369,13 +372,13 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
         }
         if (parts > 1) {
             // the lines of a row group lie WK * 16 apart
-            if constexpr (WK == 4) tree::add_parts<THREADS>(o_s, L::MERGE_LD, row_ml, count, HD, parts, put4);
+            if constexpr (WK == 4) tree::add_parts<THREADS>(o_s, L::MERGE_LD, row_ml, count, D, parts, put4);
             else {
                 __syncthreads();
                 for (int i = tid; i < 16 * (HD / 4); i += THREADS)   // the second group's to behind the first's
                     *reinterpret_cast<float4*>(o_s + (16 + i / (HD / 4)) * L::MERGE_LD + i % (HD / 4) * 4) =
                         *reinterpret_cast<const float4*>(o_s + (32 + i / (HD / 4)) * L::MERGE_LD + i % (HD / 4) * 4);
-                tree::add_parts<THREADS>(o_s, L::MERGE_LD, row_ml, count, HD, parts, put4);
+                tree::add_parts<THREADS>(o_s, L::MERGE_LD, row_ml, count, D, parts, put4);
             }
         }
     }
@@ -396,14 +399,8 @@ namespace tree {
 // Rows per CTA 16, 32 or 64; tiles of 64 keys.  The caller has checked what this kernel takes.
 int launch_mma(cudaStream_t stream, const Params& p, int row_tile, int tiles) {
 #define EG_ROWS(HD) (row_tile == 16 ? launch<HD, 1>(stream, p, tiles) : row_tile == 32 ? launch<HD, 2>(stream, p, tiles) : launch<HD, 4>(stream, p, tiles))
-    switch (p.head_dim) {
-        case 32: return EG_ROWS(32);
-        case 64: return EG_ROWS(64);
-        case 128: return EG_ROWS(128);
-        case 256: return EG_ROWS(256);
-    }
+    return p.head_dim <= 32 ? EG_ROWS(32) : p.head_dim <= 64 ? EG_ROWS(64) : p.head_dim <= 128 ? EG_ROWS(128) : EG_ROWS(256);
 #undef EG_ROWS
-    return (int)cudaErrorInvalidValue;
 }
 
 }  // namespace tree

@@ -96,7 +96,7 @@ def test_launchers_refuse_sizes_they_do_not_take():
     assert lib.eg_attention_tree(None, None) == 1
     for wrong in (dict(dtype=2), dict(heads=3), dict(kv_heads=0), dict(dim=0), dict(dim=257), dict(page=0), dict(pages=0), dict(parts=0), dict(tiles=0), dict(parts=3), dict(parts=32), dict(status=0),
                   dict(entries=65536), dict(rows=1 << 30), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(window=-1), dict(table_pages=-1), dict(row_tile=8),
-                  dict(row_tile=16, dtype=kernels.F32), dict(row_tile=16, dim=80), dict(row_tile=64, page=24), dict(row_tile=32, q=at + 2), dict(row_tile=16, ldq=257),
+                  dict(row_tile=16, dtype=kernels.F32), dict(row_tile=16, dim=84), dict(row_tile=64, page=24), dict(row_tile=32, q=at + 2), dict(row_tile=16, ldq=257),
                   dict(row_tile=16, cache=at + 8), dict(row_tile=128, dim=32), dict(row_tile=128, q=at + 8), dict(row_tile=128, dim=128, ldq=260), dict(row_tile=128, heads=258), dict(row_tile=256)):
         assert attend(**wrong) == 1, wrong
 
@@ -105,11 +105,11 @@ def test_plans():
     """From sizes alone: what the tensor-core kernels do not take on the 32-bit one, short contexts of few units on the warp-level one, the rest of heads of 64
     and 128 on tcgen05; never more parts than CTAs find room, and more of them the fewer units there are."""
     plan = kernels.attention_tree_plan
-    assert plan(kernels.F32, 2, 8, 1, 14, 2, 64, 16, 500)[0] == plan(kernels.BF16, 2, 8, 1, 14, 2, 80, 16, 500)[0] == plan(kernels.BF16, 2, 8, 1, 14, 2, 64, 24, 500)[0] == 0
+    assert plan(kernels.F32, 2, 8, 1, 14, 2, 64, 16, 500)[0] == plan(kernels.BF16, 2, 8, 1, 14, 2, 68, 16, 500)[0] == plan(kernels.BF16, 2, 8, 1, 14, 2, 64, 24, 500)[0] == 0
     assert plan(kernels.BF16, 0, 8, 1, 14, 2, 64, 16, 500)[0] == 0
     assert [plan(kernels.BF16, 2, 8, 1, 14, 2, 64, 16, keys)[0] for keys in (500, 1024, 1025, 30000)] == [16, 16, 128, 128]
     assert plan(kernels.BF16, 2, 1024, 64, 12, 2, 128, 64, 700)[0] == 128
-    assert [plan(kernels.BF16, aligned, 64 * n, 64, 14, 2, dim, 16, 5000)[0] for aligned, dim in ((1, 64), (2, 32), (2, 256)) for n in (1, 4, 64)] == [16, 32, 64] * 3
+    assert [plan(kernels.BF16, aligned, 64 * n, 64, 14, 2, dim, 16, 5000)[0] for aligned, dim in ((1, 64), (2, 32), (2, 80), (2, 256)) for n in (1, 4, 64)] == [16, 32, 64] * 4
     for aligned in (0, 1, 2):
         for nodes in (1, 9, 64, 300):
             parts = [plan(kernels.BF16, aligned, nodes * entries, entries, 28, 4, 128, 64, 4000)[1] for entries in (1, 4, 16, 64, 256)]

@@ -99,7 +99,7 @@ def check(step, window=None, scale=None, **options):
         assert float(off.max()) <= tolerance(step.dtype, step.dim), (float(off.max()), int(off.argmax()))
 
 
-HEADS = [(14, 2, 64), (12, 2, 128), (8, 8, 64), (6, 1, 32), (4, 2, 256), (3, 3, 80), (16, 1, 128), (2, 1, 18)]
+HEADS = [(14, 2, 64), (4, 4, 40), (6, 2, 136), (12, 2, 128), (8, 8, 64), (6, 1, 32), (4, 2, 256), (3, 3, 80), (16, 1, 128), (2, 1, 18)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -140,7 +140,7 @@ def run_plan(step, plan, window=None):
 
 @pytest.mark.parametrize("parts, part_tiles", [(1, 1), (2, 3), (8, 1), (16, 1)])
 @pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
-@pytest.mark.parametrize("heads, window", [((14, 2, 64), None), ((14, 2, 64), 50), ((28, 4, 128), None), ((16, 1, 128), 200), ((3, 3, 64), 70), ((4, 2, 32), None), ((8, 1, 256), 33)])
+@pytest.mark.parametrize("heads, window", [((14, 2, 64), None), ((14, 2, 64), 50), ((28, 4, 128), None), ((16, 1, 128), 200), ((3, 3, 64), 70), ((4, 2, 32), None), ((8, 1, 256), 33), ((6, 2, 80), None), ((4, 1, 200), 90), ((5, 5, 8), None)])
 def test_attention_tree_every_kernel(heads, window, row_tile, parts, part_tiles):
     """Every kernel and cut by name, whatever the rule would choose: entries of less than a tile of rows, of one and of several; parts without keys."""
     if row_tile == 128 and heads[2] not in (64, 128) or parts == 16 and heads[2] == 256:
