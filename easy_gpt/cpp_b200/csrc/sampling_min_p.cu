@@ -32,6 +32,7 @@ constexpr int SLICE = 20480, MOST_SLICE = 50176;                     // logits o
 constexpr double ONE = 4398046511104.0;                              // 2^42: with 2^20 tokens sums stay below 2^62
 constexpr int MOST_TOKENS = 1 << 20;
 constexpr float COUNT_RANGE = 32.f, WEIGHT_RANGE = 30.f;             // what a histogram's steps span below the largest logit; of weights in units of T
+constexpr int WEIGHTY_STEPS = 500;                                   // whose tokens all have a weight: exp(-30 500 / 512) 2^42 > 0.8
 constexpr float NO_WEIGHT = 31.f;                                    // exp(-31) 2^42 < 1/4
 
 // larger numbers have larger keys; NaN has key 0
@@ -90,7 +91,7 @@ struct Shared {
     __align__(16) u64 weights[LIST];                                 // of the list; a histogram's sums over the CTAs, count and weight a step
     float group_most[GROUPS];
     unsigned bin_weight[LIMBS][BINS], bin_count[BINS];
-    unsigned listed;
+    unsigned listed, gathered, room;
     int found;
     float floats[WARPS];
     u64 pair[4];
@@ -133,22 +134,39 @@ __device__ __forceinline__ void block_scan(u64& a, u64& b, Shared& s) {
     b += __shfl_sync(0xffffffffu, y, 0);
 }
 
-// Descending, n a power of two up to 2 THREADS.  A thread has a pair of every stage; pairs no more than 32 apart are within a warp's 64 places, and
-// stages of those need no barrier of the CTA.
+// Descending, n a power of two up to 2 THREADS.  A thread has two neighbours in registers; their partners up to 32 places away are in its warp, the others
+// come through shared memory.  (All stages there: 5 us for 1,024.)
 __device__ __forceinline__ void sort_descending(u64* list, int n) {
-    const int i = threadIdx.x;
+    const int t = threadIdx.x;
+    const bool mine = t < n / 2;
     __syncthreads();
-    for (int size = 2; size <= n; size *= 2)
-        for (int step = size / 2; step > 0; step /= 2) {
-            if (i < n / 2) {
-                const int a = 2 * i - (i & (step - 1)), b = a + step;
-                const u64 x = list[a], y = list[b];
-                if ((x < y) == ((a & size) == 0)) list[a] = y, list[b] = x;
+    u64 x = mine ? list[2 * t] : 0, y = mine ? list[2 * t + 1] : 0;
+    for (int size = 2; size <= n; size *= 2) {
+        const bool falls = (2 * t & size) == 0;
+        for (int step = size / 2; step > 1; step /= 2) {
+            u64 px, py;
+            if (step > 32) {
+                __syncthreads();
+                if (mine) list[2 * t] = x, list[2 * t + 1] = y;
+                __syncthreads();
+                px = mine ? list[2 * t ^ step] : 0;
+                py = mine ? list[(2 * t ^ step) + 1] : 0;
+            } else {
+                px = __shfl_xor_sync(0xffffffffu, x, step / 2);
+                py = __shfl_xor_sync(0xffffffffu, y, step / 2);
             }
-            const int next = step > 1 ? step / 2 : size;             // the next stage's step
-            if (step > 32 || next > 32) __syncthreads();
-            else __syncwarp();
+            const bool larger = ((2 * t & step) == 0) == falls;      // this place keeps the larger of the two
+            x = (px > x) == larger ? px : x;
+            y = (py > y) == larger ? py : y;
         }
+        if ((x < y) == falls) {
+            const u64 z = x;
+            x = y;
+            y = z;
+        }
+    }
+    __syncthreads();
+    if (mine) list[2 * t] = x, list[2 * t + 1] = y;
     __syncthreads();
 }
 __device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (32 - __clz(n - 1)); }
@@ -167,7 +185,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     static_assert(BINS == THREADS, "a thread a step");
     auto clear_bins = [&]() { s.bin_count[tid] = s.bin_weight[0][tid] = s.bin_weight[1][tid] = s.bin_weight[2][tid] = 0; };
     clear_bins();
-    if (tid == 0) s.listed = 0;
+    if (tid == 0) s.listed = s.gathered = 0;
     if (tid < POWERS) s.power[tid] = exp2((double)tid / POWERS);
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // the others may write here once they know that this CTA runs
     pdl_enter();
@@ -285,10 +303,20 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     };
     const float weighty = largest < INFINITY ? largest - no_weight * 1.0001f - 1e-5f * fabsf(largest) : largest;      // nothing below it has a weight
 
-    // ---- the short list, in the first CTA
+    // ---- the short list, in the first CTA: every CTA gathers its own tokens and finds room for all of them at once (a remote atomic a token had 600
+    // tokens take 11 us)
     auto put_in_list = [&](u64 token) {
-        const unsigned place = remote_add(remote(&s.listed, 0), 1);
-        if (place < LIST) remote_store(remote(&s.list[place], 0), token);
+        const unsigned place = atomicAdd(&s.gathered, 1u);
+        if (place < LIST) s.weights[place] = token;
+    };
+    auto send_list = [&]() {
+        __syncthreads();
+        const unsigned mine = s.gathered;
+        if (tid == 0 && mine) s.room = remote_add(remote(&s.listed, 0), mine);
+        __syncthreads();
+        for (unsigned i = tid; i < mine && i < LIST && s.room + i < LIST; i += THREADS) remote_store(remote(&s.list[s.room + i], 0), s.weights[i]);
+        if (tid == 0) s.gathered = 0;
+        cluster_barrier();
     };
     // The first token whose running sum passes u times the whole: at least 1, and at most the whole itself.
     auto goal_of = [&](u64 total) -> u64 {
@@ -387,7 +415,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     // After the candidates have been put in the list: whether that was all (the draw is done then), or there are too many, which the first CTA tells
     // the others while it goes on.
     auto finish_list = [&](bool by_k, u64 whole) {
-        cluster_barrier();
+        send_list();
         bool done = true;
         if (rank == 0) {
             const unsigned listed = s.listed;
@@ -525,28 +553,16 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     // Narrows a cut down to that token: of the tokens in the cut's step the first ones until before + theirs reach the goal.
     auto narrow = [&](bool by_weight, float scale, Cut cut, u64 count_goal, double weight_goal) {
         u64 before = by_weight ? cut.weight_before : cut.count_before, inside = cut.count;
-        unsigned high_key = 0, low_key = 0;                          // of the step's tokens, once it has been refined
-        bool by_step = true;
+        // keys that the step's tokens lie between (a little apart, for the roundings of step_of), narrowed as the step is refined
+        const bool last_step = cut.step == BINS - 1;
+        const float high = largest - (float)cut.step / scale, slack = 1e-5f * (fabsf(largest) + fabsf((float)cut.step / scale));
+        unsigned high_key = cut.step && high + slack < largest ? key_of(high + slack) : top;
+        unsigned low_key = last_step || !(high - 1.f / scale - slack > -INFINITY) ? MINUS_INFINITY_KEY + 1 : key_of(high - 1.f / scale - slack);
         auto is_inside = [&](float x, u64 token) {
             const unsigned key = (unsigned)(token >> 32);
-            return token >= last && (by_step ? step_of(x, scale) == cut.step && (!by_weight || weight(x) > 0) : key >= low_key && key <= high_key);
+            return token >= last && key >= low_key && key <= high_key && step_of(x, scale) == cut.step && (!by_weight || cut.step < WEIGHTY_STEPS || weight(x) > 0);
         };
         while (inside > LIST) {
-            if (by_step) {                                           // the step's tokens are those of a run of keys
-                unsigned a = 0, b = 0;
-                for_all(-INFINITY, [&](float x, int i) {
-                    const unsigned key = key_of(x);
-                    if (is_inside(x, token_of(key, lo + i))) {
-                        a = max(a, key);
-                        b = max(b, ~key);
-                    }
-                });
-                const u64 most_key = block_join<true>(a, s), most_other = block_join<true>(b, s);
-                exchange(most_key, most_other, true, all, front);
-                high_key = (unsigned)all[0];
-                low_key = ~(unsigned)all[1];
-                by_step = false;
-            }
             if (high_key == low_key) break;
             const int shift = max(0, 32 - __clz(high_key - low_key) - 9);      // at most BINS steps of 2^shift keys
             clear_bins();                                            // every CTA has read the last ones
@@ -583,11 +599,11 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
             }
             result = block_join<true>(result, s);
         } else {
-            for_all(by_step ? -INFINITY : value_of(low_key), [&](float x, int i) {
+            for_all(value_of(low_key), [&](float x, int i) {
                 const u64 token = token_of(key_of(x), lo + i);
                 if (is_inside(x, token)) put_in_list(token);
             });
-            cluster_barrier();
+            send_list();
             const int listed = (int)s.listed;
             if (rank == 0 && listed <= SHORT) {                      // places by counting: four threads a token
                 const int e = tid / 4, part = tid % 4;
