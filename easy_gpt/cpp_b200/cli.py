@@ -14,12 +14,13 @@ from pathlib import Path
 from typing import List, Optional, Tuple
 
 USAGE = """Usage: easy_llm [--model <dir>] [--prompt-file <path>] [--max-steps <n>]
-                [--temperature <float>] [--top-p <float>] [--top-k <int>] [--seed <int>] [--greedy]
+                [--temperature <float>] [--top-p <float>] [--min-p <float>] [--top-k <int>] [--seed <int>] [--greedy]
                 [--token-ids] [--dtype <bfloat16|float32>] ["prompt"]
   -f, --prompt-file <path>  Read prompts from file (one per line, ignore empty lines)
   -m, --max-steps <n>        Maximum generation steps per request (default: 100)
       --temperature <float> Sampling temperature (default: 0.8)
       --top-p <float>        Nucleus sampling cutoff in (0,1] (default: 0.95)
+      --min-p <float>        Least share of the likeliest token's probability, in [0,1] (default: 0, off)
       --top-k <int>          Top-K sampling cutoff, 0 disables (default: 20)
       --seed <int>           RNG seed for sampling (default: 42)
       --greedy               Use greedy decoding (override sampling)
@@ -50,6 +51,7 @@ class CliOptions:
     max_steps: int = 100
     temperature: float = 0.8
     top_p: float = 0.95
+    min_p: float = 0.0
     top_k: int = 20
     seed: int = 42
     use_greedy: bool = False
@@ -103,6 +105,7 @@ def parse_args(argv: List[str]) -> Tuple[Optional[CliOptions], str]:
     float_options = {
         "--temperature": ("temperature", "temperature", lambda v: v > 0.0, "Temperature must be greater than 0"),
         "--top-p": ("top_p", "top-p", lambda v: 0.0 < v <= 1.0, "Top-p must be in (0, 1]"),
+        "--min-p": ("min_p", "min-p", lambda v: 0.0 <= v <= 1.0, "Min-p must be in [0, 1]"),
     }
     while i < len(argv):
         arg = argv[i]
@@ -241,7 +244,7 @@ def main(argv: Optional[List[str]] = None) -> int:
                        max_active=opts.max_active, prefill_batch=opts.prefill_batch,
                        max_batch_tokens=opts.max_batch_tokens, chunk_size=opts.chunk_size)
     outputs = engine.generate(token_prompts, max_steps=opts.max_steps, temperature=opts.temperature, top_p=opts.top_p,
-                              top_k=opts.top_k, seed=opts.seed, greedy=opts.use_greedy)
+                              top_k=opts.top_k, seed=opts.seed, greedy=opts.use_greedy, min_p=opts.min_p)
     lines = [" ".join(map(str, out)) if tokenizer is None else escape_single_line(tokenizer.decode(out)) for out in outputs]
     if opts.prompt_file:
         path = output_path_for(opts.prompt_file)

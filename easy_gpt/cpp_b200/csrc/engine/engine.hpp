@@ -16,17 +16,20 @@
 namespace easygpt::engine {
 
 // Sampling options of one request.  Names and meanings are the reference's command line (src/cli_options.cpp:23-47,
-// 105-198): temperature > 0, top_p in (0, 1], top_k >= 0 (0 disables), seed >= 0, greedy overrides sampling.
+// 105-198): temperature > 0, top_p in (0, 1], top_k >= 0 (0 disables), seed >= 0, greedy overrides sampling.  min_p, in [0, 1] (0 disables), is
+// this engine's own: of what top-k and top-p leave, the tokens with at least min_p times the likeliest one's probability.
 struct SamplingParams {
     float temperature = 0.8f, top_p = 0.95f;
     int top_k = 20;
     long long seed = 42;
     bool greedy = false;
+    float min_p = 0.0f;
     void validate() const {
         if (!greedy && !(temperature > 0.0f)) throw std::invalid_argument("Temperature must be greater than 0");
         if (!(top_p > 0.0f && top_p <= 1.0f)) throw std::invalid_argument("Top-p must be in (0, 1]");
         if (top_k < 0) throw std::invalid_argument("Top-k must be >= 0");
         if (seed < 0) throw std::invalid_argument("Seed must be >= 0");
+        if (!(min_p >= 0.0f && min_p <= 1.0f)) throw std::invalid_argument("Min-p must be in [0, 1]");
     }
     bool is_greedy() const { return greedy || temperature <= 0.0f; }      // src/sampler.cpp:43-49
 };
@@ -92,9 +95,9 @@ public:
         if (so.max_batch_tokens <= 0 || so.chunk_size <= 0 || so.max_active <= 0 || so.prefill_batch <= 0) throw std::invalid_argument("scheduler limits must be positive");
         scheduler.reset(new host::SchedulerCore(&runner->cache.core, so));
         const size_t rows = (size_t)std::max(opt.max_active, 1);
-        sample_params_dev_.allocate(4 * rows * 4);
+        sample_params_dev_.allocate(5 * rows * 4);
         sample_out_dev_.allocate(rows * 4);
-        sample_params_host_.ensure(4 * rows * 4);
+        sample_params_host_.ensure(5 * rows * 4);
         sample_out_host_.ensure(rows * 4);
         max_rows_ = rows;
     }
@@ -239,10 +242,21 @@ private:
                 h[max_rows_ + r] = p.top_p;
                 h[2 * max_rows_ + r] = p.is_greedy() ? 0.0f : uniform_from_counter((uint64_t)p.seed, (uint64_t)req.id, index);
                 ((int*)h)[3 * max_rows_ + r] = p.top_k;
+                h[4 * max_rows_ + r] = p.is_greedy() ? 0.0f : p.min_p;
             }
-            EG_CUDA(cudaMemcpyAsync(sample_params_dev_.get(), h, 4 * max_rows_ * 4, cudaMemcpyHostToDevice, stream));
+            EG_CUDA(cudaMemcpyAsync(sample_params_dev_.get(), h, 5 * max_rows_ * 4, cudaMemcpyHostToDevice, stream));
             const float* d = sample_params_dev_.as<float>();
-            launch_check(eg_sample(stream, logits, vocab, (int)rows, vocab, d, (const int*)(d + 3 * max_rows_), d + max_rows_, d + 2 * max_rows_, out), "sample");
+            // rows with min-p go through a kernel of their own, so that a request's tokens do not hang on what it shares its batch with: a launch for
+            // every run of rows of one kind
+            for (size_t start = 0, end; start < rows; start = end) {
+                const bool with_min_p = h[4 * max_rows_ + start] > 0.0f;
+                for (end = start + 1; end < rows && (h[4 * max_rows_ + end] > 0.0f) == with_min_p;) ++end;
+                const float* x = logits + start * (size_t)vocab;
+                const float *temperature = d + start, *top_p = d + max_rows_ + start, *u = d + 2 * max_rows_ + start, *min_p = d + 4 * max_rows_ + start;
+                const int* top_k = (const int*)(d + 3 * max_rows_ + start);
+                if (with_min_p) launch_check(eg_sample_min_p(stream, x, vocab, (int)(end - start), vocab, temperature, top_k, top_p, min_p, u, out + start), "sample_min_p");
+                else launch_check(eg_sample(stream, x, vocab, (int)(end - start), vocab, temperature, top_k, top_p, u, out + start), "sample");
+            }
         }
         EG_CUDA(cudaMemcpyAsync(sample_out_host_.as<int>(), out, rows * 4, cudaMemcpyDeviceToHost, stream));
         EG_CUDA(cudaStreamSynchronize(stream));

@@ -101,17 +101,22 @@ EGE_API void* ege_engine_create(const char* model_dir, const char* dtype, const 
 }
 EGE_API void ege_engine_destroy(void* e) { delete static_cast<GptEngine*>(e); }
 
-EGE_API long long ege_engine_add_request(void* e, const long long* prompt, long long n, float temperature, float top_p, int top_k, long long seed,
-                                         int greedy, long long max_new_tokens, char* error, int cap) {
+EGE_API long long ege_engine_add_request_min_p(void* e, const long long* prompt, long long n, float temperature, float top_p, int top_k, float min_p,
+                                               long long seed, int greedy, long long max_new_tokens, char* error, int cap) {
     return guarded(error, cap, [&]() {
         SamplingParams p;
         p.temperature = temperature;
         p.top_p = top_p;
         p.top_k = top_k;
+        p.min_p = min_p;
         p.seed = seed;
         p.greedy = greedy != 0;
         return (long long)static_cast<GptEngine*>(e)->add_request(std::vector<int64_t>(prompt, prompt + n), p, max_new_tokens);
     });
+}
+EGE_API long long ege_engine_add_request(void* e, const long long* prompt, long long n, float temperature, float top_p, int top_k, long long seed,
+                                         int greedy, long long max_new_tokens, char* error, int cap) {
+    return ege_engine_add_request_min_p(e, prompt, n, temperature, top_p, top_k, 0.0f, seed, greedy, max_new_tokens, error, cap);
 }
 // one scheduler round and one model step; the ids of the requests that finished go to `finished` (at most cap_finished)
 EGE_API long long ege_engine_step(void* e, long long* finished, int cap_finished, char* error, int cap) {

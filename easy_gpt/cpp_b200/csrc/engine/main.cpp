@@ -22,12 +22,13 @@ namespace {
 
 const char* kUsage =
     "Usage: easy_llm [--model <dir>] [--prompt-file <path>] [--max-steps <n>]\n"
-    "                [--temperature <float>] [--top-p <float>] [--top-k <int>] [--seed <int>] [--greedy]\n"
+    "                [--temperature <float>] [--top-p <float>] [--min-p <float>] [--top-k <int>] [--seed <int>] [--greedy]\n"
     "                [--token-ids] [--dtype <bfloat16|float32>] [\"prompt\"]\n"
     "  -f, --prompt-file <path>  Read prompts from file (one per line, ignore empty lines)\n"
     "  -m, --max-steps <n>        Maximum generation steps per request (default: 100)\n"
     "      --temperature <float> Sampling temperature (default: 0.8)\n"
     "      --top-p <float>        Nucleus sampling cutoff in (0,1] (default: 0.95)\n"
+    "      --min-p <float>        Least share of the likeliest token's probability, in [0,1] (default: 0, off)\n"
     "      --top-k <int>          Top-K sampling cutoff, 0 disables (default: 20)\n"
     "      --seed <int>           RNG seed for sampling (default: 42)\n"
     "      --greedy               Use greedy decoding (override sampling)\n"
@@ -53,7 +54,7 @@ struct CliOptions {
     std::string prompt_file, prompt, model = "data/model", dtype = "bfloat16", config;
     long long max_steps = 100, top_k = 20, seed = 42, random_weights = -1, page_size = 16, cache_tokens = 0, max_active = 16, prefill_batch = 4,
               max_batch_tokens = 2048, chunk_size = 512;
-    double temperature = 0.8, top_p = 0.95;
+    double temperature = 0.8, top_p = 0.95, min_p = 0.0;
     bool use_greedy = false, show_help = false, token_ids = false, chat_template = true;
 };
 
@@ -125,15 +126,18 @@ std::string parse_args(int argc, char** argv, CliOptions* o) {
                 break;
             }
         if (handled) continue;
-        if (arg == "--temperature" || arg == "--top-p") {
+        if (arg == "--temperature" || arg == "--top-p" || arg == "--min-p") {
             std::string v;
             const std::string err = value("number", &v);
             if (!err.empty()) return err;
             double num;
-            if (!whole_real(v, &num)) return std::string("Invalid number for ") + (arg == "--top-p" ? "top-p" : "temperature") + ": " + v;
+            if (!whole_real(v, &num)) return std::string("Invalid number for ") + (arg == "--top-p" ? "top-p" : arg == "--min-p" ? "min-p" : "temperature") + ": " + v;
             if (arg == "--temperature") {
                 if (!(num > 0.0)) return "Temperature must be greater than 0";
                 o->temperature = num;
+            } else if (arg == "--min-p") {
+                if (!(num >= 0.0 && num <= 1.0)) return "Min-p must be in [0, 1]";
+                o->min_p = num;
             } else {
                 if (!(num > 0.0 && num <= 1.0)) return "Top-p must be in (0, 1]";
                 o->top_p = num;
@@ -338,6 +342,7 @@ int main(int argc, char** argv) {
         params.temperature = (float)opts.temperature;
         params.top_p = (float)opts.top_p;
         params.top_k = (int)opts.top_k;
+        params.min_p = (float)opts.min_p;
         params.seed = opts.seed;
         params.greedy = opts.use_greedy;
         const std::vector<std::vector<int64_t>> outputs = engine.generate(token_prompts, params, /*max_new_tokens=*/0, opts.max_steps);

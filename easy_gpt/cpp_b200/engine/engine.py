@@ -181,9 +181,9 @@ class GptEngine:
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: Optional[int] = None,
                  max_steps: Optional[int] = None, temperature: float = 0.8, top_p: float = 0.95, top_k: int = 20,
-                 seed: int = 42, greedy: bool = False) -> List[List[int]]:
+                 seed: int = 42, greedy: bool = False, min_p: float = 0.0) -> List[List[int]]:
         """Generates for every prompt (lists of token ids) and returns the new tokens of each."""
-        params = SamplingParams(temperature=temperature, top_p=top_p, top_k=top_k, seed=seed, greedy=greedy)
+        params = SamplingParams(temperature=temperature, top_p=top_p, top_k=top_k, seed=seed, greedy=greedy, min_p=min_p)
         requests = [self.add_request(p, params, max_new_tokens, max_steps) for p in prompts]
         self.run_to_completion()
         errors = [(r.id, r.error) for r in requests if r.error]

@@ -41,6 +41,8 @@ def library() -> ctypes.CDLL:
         sig = {
             "ege_engine_create": (c_void_p, [c_char_p, c_char_p, c_void_p, c_char_p, c_int]),
             "ege_engine_destroy": (None, [c_void_p]),
+            "ege_engine_add_request_min_p": (c_longlong, [c_void_p, c_void_p, c_longlong, c_float, c_float, c_int, c_float, c_longlong, c_int, c_longlong, c_char_p,
+                                                          c_int]),
             "ege_engine_add_request": (c_longlong, [c_void_p, c_void_p, c_longlong, c_float, c_float, c_int, c_longlong, c_int, c_longlong, c_char_p, c_int]),
             "ege_engine_step": (c_longlong, [c_void_p, c_void_p, c_int, c_char_p, c_int]),
             "ege_engine_has_work": (c_int, [c_void_p]),
@@ -123,8 +125,8 @@ class NativeEngine:
         if max_new_tokens is None:
             max_new_tokens = max(1, (max_steps if max_steps is not None else 100) - len(prompt) + 1)
         arr = np.asarray(list(prompt), dtype=np.int64)
-        rid = self._lib.ege_engine_add_request(self._h, arr.ctypes.data, len(arr), params.temperature, params.top_p, params.top_k, params.seed,
-                                               int(params.greedy), int(max_new_tokens), self._err, _ERR)
+        rid = self._lib.ege_engine_add_request_min_p(self._h, arr.ctypes.data, len(arr), params.temperature, params.top_p, params.top_k, params.min_p, params.seed,
+                                                     int(params.greedy), int(max_new_tokens), self._err, _ERR)
         if rid < 0:
             msg = self._err.value.decode(errors="replace")
             raise ValueError(msg) if "vocabulary" in msg or "must be" in msg else NativeError(msg)
@@ -209,9 +211,10 @@ class NativeEngine:
         return float(out[0]) / 1e3, float(out[1]) / 1e3
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: Optional[int] = None, max_steps: Optional[int] = None,
-                 temperature: float = 0.8, top_p: float = 0.95, top_k: int = 20, seed: int = 42, greedy: bool = False) -> List[List[int]]:
+                 temperature: float = 0.8, top_p: float = 0.95, top_k: int = 20, seed: int = 42, greedy: bool = False,
+                 min_p: float = 0.0) -> List[List[int]]:
         """Generates for every prompt (lists of token ids) and returns the new tokens of each."""
-        params = SamplingParams(temperature=temperature, top_p=top_p, top_k=top_k, seed=seed, greedy=greedy)
+        params = SamplingParams(temperature=temperature, top_p=top_p, top_k=top_k, seed=seed, greedy=greedy, min_p=min_p)
         ids = [self.add_request(p, params, max_new_tokens, max_steps) for p in prompts]
         self.run_to_completion()
         outputs, errors = [], []
