@@ -10,7 +10,7 @@
 // Which keys a row sees is decided by a select, never by adding: a hidden score may be anything.  A hidden value takes part as 0 * v; where
 // there are values that are not finite, every row leaves out those that it does not see.
 #include "attention_tree.cuh"
-#include "attention_tree_args.h"
+#include "tree_args.h"
 
 namespace {
 

@@ -5,7 +5,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
-#include "../attention_tree_args.h"
+#include "../tree_args.h"
 
 extern "C" {
 // activation.cu
@@ -235,7 +235,7 @@ int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int nu
 // sampling_min_p.cu
 int eg_sample_min_p(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* out);
 // tree_step.cu
-int eg_tree_accept(cudaStream_t stream, const int* tokens, const int* targets, const int* entry_starts, const int* parents, int entries, int rows, int longest, int* path, int* accepted, int* emitted, int* status);
+int eg_tree_accept(cudaStream_t stream, const eg_tree_accept_args* args);
 // tree_step.cu
-int eg_cache_keep(cudaStream_t stream, void* kv, int element_size, int layers, int num_pages, int kv_heads, int page_size, int head_dim, long long layer_stride, long long page_stride, long long plane_stride, long long head_stride, const int* block_table, int table_stride, int table_pages, const int* context, const int* path, const int* accepted, int entries, int longest, int* status);
+int eg_cache_keep(cudaStream_t stream, const eg_cache_keep_args* args);
 }  // extern "C"

@@ -5,6 +5,7 @@
 // number of a node's parent in the same entry (lower than its own), -1 for a node without one.  Node 0 is the entry's last token that is
 // known already; the others are drafts.
 #include "common.cuh"
+#include "tree_args.h"
 
 namespace {
 
@@ -143,36 +144,37 @@ __global__ void __launch_bounds__(KEEP_THREADS) cache_keep_kernel(const KeepPara
 
 }  // namespace
 
-// path, emitted: [entries, longest]; accepted: [entries].  rows: how many nodes tokens, targets and parents hold.
-EG_API int eg_tree_accept(cudaStream_t stream, const int* tokens, const int* targets, const int* entry_starts, const int* parents, int entries, int rows, int longest,
-                          int* path, int* accepted, int* emitted, int* status) {
-    if (entries <= 0) return 0;
-    if (rows < 0 || longest < 1 || !status) return (int)cudaErrorInvalidValue;
-    eg_pdl_launch(tree_accept_kernel, dim3((entries + ACCEPT_WARPS - 1) / ACCEPT_WARPS), dim3(ACCEPT_WARPS * 32), 0, stream, tokens, targets, entry_starts, parents,
-                  entries, rows, longest, path, accepted, emitted, status);
+EG_API int eg_tree_accept(cudaStream_t stream, const eg_tree_accept_args* args) {
+    if (!args) return (int)cudaErrorInvalidValue;
+    const eg_tree_accept_args& a = *args;
+    constexpr long long INT = 0x7fffffff;
+    if (a.entries <= 0) return 0;
+    if (a.entries > INT || a.rows < 0 || a.rows > INT || a.longest < 1 || a.longest > INT || !a.status) return (int)cudaErrorInvalidValue;
+    eg_pdl_launch(tree_accept_kernel, dim3((unsigned)((a.entries + ACCEPT_WARPS - 1) / ACCEPT_WARPS)), dim3(ACCEPT_WARPS * 32), 0, stream, a.tokens, a.targets, a.entry_starts,
+                  a.parents, (int)a.entries, (int)a.rows, (int)a.longest, a.path, a.accepted, a.emitted, a.status);
     return eg_launch_status();
 }
 
-// kv: [layers][pages][2][kv_heads][page_size][head_dim] of element_size bytes an element, the strides of the first four in elements.
-// block_table: [entries, table_pages] with row stride table_stride; path: [entries, longest]; context, accepted: [entries].
-EG_API int eg_cache_keep(cudaStream_t stream, void* kv, int element_size, int layers, int num_pages, int kv_heads, int page_size, int head_dim, long long layer_stride,
-                         long long page_stride, long long plane_stride, long long head_stride, const int* block_table, int table_stride, int table_pages,
-                         const int* context, const int* path, const int* accepted, int entries, int longest, int* status) {
-    if (entries <= 0 || layers <= 0) return 0;
-    if (entries > 65535 || num_pages < 1 || kv_heads < 1 || page_size < 1 || head_dim < 1 || longest < 1 || table_pages < 0 || !status ||
-        (element_size != 2 && element_size != 4))
+EG_API int eg_cache_keep(cudaStream_t stream, const eg_cache_keep_args* args) {
+    if (!args) return (int)cudaErrorInvalidValue;
+    const eg_cache_keep_args& a = *args;
+    constexpr long long INT = 0x7fffffff;
+    if (a.entries <= 0 || a.layers <= 0) return 0;
+    if (a.entries > 65535 || a.num_pages < 1 || a.num_pages > INT || a.kv_heads < 1 || a.page_size < 1 || a.page_size > INT || a.head_dim < 1 || a.longest < 1 || a.longest > INT ||
+        a.table_pages < 0 || a.table_pages > INT || a.table_stride < 0 || a.table_stride > INT || !a.status || (a.element_size != 2 && a.element_size != 4))
         return (int)cudaErrorInvalidValue;
     int width = 16;                                                  // bytes of a piece: every row starts on a multiple of it and is made of whole ones
-    const unsigned long long where = (unsigned long long)(uintptr_t)kv | (unsigned long long)element_size *
-        ((unsigned long long)layer_stride | (unsigned long long)page_stride | (unsigned long long)plane_stride | (unsigned long long)head_stride | (unsigned long long)head_dim);
+    const unsigned long long where = (unsigned long long)(uintptr_t)a.kv | (unsigned long long)a.element_size *
+        (unsigned long long)(a.layer_stride | a.page_stride | a.plane_stride | a.head_stride | a.head_dim);
     while (where % width) width /= 2;
-    if (width < element_size) return (int)cudaErrorInvalidValue;
-    const int per = width / element_size;
-    const long long columns = (long long)layers * 2 * kv_heads * (head_dim / per);
-    if (columns > 1ll << 30) return (int)cudaErrorInvalidValue;
-    const KeepParams p = {kv, layer_stride / per, page_stride / per, plane_stride / per, head_stride / per, block_table, context, path, accepted, status,
-                          table_stride, table_pages, num_pages, kv_heads, page_size, head_dim / per, (int)columns, longest};
-    const dim3 grid((unsigned)((columns + KEEP_THREADS - 1) / KEEP_THREADS), entries);
+    if (width < a.element_size) return (int)cudaErrorInvalidValue;
+    const long long per = width / a.element_size, most = 1ll << 30;
+    if (a.layers > most || a.kv_heads > most || a.head_dim > most || a.layers * 2 * a.kv_heads > most || a.layers * 2 * a.kv_heads * (a.head_dim / per) > most)
+        return (int)cudaErrorInvalidValue;
+    const int columns = (int)(a.layers * 2 * a.kv_heads * (a.head_dim / per));
+    const KeepParams p = {a.kv, a.layer_stride / per, a.page_stride / per, a.plane_stride / per, a.head_stride / per, a.block_table, a.context, a.path, a.accepted, a.status,
+                          (int)a.table_stride, (int)a.table_pages, (int)a.num_pages, (int)a.kv_heads, (int)a.page_size, (int)(a.head_dim / per), columns, (int)a.longest};
+    const dim3 grid((unsigned)((columns + KEEP_THREADS - 1) / KEEP_THREADS), (unsigned)a.entries);
     if (width == 16) eg_pdl_launch(cache_keep_kernel<uint4>, grid, dim3(KEEP_THREADS), 0, stream, p);
     else if (width == 8) eg_pdl_launch(cache_keep_kernel<uint2>, grid, dim3(KEEP_THREADS), 0, stream, p);
     else if (width == 4) eg_pdl_launch(cache_keep_kernel<unsigned>, grid, dim3(KEEP_THREADS), 0, stream, p);

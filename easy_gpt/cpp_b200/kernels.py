@@ -102,9 +102,8 @@ class _Signatures:
     eg_sample_min_p = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     eg_attention_tree = [c_void_p, ctypes.c_char_p]
     eg_attention_tree_plan = [c_int] * 10 + [c_void_p]
-    eg_tree_accept = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
-    eg_cache_keep = [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_longlong, c_longlong, c_longlong, c_longlong, c_void_p, c_int, c_int,
-                     c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p]
+    eg_tree_accept = [c_void_p, ctypes.c_char_p]
+    eg_cache_keep = [c_void_p, ctypes.c_char_p]
 
 
 class Timeline:
@@ -953,7 +952,8 @@ def attention_tree_plan(dtype: int, aligned: int, rows: int, entries: int, num_h
     return tuple(plan)
 
 
-_pack_attention_tree = struct.Struct("=28qd").pack         # the fields of attention_tree_args.h
+# the blocks of tree_args.h
+_pack_attention_tree, _pack_tree_accept, _pack_cache_keep = struct.Struct("=28qd").pack, struct.Struct("=11q").pack, struct.Struct("=20q").pack
 
 
 def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, entry_starts: torch.Tensor,
@@ -1012,11 +1012,12 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch
     nodes (at most P), then -1; accepted [entries]: how many they are; emitted [entries, P]: the model's answer at each, which is the entry's
     new tokens (the last one is drafted by nobody), then -1.  An entry without rows accepts 0.  Bit 16 of ``status``: rows or a parent that
     cannot be."""
-    device = _device_of(tokens, targets, entry_starts, parents, path, accepted, emitted, status)
+    tensors = tokens, targets, entry_starts, parents, path, accepted, emitted, status
+    device = _device_of(*tensors)
     if device != _current_device():
         with torch.cuda.device(device):
-            return tree_accept(tokens, targets, entry_starts, parents, path, accepted, emitted, status)
-    for t in (tokens, targets, entry_starts, parents, path, accepted, emitted, status):
+            return tree_accept(*tensors)
+    for t in tensors:
         if t.dtype is not _I32 or not t.is_contiguous():
             raise KernelError("contiguous int32 tensors")
     entries, rows, shape = entry_starts.numel() - 1, tokens.numel(), path.shape
@@ -1024,8 +1025,9 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch
         raise KernelError("one target and one parent per token, entry_starts [entries + 1]")
     if len(shape) != 2 or shape[0] != entries or shape[1] < 1 or emitted.shape != shape or accepted.numel() < entries:
         raise KernelError("path and emitted [entries, P], accepted [entries]")
-    _check(library().eg_tree_accept(_stream_of(device), tokens.data_ptr(), targets.data_ptr(), entry_starts.data_ptr(), parents.data_ptr(), entries, rows, shape[1],
-                                    path.data_ptr(), accepted.data_ptr(), emitted.data_ptr(), status.data_ptr()), "tree_accept")
+    _check(library().eg_tree_accept(_stream_of(device), _pack_tree_accept(
+        tokens.data_ptr(), targets.data_ptr(), entry_starts.data_ptr(), parents.data_ptr(), path.data_ptr(), accepted.data_ptr(), emitted.data_ptr(), status.data_ptr(),
+        entries, rows, shape[1])), "tree_accept")
 
 
 def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, context: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor,
@@ -1053,9 +1055,9 @@ def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, context: torch.Tenso
         raise KernelError("path [entries, P], accepted and context [entries]")
     if block_table.dtype is not _I32 or len(table_shape) != 2 or table_shape[0] < path_shape[0] or (block_table.stride(1) != 1 and table_shape[1] > 1):
         raise KernelError("an int32 block table [entries, pages]")
-    _check(library().eg_cache_keep(_stream_of(device), kv.data_ptr(), element_size, layers, pages, kv_heads, page_size, head_dim, layer_stride, page_stride, plane_stride,
-                                   head_stride, block_table.data_ptr(), block_table.stride(0), table_shape[1], context.data_ptr(), path.data_ptr(), accepted.data_ptr(),
-                                   path_shape[0], path_shape[1], status.data_ptr()), "cache_keep")
+    _check(library().eg_cache_keep(_stream_of(device), _pack_cache_keep(
+        kv.data_ptr(), block_table.data_ptr(), context.data_ptr(), path.data_ptr(), accepted.data_ptr(), status.data_ptr(), element_size, layers, pages, kv_heads, page_size,
+        head_dim, layer_stride, page_stride, plane_stride, head_stride, block_table.stride(0), table_shape[1], path_shape[0], path_shape[1])), "cache_keep")
 
 
 def wait_probe(limit: int, threads: int, status: torch.Tensor) -> int:

@@ -77,15 +77,16 @@ def test_launchers_refuse_sizes_they_do_not_take():
     lib, at = kernels.library(), 0x1000
     sample = lambda rows, vocab: lib.eg_sample_min_p(None, at, vocab, rows, vocab, at, at, at, at, at, at)  # noqa: E731
     assert [sample(0, 8), sample(1, 0), sample(1, (1 << 20) + 1)] == [0, 1, 1]
-    accept = lambda entries, rows, longest, status=at: lib.eg_tree_accept(None, at, at, at, at, entries, rows, longest, at, at, at, status)  # noqa: E731
-    assert [accept(0, 0, 1), accept(1, -1, 1), accept(1, 1, 0), accept(1, 1, 1, None)] == [0, 1, 1, 1]
+    accept = lambda entries, rows, longest, status=at: lib.eg_tree_accept(None, kernels._pack_tree_accept(at, at, at, at, at, at, at, status, entries, rows, longest))  # noqa: E731
+    assert [accept(0, 0, 1), accept(1, -1, 1), accept(1, 1, 0), accept(1, 1, 1, 0), accept(1, 1 << 31, 1), accept(1 << 31, 1, 1), lib.eg_tree_accept(None, None)] == [0, 1, 1, 1, 1, 1, 1]
 
     def keep(kv=at, size=2, layers=1, pages=4, heads=2, page=16, dim=64, entries=1, longest=3, status=at):
-        return lib.eg_cache_keep(None, kv, size, layers, pages, heads, page, dim, 0, 2 * heads * page * dim, heads * page * dim, page * dim, at, 2, 2, at, at, at, entries, longest, status)
+        return lib.eg_cache_keep(None, kernels._pack_cache_keep(kv, at, at, at, at, status, size, layers, pages, heads, page, dim, 0, 2 * heads * page * dim, heads * page * dim, page * dim, 2, 2,
+                                                                entries, longest))
 
     assert [keep(entries=0), keep(layers=0)] == [0, 0]
-    assert [keep(size=1), keep(size=8), keep(pages=0), keep(heads=0), keep(page=0), keep(dim=0), keep(longest=0), keep(status=None), keep(entries=65536), keep(kv=at + 1),
-            keep(layers=1 << 30)] == [1] * 11
+    assert [keep(size=1), keep(size=8), keep(pages=0), keep(heads=0), keep(page=0), keep(dim=0), keep(longest=0), keep(status=0), keep(entries=65536), keep(kv=at + 1),
+            keep(layers=1 << 30), keep(layers=1 << 40), lib.eg_cache_keep(None, None)] == [1] * 13
 
     def attend(dtype=kernels.BF16, rows=4, entries=1, heads=4, kv_heads=2, dim=64, page=16, pages=4, parts=1, tiles=1, status=at, q=at, ldq=256, row_tile=0, scale=0.125,
                window=0, table_pages=3, cache=at):
