@@ -4,8 +4,9 @@
 // A CTA takes 64 rows (node, query head) of an entry and KV head and a part of the keys, 32 at a time, in shared memory as float32; 256
 // threads have 4 rows x 2 keys of the scores and 4 rows x (head size / 16) columns of the output each.  Sums, reference and exponents are
 // 32-bit, the reference is the running maximum.  Where rows of float32 are whole 16-byte pieces, the next tile comes by
-// asynchronous copies while this one is worked on; else a tile is read and converted when it is its turn.  Bound by the multiply-adds, and with few
-// keys a part by the trips to memory in front of the first tile.
+// asynchronous copies while this one is worked on; else a tile is read and converted when it is its turn.  Bound by shared memory: a 16-byte read of
+// a warp takes four cycles whatever its lanes share, 9,200 cycles a tile (5 us) where the multiply-adds take 4,100; thread tiles of 8 x 8 would
+// halve that and leave a CTA two warps.  (Four requests of up to 1,000 keys, 12 heads of 128: 34 us, of which 15 are the start and the adding up.)
 //
 // Which keys a row sees is decided by a select, never by adding: a hidden score may be anything.  A hidden value takes part as 0 * v; where
 // there are values that are not finite, every row leaves out those that it does not see.
@@ -19,6 +20,26 @@ using tree::Params;
 
 constexpr int ROWS = 64, KEYS = 32, THREADS = 256, STAGED_NODES = 1024;
 constexpr int LISTED = 16;                                           // key tiles whose places in the cache are looked up at a time
+
+// two float32 in 64 bits, for the packed instructions
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pair_of(float low, float high) {
+    u64 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(low), "f"(high));
+    return d;
+}
+__device__ __forceinline__ float low_of(u64 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float high_of(u64 v) { return __uint_as_float((unsigned)(v >> 32)); }
+__device__ __forceinline__ u64 fma_pair(u64 a, u64 b, u64 c) {
+    u64 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ u64 mul_pair(u64 a, u64 b) {
+    u64 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 
 template <int DMAX>
 struct Layout {
@@ -144,13 +165,14 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
     }
     const int tx = tid & 15, ty = tid >> 4;                          // keys tx, tx + 16; rows 4 ty ..; columns 4 tx + 64 c ..
     const float scale_log2 = p.scale * 1.4426950408889634f;
-    float m[4], l[4], acc[4][COLS][4];
+    float m[4], l[4];
+    u64 acc[4][COLS][2];                                             // pairs of columns
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) acc[i][c][0] = acc[i][c][1] = acc[i][c][2] = acc[i][c][3] = 0.f;
+        for (int c = 0; c < COLS; ++c) acc[i][c][0] = acc[i][c][1] = 0;
     }
     for (int tile = begin; tile < stop; ++tile) {
         const int key0 = tile * KEYS;
@@ -199,18 +221,26 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
             odd = __syncthreads_or(odd);
         }
         // ---- scores
-        float s[4][2] = {};
+        // (multiply-adds on pairs: of neighbouring terms here, of neighbouring columns below; half the instructions)
+        float s[4][2];
+        {
+            u64 sums[4][2] = {};
 #pragma unroll 8
-        for (int d = 0; d < DMAX; d += 4) {
-            float4 a[4], b[2];
+            for (int d = 0; d < DMAX; d += 4) {
+                ulonglong2 a[4], b[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(q_s + (4 * ty + i) * L::LD + d);
+                for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(q_s + (4 * ty + i) * L::LD + d);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const float4*>(k_s + (tx + 16 * j) * L::LD + d);
+                for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(k_s + (tx + 16 * j) * L::LD + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) sums[i][j] = fma_pair(a[i].y, b[j].y, fma_pair(a[i].x, b[j].x, sums[i][j]));
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) s[i][j] = fmaf(a[i].x, b[j].x, fmaf(a[i].y, b[j].y, fmaf(a[i].z, b[j].z, fmaf(a[i].w, b[j].w, s[i][j]))));
+                for (int j = 0; j < 2; ++j) s[i][j] = low_of(sums[i][j]) + high_of(sums[i][j]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -236,10 +266,9 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
             for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             l[i] = l[i] * keep + sum;
             m[i] = now;
+            const u64 both = pair_of(keep, keep);
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) acc[i][c][x] *= keep;
+            for (int c = 0; c < COLS; ++c) acc[i][c][0] = mul_pair(acc[i][c][0], both), acc[i][c][1] = mul_pair(acc[i][c][1], both);
         }
         __syncwarp();                                                // a row's weights come from its own half warp
         // ---- output
@@ -251,15 +280,18 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
                 for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(p_s + (4 * ty + i) * L::P_LD + key);
 #pragma unroll
                 for (int c = 0; c < COLS; ++c) {
-                    float4 v[4];
+                    ulonglong2 v[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const float4*>(v_s + (key + x) * L::LD + 4 * tx + 64 * c);
+                    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const ulonglong2*>(v_s + (key + x) * L::LD + 4 * tx + 64 * c);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        acc[i][c][0] = fmaf(w[i].w, v[3].x, fmaf(w[i].z, v[2].x, fmaf(w[i].y, v[1].x, fmaf(w[i].x, v[0].x, acc[i][c][0]))));
-                        acc[i][c][1] = fmaf(w[i].w, v[3].y, fmaf(w[i].z, v[2].y, fmaf(w[i].y, v[1].y, fmaf(w[i].x, v[0].y, acc[i][c][1]))));
-                        acc[i][c][2] = fmaf(w[i].w, v[3].z, fmaf(w[i].z, v[2].z, fmaf(w[i].y, v[1].z, fmaf(w[i].x, v[0].z, acc[i][c][2]))));
-                        acc[i][c][3] = fmaf(w[i].w, v[3].w, fmaf(w[i].z, v[2].w, fmaf(w[i].y, v[1].w, fmaf(w[i].x, v[0].w, acc[i][c][3]))));
+                        const float each[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const u64 both = pair_of(each[x], each[x]);
+                            acc[i][c][0] = fma_pair(both, v[x].x, acc[i][c][0]);
+                            acc[i][c][1] = fma_pair(both, v[x].y, acc[i][c][1]);
+                        }
                     }
                 }
             }
@@ -270,9 +302,11 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
                     if (!(seen[4 * ty + i] >> key & 1)) continue;
                     const float w = p_s[(4 * ty + i) * L::P_LD + key];
 #pragma unroll
-                    for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) acc[i][c][x] = fmaf(w, v_s[key * L::LD + 4 * tx + 64 * c + x], acc[i][c][x]);
+                    for (int c = 0; c < COLS; ++c) {
+                        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(v_s + key * L::LD + 4 * tx + 64 * c);
+                        acc[i][c][0] = fma_pair(pair_of(w, w), v.x, acc[i][c][0]);
+                        acc[i][c][1] = fma_pair(pair_of(w, w), v.y, acc[i][c][1]);
+                    }
                 }
         }
     }
@@ -290,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
             for (int c = 0; c < COLS; ++c)
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    if (4 * tx + 64 * c + x < D) line[4 * tx + 64 * c + x] = from_f32<T>(acc[i][c][x] * inv);
+                    if (4 * tx + 64 * c + x < D) line[4 * tx + 64 * c + x] = from_f32<T>((x & 1 ? high_of(acc[i][c][x / 2]) : low_of(acc[i][c][x / 2])) * inv);
         }
         return;
     }
@@ -301,7 +335,7 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int c = 0; c < COLS; ++c)
-            *reinterpret_cast<float4*>(o_s + (4 * ty + i) * L::LD + 4 * tx + 64 * c) = make_float4(acc[i][c][0], acc[i][c][1], acc[i][c][2], acc[i][c][3]);
+            *reinterpret_cast<ulonglong2*>(o_s + (4 * ty + i) * L::LD + 4 * tx + 64 * c) = make_ulonglong2(acc[i][c][0], acc[i][c][1]);
         if (tx == 0) *reinterpret_cast<float2*>(ml_s + 2 * (4 * ty + i)) = make_float2(m[i], l[i]);
     }
     tree::add_parts<THREADS>(o_s, L::LD, ml_s, count, DMAX, parts, [&](int row, int d, float4 v) {
