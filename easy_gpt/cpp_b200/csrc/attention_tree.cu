@@ -64,11 +64,11 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
     __shared__ int latest;                                           // the largest of those
     __shared__ long long key_row[LISTED * KEYS];                     // where a key's row lies in the cache; -1: nowhere
     pdl_enter();
-    const int part = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
+    const int part = blockIdx.x % p.max_parts, kvh = blockIdx.y, tid = threadIdx.x;
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
-    if (!tree::find_tile(p, blockIdx.z, ROWS, r, e, within)) return;
+    if (!tree::find_tile(p, blockIdx.x / p.max_parts, ROWS, r, e, within)) return;
     const int D = p.head_dim, row0 = within * ROWS, count = min(ROWS, e.n * group - row0);
     const int last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;    // the tile's keys: first .. end - 1
@@ -348,14 +348,14 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
 }
 
 template <typename T, int DMAX, bool ASYNC>
-int launch(cudaStream_t stream, const Params& p, int tiles) {
+int launch(cudaStream_t stream, const Params& p, long long tiles) {
     constexpr int bytes = Layout<DMAX>::FLOATS * 4;
     static unsigned long long seen = 0;
     if (const int code = tree::prepare_kernel(attention_tree_kernel<T, DMAX, ASYNC>, bytes, seen)) return code;
-    return tree::launch_clusters(attention_tree_kernel<T, DMAX, ASYNC>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, p);
+    return tree::launch_clusters(attention_tree_kernel<T, DMAX, ASYNC>, p.max_parts, p.num_kv_heads, tiles, THREADS, bytes, stream, p);
 }
 template <typename T, bool ASYNC>
-int launch_any(cudaStream_t stream, const Params& p, int tiles) {
+int launch_any(cudaStream_t stream, const Params& p, long long tiles) {
     return p.head_dim <= 64 ? launch<T, 64, ASYNC>(stream, p, tiles) : p.head_dim <= 128 ? launch<T, 128, ASYNC>(stream, p, tiles) : launch<T, 256, ASYNC>(stream, p, tiles);
 }
 
@@ -426,13 +426,12 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
     if (row_tile == 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
     const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
     const long long tiles = a.rows * group / tile_rows + a.entries;   // at most: every entry's last tile may be a short one
-    if (tiles > 65535) return (int)cudaErrorInvalidValue;
     const Params p = {a.q, a.ldq, a.k_cache, a.v_cache, a.page_stride, a.head_stride, a.block_table, (int)a.table_stride, (int)a.table_pages, (int)a.num_pages,
                       a.entry_starts, a.context, a.parents, a.out, a.ldo, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
                       (int)a.window, (float)a.scale, plan[1], plan[2] * (64 / tile_keys), a.status};
     if (row_tile == 128) return tree::launch_tc(stream, p);
-    if (row_tile) return tree::launch_mma(stream, p, row_tile, (int)tiles);
-    if (a.dtype == EG_BF16) return launch_any<bf16, false>(stream, p, (int)tiles);
+    if (row_tile) return tree::launch_mma(stream, p, row_tile, tiles);
+    if (a.dtype == EG_BF16) return launch_any<bf16, false>(stream, p, tiles);
     const bool pieces = (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.ldq | a.page_stride | a.head_stride | a.head_dim) & 3) == 0;
-    return pieces ? launch_any<float, true>(stream, p, (int)tiles) : launch_any<float, false>(stream, p, (int)tiles);
+    return pieces ? launch_any<float, true>(stream, p, tiles) : launch_any<float, false>(stream, p, tiles);
 }

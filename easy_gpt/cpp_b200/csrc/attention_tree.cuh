@@ -58,12 +58,22 @@ __device__ __forceinline__ int sound_parent(const Params& p, int i, int up) {
 __device__ __forceinline__ int parent_of(const Params& p, const Entry& e, int i) { return sound_parent(p, i, p.parents[e.first + i]); }
 
 // The entry whose tile number `tile` is, counting ceil(n * group / row_tile) tiles an entry, and the tile's number within it; false: there
-// is none.  For a whole warp: 32 entries at a time, in one trip to memory.
+// is none.  For a whole warp: 32 entries at a time, in one trip to memory, the next 32 asked for meanwhile.
 __device__ __forceinline__ bool find_tile(const Params& p, int tile, int row_tile, int& r, Entry& e, int& within) {
     const int lane = threadIdx.x & 31, group = p.num_heads / p.num_kv_heads;
+    int first = 0, end = 0, context = 0;
+    const auto ask = [&](int i) {
+        if (i < p.entries) {
+            first = p.entry_starts[i];
+            end = p.entry_starts[i + 1];
+            context = p.context[i];
+        }
+    };
+    ask(lane);
     for (int base = 0; base < p.entries; base += 32) {
         Entry mine = {0, 0, 0};
-        if (base + lane < p.entries) mine = sound(p, p.entry_starts[base + lane], p.entry_starts[base + lane + 1], p.context[base + lane]);
+        if (base + lane < p.entries) mine = sound(p, first, end, context);
+        ask(base + 32 + lane);
         const int tiles = (int)(((long long)mine.n * group + row_tile - 1) / row_tile);
         int upto = tiles;
 #pragma unroll
@@ -92,7 +102,7 @@ __device__ __forceinline__ int first_key(const Params& p, const Entry& e) { retu
 __device__ __forceinline__ int parts_of(const Params& p, int key_tiles) { return max(1, min(p.max_parts, key_tiles / p.part_tiles)); }
 
 // The kernel in attention_tree_mma.cu (16, 32 or 64 rows a CTA, key tiles of 64).  Its caller has checked what it takes.
-int launch_mma(cudaStream_t stream, const Params& p, int row_tile, int tiles);
+int launch_mma(cudaStream_t stream, const Params& p, int row_tile, long long tiles);
 // The kernel in attention_tree_tc.cu (128 rows a CTA, or as many as whole nodes have; key tiles of 64).  Its caller has checked what it takes, but for the
 // size of the tensor maps.
 int launch_tc(cudaStream_t stream, const Params& p);
@@ -160,11 +170,13 @@ __device__ __forceinline__ void add_parts(const float* o, int ld, const float* m
     cluster_barrier();
 }
 
-// A launch whose CTAs along x are clusters, behind the kernel in front as a programmatic dependent.
+// A launch of `tiles` clusters of p.max_parts CTAs for every KV head (blockIdx.x = tile * max_parts + part, blockIdx.y = KV head), behind the kernel in
+// front as a programmatic dependent.
 template <class... P, class... A>
-static inline int launch_clusters(void (*kernel)(P...), dim3 grid, int threads, size_t bytes, cudaStream_t stream, A... args) {
+static inline int launch_clusters(void (*kernel)(P...), int max_parts, int num_kv_heads, long long tiles, int threads, size_t bytes, cudaStream_t stream, A... args) {
+    if (tiles * max_parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3((unsigned)(tiles * max_parts), num_kv_heads);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
@@ -172,7 +184,7 @@ static inline int launch_clusters(void (*kernel)(P...), dim3 grid, int threads, 
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = grid.x;
+    attr[1].val.clusterDim.x = max_parts;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;

@@ -51,12 +51,12 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     __shared__ int lowest[ROWS];                                     // a row's first cached key
     __shared__ int latest;                                           // the largest of those
     pdl_enter();
-    const int part = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int part = blockIdx.x % p.max_parts, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int gid = lane >> 2, tig = lane & 3, wr = warp / WK, wk = warp % WK;
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
-    if (!tree::find_tile(p, blockIdx.z, ROWS, r, e, within)) return;
+    if (!tree::find_tile(p, blockIdx.x / p.max_parts, ROWS, r, e, within)) return;
     const int row0 = within * ROWS, count = min(ROWS, e.n * group - row0), last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
@@ -385,11 +385,11 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
 }
 
 template <int HD, int WR>
-int launch(cudaStream_t stream, const Params& p, int tiles) {
+int launch(cudaStream_t stream, const Params& p, long long tiles) {
     constexpr int bytes = Layout<HD, WR>::SMEM;
     static unsigned long long seen = 0;
     if (const int code = tree::prepare_kernel(attention_tree_mma_kernel<HD, WR>, bytes, seen)) return code;
-    return tree::launch_clusters(attention_tree_mma_kernel<HD, WR>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, p);
+    return tree::launch_clusters(attention_tree_mma_kernel<HD, WR>, p.max_parts, p.num_kv_heads, tiles, THREADS, bytes, stream, p);
 }
 
 }  // namespace
@@ -397,7 +397,7 @@ int launch(cudaStream_t stream, const Params& p, int tiles) {
 namespace tree {
 
 // Rows per CTA 16, 32 or 64; tiles of 64 keys.  The caller has checked what this kernel takes.
-int launch_mma(cudaStream_t stream, const Params& p, int row_tile, int tiles) {
+int launch_mma(cudaStream_t stream, const Params& p, int row_tile, long long tiles) {
 #define EG_ROWS(HD) (row_tile == 16 ? launch<HD, 1>(stream, p, tiles) : row_tile == 32 ? launch<HD, 2>(stream, p, tiles) : launch<HD, 4>(stream, p, tiles))
     return p.head_dim <= 32 ? EG_ROWS(32) : p.head_dim <= 64 ? EG_ROWS(64) : p.head_dim <= 128 ? EG_ROWS(128) : EG_ROWS(256);
 #undef EG_ROWS

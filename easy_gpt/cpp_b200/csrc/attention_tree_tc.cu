@@ -59,7 +59,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     __shared__ float row_ml[2 * BM];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, latest, holes;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.x, kvh = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.x % p.max_parts, kvh = blockIdx.y;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_addr = base, k_ring = base + S::Q_BYTES, v_ring = k_ring + STAGES * S::TILE_BYTES;
     unsigned char* const aligned = smem_raw + (base - smem_addr(smem_raw));
@@ -67,7 +67,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
-    if (!tree::find_tile(p, blockIdx.z, maps.nodes * group, r, e, within)) return;
+    if (!tree::find_tile(p, blockIdx.x / p.max_parts, maps.nodes * group, r, e, within)) return;
     const int node0 = within * maps.nodes, nodes = min(maps.nodes, e.n - node0), count = nodes * group, last_node = node0 + nodes - 1;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
@@ -397,11 +397,11 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
 }
 
 template <int HD>
-int launch(cudaStream_t stream, const Params& p, const Maps& maps, const CUtensorMap& map_k, const CUtensorMap& map_v, int tiles) {
+int launch(cudaStream_t stream, const Params& p, const Maps& maps, const CUtensorMap& map_k, const CUtensorMap& map_v, long long tiles) {
     constexpr int bytes = Shape<HD>::SMEM;
     static unsigned long long seen = 0;
     if (const int code = tree::prepare_kernel(attention_tree_tc_kernel<HD>, bytes, seen)) return code;
-    return tree::launch_clusters(attention_tree_tc_kernel<HD>, dim3(p.max_parts, p.num_kv_heads, tiles), THREADS, bytes, stream, map_k, map_v, p, maps);
+    return tree::launch_clusters(attention_tree_tc_kernel<HD>, p.max_parts, p.num_kv_heads, tiles, THREADS, bytes, stream, map_k, map_v, p, maps);
 }
 
 }  // namespace
@@ -417,12 +417,12 @@ int launch_tc(cudaStream_t stream, const Params& p) {
     maps.head_rows = p.head_stride / p.head_dim;
     const long long kv_rows = (long long)(p.num_pages - 1) * maps.page_rows + (long long)(p.num_kv_heads - 1) * maps.head_rows + p.page_size;
     const long long tiles = (long long)p.rows / maps.nodes + p.entries;
-    if (kv_rows >= (1ll << 31) || tiles > 65535) return (int)cudaErrorInvalidValue;
+    if (kv_rows >= (1ll << 31)) return (int)cudaErrorInvalidValue;
     maps.nowhere = (int)kv_rows;
     CUtensorMap map_k, map_v;
     if (make_map(&map_k, p.k_cache, kv_rows, p.head_dim, p.head_dim, maps.piece_rows) || make_map(&map_v, p.v_cache, kv_rows, p.head_dim, p.head_dim, maps.piece_rows))
         return (int)cudaErrorInvalidValue;
-    return p.head_dim == 64 ? launch<64>(stream, p, maps, map_k, map_v, (int)tiles) : launch<128>(stream, p, maps, map_k, map_v, (int)tiles);
+    return p.head_dim == 64 ? launch<64>(stream, p, maps, map_k, map_v, tiles) : launch<128>(stream, p, maps, map_k, map_v, tiles);
 }
 
 }  // namespace tree

@@ -152,6 +152,53 @@ def test_attention_tree_every_kernel(heads, window, row_tile, parts, part_tiles)
     assert float(((got[:total] - want[:total]).norm(dim=1) / want[:total].norm(dim=1)).max()) <= tolerance(step.dtype, step.dim)
 
 
+@pytest.mark.parametrize("parts", [1, 4])
+@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128)])
+def test_attention_tree_every_kernel_does_not_see_pages_that_are_none(heads, row_tile, parts):
+    """Pages in the middle of a context, the tree's own and the table's end: their keys are left out, which is what the same cache without them gives."""
+    step = Step([*heads, row_tile], [9, 12, 30], [700, 300, 500], *heads, 16)
+    step.block_table[0, 20], step.block_table[0, 3], step.block_table[1, 18] = -1, step.cache.shape[0] + 5, -9
+    step.block_table = step.block_table[:, :32].contiguous()          # entry 0 has 44 pages, entry 2 reaches into page 33
+    got, at, group = run_plan(step, (row_tile, parts, 1)).double(), 0, heads[0] // heads[1]
+    assert int(step.status) == 2
+    for r, (n, c) in enumerate(zip(step.nodes, step.contexts)):
+        gone = {0: {3, 20}, 1: {18}, 2: set()}[r]
+        k, v = step.rows_of(r, 0), step.rows_of(r, 1)
+        for i in range(n):
+            seen = [x for x in [*range(c), *(c + a for a in line_of(step.parents[r], i))] if x // 16 not in gone and x // 16 < 32]
+            q = step.q[at + i].double().view(heads[1], group, heads[2])
+            w = (torch.einsum("ghd,gkd->ghk", q, k[:, seen]) * heads[2] ** -0.5).softmax(-1)
+            want = torch.einsum("ghk,gkd->ghd", w, v[:, seen]).reshape(-1)
+            assert float((got[at + i] - want).norm() / want.norm()) <= tolerance(step.dtype, step.dim), (r, i)
+        at += n
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_tree_many_entries(dtype):
+    """More entries than a warp looks at at once, some without rows, one of them with rows that cannot be in the middle."""
+    rng = np.random.default_rng(3)
+    nodes, contexts = [int(n) for n in rng.integers(0, 4, 150)], [int(c) for c in rng.integers(0, 40, 150)]
+    step = Step(7, nodes, contexts, 4, 2, 64, 16, dtype)
+    check(step)
+    step.context[75] = -1
+    want, got = step.plain(), step.run().double()
+    first = sum(nodes[:75])
+    keep = torch.ones(got.shape[0], dtype=torch.bool, device="cuda")
+    keep[first:first + nodes[75]] = False
+    assert int(step.status) == 16
+    off = (got - want)[keep].norm(dim=1) / want[keep].norm(dim=1)
+    assert float(off.max()) <= tolerance(dtype, 64)
+
+
+def test_attention_tree_no_rows():
+    step = Step(8, [0, 0], [5, 0], 4, 2, 64, 16, pad=3)
+    before = step.out.clone()
+    assert torch.equal(step.run(), before) and int(step.status) == 0
+    step.flat = step.flat[:0]
+    assert torch.equal(step.run(), before) and int(step.status) == 0
+
+
 @pytest.mark.parametrize("row_tile", [0, 16, 64, 128])
 def test_attention_tree_every_kernel_hides_what_is_not_a_number(row_tile):
     step = Step(6, [40, 20], [100, 700], 14, 2, 64, 16, kind="chain")
@@ -449,6 +496,20 @@ def test_sample_min_p_strides_and_rows():
     assert got[:9] == [plain_sample(x[r].cpu().numpy(), float(np.float32(0.9)), 100, float(np.float32(0.9)), float(np.float32(0.01)), float(u[r]))[0] for r in range(9)]
     assert got[9:] == [-9] * 3
     run_sample(wide[:0], 1.0, 0, 1.0, 0.0, 0.5)
+
+
+@pytest.mark.parametrize("vocab", [262147, 600001, 800000, 1048576])
+def test_sample_min_p_large_vocabularies(vocab):
+    """Slices of every size, and rows that 16 CTAs do not hold."""
+    rng = np.random.default_rng(vocab)
+    x = rng.normal(0, 2, size=(len(SETTINGS), vocab)).astype(np.float32)
+    u = rng.random(len(SETTINGS)).astype(np.float32)
+    t, k, p, low = (np.array([s[i] for s in SETTINGS]) for i in range(4))
+    t, p, low = (a.astype(np.float32) for a in (t, p, low))
+    got = run_sample(torch.from_numpy(x).cuda(), t, k, p, low, u).tolist()
+    for r in range(len(SETTINGS)):
+        want, room = plain_sample(x[r], float(t[r]), int(k[r]), float(p[r]), float(low[r]), float(u[r]))
+        assert got[r] == want or room < vocab * 2.0 ** -43, (r, SETTINGS[r], got[r], want, room)
 
 
 def test_sample_min_p_agrees_with_sample():
