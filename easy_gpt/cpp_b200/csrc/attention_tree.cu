@@ -64,11 +64,11 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
     __shared__ int latest;                                           // the largest of those
     __shared__ long long key_row[LISTED * KEYS];                     // where a key's row lies in the cache; -1: nowhere
     pdl_enter();
-    const int part = blockIdx.x % p.max_parts, kvh = blockIdx.y, tid = threadIdx.x;
+    const int part = blockIdx.x % p.max_parts, kvh = blockIdx.x / p.max_parts % p.num_kv_heads, tid = threadIdx.x;
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
-    if (!tree::find_tile(p, blockIdx.x / p.max_parts, ROWS, r, e, within)) return;
+    if (!tree::find_tile(p, blockIdx.x / p.max_parts / p.num_kv_heads, ROWS, r, e, within)) return;
     const int D = p.head_dim, row0 = within * ROWS, count = min(ROWS, e.n * group - row0);
     const int last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;    // the tile's keys: first .. end - 1
@@ -428,7 +428,7 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
     const long long tiles = a.rows * group / tile_rows + a.entries;   // at most: every entry's last tile may be a short one
     const Params p = {a.q, a.ldq, a.k_cache, a.v_cache, a.page_stride, a.head_stride, a.block_table, (int)a.table_stride, (int)a.table_pages, (int)a.num_pages,
                       a.entry_starts, a.context, a.parents, a.out, a.ldo, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
-                      (int)a.window, (float)a.scale, plan[1], plan[2] * (64 / tile_keys), a.status};
+                      (int)a.window, (float)a.scale, plan[1], plan[2] * (64 / tile_keys), a.status, tiles * a.num_kv_heads * plan[1] > 2 * eg_sm_count()};
     if (row_tile == 128) return tree::launch_tc(stream, p);
     if (row_tile) return tree::launch_mma(stream, p, row_tile, tiles);
     if (a.dtype == EG_BF16) return launch_any<bf16, false>(stream, p, tiles);

@@ -31,6 +31,7 @@ struct Params {
     float scale;
     int max_parts, part_tiles;       // a tile's keys are cut into min(max_parts, key tiles / part_tiles) parts, one at least
     int* status;
+    int longest_first;               // tiles of entries with more keys are numbered first (of 32 entries at a time)
 };
 
 // An entry's place in the step.
@@ -58,7 +59,8 @@ __device__ __forceinline__ int sound_parent(const Params& p, int i, int up) {
 __device__ __forceinline__ int parent_of(const Params& p, const Entry& e, int i) { return sound_parent(p, i, p.parents[e.first + i]); }
 
 // The entry whose tile number `tile` is, counting ceil(n * group / row_tile) tiles an entry, and the tile's number within it; false: there
-// is none.  For a whole warp: 32 entries at a time, in one trip to memory, the next 32 asked for meanwhile.
+// is none.  For a whole warp: 32 entries at a time, in one trip to memory, the next 32 asked for meanwhile.  CTAs start in the order of their tiles, and
+// where there are more of them than places, the ones with most keys had better start first: a tile's number then goes by its entry's place in that order.
 __device__ __forceinline__ bool find_tile(const Params& p, int tile, int row_tile, int& r, Entry& e, int& within) {
     const int lane = threadIdx.x & 31, group = p.num_heads / p.num_kv_heads;
     int first = 0, end = 0, context = 0;
@@ -76,12 +78,20 @@ __device__ __forceinline__ bool find_tile(const Params& p, int tile, int row_til
         ask(base + 32 + lane);
         const int tiles = (int)(((long long)mine.n * group + row_tile - 1) / row_tile);
         int upto = tiles;
+        if (p.longest_first) {
+            const int keys = mine.context;
+            for (int j = 0; j < 32; ++j) {
+                const int other = __shfl_sync(0xffffffffu, keys, j), its = __shfl_sync(0xffffffffu, tiles, j);
+                if (other > keys || (other == keys && j < lane)) upto += its;
+            }
+        } else {
 #pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int below = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += below;
+            for (int o = 1; o < 32; o *= 2) {
+                const int below = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += below;
+            }
         }
-        const unsigned here = __ballot_sync(0xffffffffu, tile < upto);
+        const unsigned here = __ballot_sync(0xffffffffu, tile < upto && tile >= upto - tiles);
         if (here) {
             const int who = __ffs(here) - 1;
             r = base + who;
@@ -91,7 +101,7 @@ __device__ __forceinline__ bool find_tile(const Params& p, int tile, int row_til
             within = tile - __shfl_sync(0xffffffffu, upto - tiles, who);
             return true;
         }
-        tile -= __shfl_sync(0xffffffffu, upto, 31);
+        tile -= __reduce_max_sync(0xffffffffu, upto);
     }
     return false;
 }
@@ -170,13 +180,13 @@ __device__ __forceinline__ void add_parts(const float* o, int ld, const float* m
     cluster_barrier();
 }
 
-// A launch of `tiles` clusters of p.max_parts CTAs for every KV head (blockIdx.x = tile * max_parts + part, blockIdx.y = KV head), behind the kernel in
-// front as a programmatic dependent.
+// A launch of `tiles` clusters of p.max_parts CTAs for every KV head (blockIdx.x = (tile * num_kv_heads + KV head) * max_parts + part), behind the kernel
+// in front as a programmatic dependent.
 template <class... P, class... A>
 static inline int launch_clusters(void (*kernel)(P...), int max_parts, int num_kv_heads, long long tiles, int threads, size_t bytes, cudaStream_t stream, A... args) {
-    if (tiles * max_parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    if (tiles * num_kv_heads * max_parts > 0x7fffffff) return (int)cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * max_parts), num_kv_heads);
+    cfg.gridDim = dim3((unsigned)(tiles * num_kv_heads * max_parts));
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;

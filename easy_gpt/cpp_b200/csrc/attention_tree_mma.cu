@@ -51,12 +51,12 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     __shared__ int lowest[ROWS];                                     // a row's first cached key
     __shared__ int latest;                                           // the largest of those
     pdl_enter();
-    const int part = blockIdx.x % p.max_parts, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int part = blockIdx.x % p.max_parts, kvh = blockIdx.x / p.max_parts % p.num_kv_heads, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int gid = lane >> 2, tig = lane & 3, wr = warp / WK, wk = warp % WK;
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
-    if (!tree::find_tile(p, blockIdx.x / p.max_parts, ROWS, r, e, within)) return;
+    if (!tree::find_tile(p, blockIdx.x / p.max_parts / p.num_kv_heads, ROWS, r, e, within)) return;
     const int row0 = within * ROWS, count = min(ROWS, e.n * group - row0), last_node = (row0 + count - 1) / group;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);

@@ -59,7 +59,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     __shared__ float row_ml[2 * BM];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag, latest, holes;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.x % p.max_parts, kvh = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.x % p.max_parts, kvh = blockIdx.x / p.max_parts % p.num_kv_heads;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_addr = base, k_ring = base + S::Q_BYTES, v_ring = k_ring + STAGES * S::TILE_BYTES;
     unsigned char* const aligned = smem_raw + (base - smem_addr(smem_raw));
@@ -67,7 +67,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
-    if (!tree::find_tile(p, blockIdx.x / p.max_parts, maps.nodes * group, r, e, within)) return;
+    if (!tree::find_tile(p, blockIdx.x / p.max_parts / p.num_kv_heads, maps.nodes * group, r, e, within)) return;
     const int node0 = within * maps.nodes, nodes = min(maps.nodes, e.n - node0), count = nodes * group, last_node = node0 + nodes - 1;
     const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
