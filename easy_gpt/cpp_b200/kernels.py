@@ -179,7 +179,7 @@ def _device_of(*tensors) -> int:
     """The one CUDA device of the tensors."""
     device = tensors[0].get_device()
     for t in tensors:
-        if t.get_device() != device or device < 0:
+        if t.get_device() != device or device < 0:          # -1: the host
             raise KernelError("kernels run on CUDA tensors only, all of one device; there is no CPU path")
     return device
 
@@ -937,9 +937,10 @@ def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
     (rows, vocab), (ld, step) = logits.shape, logits.stride()
     if step != 1 or ld < 0 or not 1 <= vocab <= SAMPLE_MAX_VOCAB:
         raise KernelError(f"rows of 1 to {SAMPLE_MAX_VOCAB} logits, side by side")
-    for t, dtype in ((temperature, _F32), (top_k, _I32), (top_p, _F32), (min_p, _F32), (uniform, _F32), (out, _I32)):
-        if t.dtype is not dtype or t.numel() < rows or not t.is_contiguous():
-            raise KernelError("float32 temperature/top_p/min_p/uniform, int32 top_k/out, one value per row, contiguous")
+    if not (temperature.dtype is top_p.dtype is min_p.dtype is uniform.dtype is _F32 and top_k.dtype is out.dtype is _I32
+            and temperature.is_contiguous() and top_k.is_contiguous() and top_p.is_contiguous() and min_p.is_contiguous() and uniform.is_contiguous()
+            and out.is_contiguous() and min(temperature.numel(), top_k.numel(), top_p.numel(), min_p.numel(), uniform.numel(), out.numel()) >= rows):
+        raise KernelError("float32 temperature/top_p/min_p/uniform, int32 top_k/out, one value per row, contiguous")
     _check(library().eg_sample_min_p(_stream_of(device), logits.data_ptr(), ld, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
                                      min_p.data_ptr(), uniform.data_ptr(), out.data_ptr()), "sample_min_p")
 
@@ -978,9 +979,8 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     code = dtype_code(dtype)
     if out.dtype is not dtype or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise KernelError("q, out and the caches of one dtype")
-    for t in (block_table, entry_starts, context, parents, status):
-        if t.dtype is not _I32:
-            raise KernelError("int32 metadata")
+    if not block_table.dtype is entry_starts.dtype is context.dtype is parents.dtype is status.dtype is _I32:
+        raise KernelError("int32 metadata")
     if not 0 < num_kv_heads <= num_heads or num_heads % num_kv_heads or not 0 < head_dim <= 256:
         raise KernelError("heads in whole groups, head sizes up to 256")
     if len(cache_shape) != 4 or cache_shape[1] != num_kv_heads or cache_shape[3] != head_dim or v_cache.shape != cache_shape or v_cache.stride() != cache_stride \
@@ -1013,22 +1013,26 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, entry_starts: torch
     nodes (at most P), then -1; accepted [entries]: how many they are; emitted [entries, P]: the model's answer at each, which is the entry's
     new tokens (the last one is drafted by nobody), then -1.  An entry without rows accepts 0.  Bit 16 of ``status``: rows or a parent that
     cannot be."""
-    tensors = tokens, targets, entry_starts, parents, path, accepted, emitted, status
-    device = _device_of(*tensors)
+    device = _device_of(tokens, targets, entry_starts, parents, path, accepted, emitted, status)
     if device != _current_device():
         with torch.cuda.device(device):
-            return tree_accept(*tensors)
-    for t in tensors:
-        if t.dtype is not _I32 or not t.is_contiguous():
-            raise KernelError("contiguous int32 tensors")
+            return tree_accept(tokens, targets, entry_starts, parents, path, accepted, emitted, status)
+    # (chains, not loops: this call is short, and what is asked of a tensor here is most of it)
+    if not (tokens.dtype is targets.dtype is entry_starts.dtype is parents.dtype is path.dtype is accepted.dtype is emitted.dtype is status.dtype is _I32
+            and tokens.is_contiguous() and targets.is_contiguous() and entry_starts.is_contiguous() and parents.is_contiguous() and path.is_contiguous()
+            and accepted.is_contiguous() and emitted.is_contiguous()):
+        raise KernelError("contiguous int32 tensors")
     entries, rows, shape = entry_starts.numel() - 1, tokens.numel(), path.shape
     if entries < 0 or targets.numel() != rows or parents.numel() < rows or status.numel() < 1:
         raise KernelError("one target and one parent per token, entry_starts [entries + 1]")
-    if len(shape) != 2 or shape[0] != entries or shape[1] < 1 or emitted.shape != shape or accepted.numel() < entries:
+    if path.dim() != 2 or emitted.shape != shape or accepted.numel() < entries:
+        raise KernelError("path and emitted [entries, P], accepted [entries]")
+    of_path, longest = shape
+    if of_path != entries or longest < 1:
         raise KernelError("path and emitted [entries, P], accepted [entries]")
     _check(library().eg_tree_accept(_stream_of(device), _pack_tree_accept(
         tokens.data_ptr(), targets.data_ptr(), entry_starts.data_ptr(), parents.data_ptr(), path.data_ptr(), accepted.data_ptr(), emitted.data_ptr(), status.data_ptr(),
-        entries, rows, shape[1])), "tree_accept")
+        entries, rows, longest)), "tree_accept")
 
 
 def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, context: torch.Tensor, path: torch.Tensor, accepted: torch.Tensor,
@@ -1042,23 +1046,24 @@ def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, context: torch.Tenso
     if device != _current_device():
         with torch.cuda.device(device):
             return cache_keep(kv, block_table, context, path, accepted, status)
-    for t in (context, path, accepted, status):
-        if t.dtype is not _I32 or not t.is_contiguous():
-            raise KernelError("contiguous int32 context, path, accepted and status")
-    shape, path_shape, table_shape, element_size = kv.shape, path.shape, block_table.shape, kv.element_size()
-    if len(shape) != 6 or shape[2] != 2 or element_size not in (2, 4):
-        raise KernelError("kv [layers, pages, 2, NKV, page_size, HD] of 2 or 4 bytes")
-    layers, pages, _, kv_heads, page_size, head_dim = shape
+    if not (block_table.dtype is context.dtype is path.dtype is accepted.dtype is status.dtype is _I32 and context.is_contiguous() and path.is_contiguous()
+            and accepted.is_contiguous()):
+        raise KernelError("int32 metadata, contiguous context, path and accepted")
+    element_size = kv.element_size()
+    if kv.dim() != 6 or element_size not in (2, 4) or path.dim() != 2 or block_table.dim() != 2:
+        raise KernelError("kv [layers, pages, 2, NKV, page_size, HD] of 2 or 4 bytes, path [entries, P], block table [entries, pages]")
+    layers, pages, planes, kv_heads, page_size, head_dim = kv.shape
     layer_stride, page_stride, plane_stride, head_stride, row_stride, step = kv.stride()
-    if (step != 1 and head_dim > 1) or (row_stride != head_dim and page_size > 1):
-        raise KernelError("kv's pages in whole rows")
-    if len(path_shape) != 2 or path_shape[1] < 1 or accepted.numel() < path_shape[0] or context.numel() < path_shape[0] or status.numel() < 1:
+    if planes != 2 or (step != 1 and head_dim > 1) or (row_stride != head_dim and page_size > 1):
+        raise KernelError("kv [layers, pages, 2, NKV, page_size, HD], pages in whole rows")
+    (entries, longest), (table_entries, table_pages), (table_stride, table_step) = path.shape, block_table.shape, block_table.stride()
+    if longest < 1 or accepted.numel() < entries or context.numel() < entries or status.numel() < 1:
         raise KernelError("path [entries, P], accepted and context [entries]")
-    if block_table.dtype is not _I32 or len(table_shape) != 2 or table_shape[0] < path_shape[0] or (block_table.stride(1) != 1 and table_shape[1] > 1):
-        raise KernelError("an int32 block table [entries, pages]")
+    if table_entries < entries or (table_step != 1 and table_pages > 1):
+        raise KernelError("a block table [entries, pages], rows side by side")
     _check(library().eg_cache_keep(_stream_of(device), _pack_cache_keep(
         kv.data_ptr(), block_table.data_ptr(), context.data_ptr(), path.data_ptr(), accepted.data_ptr(), status.data_ptr(), element_size, layers, pages, kv_heads, page_size,
-        head_dim, layer_stride, page_stride, plane_stride, head_stride, block_table.stride(0), table_shape[1], path_shape[0], path_shape[1])), "cache_keep")
+        head_dim, layer_stride, page_stride, plane_stride, head_stride, table_stride, table_pages, entries, longest)), "cache_keep")
 
 
 def wait_probe(limit: int, threads: int, status: torch.Tensor) -> int:
