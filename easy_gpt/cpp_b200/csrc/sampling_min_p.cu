@@ -28,7 +28,7 @@ typedef unsigned long long u64;
 
 constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = 1024, SHORT = 128, MOST_CTAS = 16, GROUPS = 1024;
 constexpr int LIMBS = 3, LIMB_BITS = 14;                             // of a weight, at most 2^42: sums of 2^17 of them stay below 2^32
-constexpr int SLICE = 20480, MOST_SLICE = 50176;                     // logits of a slice: two CTAs an SM, and what fits at all
+constexpr int SLICE = 20480, MOST_SLICE = 49664;                     // logits of a slice: two CTAs an SM, and what fits at all
 constexpr double ONE = 4398046511104.0;                              // 2^42: with 2^20 tokens sums stay below 2^62
 constexpr int MOST_TOKENS = 1 << 20;
 constexpr float COUNT_RANGE = 32.f, WEIGHT_RANGE = 30.f;             // what a histogram's steps span below the largest logit; of weights in units of T
@@ -88,7 +88,7 @@ struct Shared {
     u64 warp_a[WARPS], warp_b[WARPS];
     u64 list[LIST];
     __align__(16) u64 weights[LIST];                                 // of the list; a histogram's sums over the CTAs, count and weight a step
-    float group_most[GROUPS];
+    float group_most[GROUPS], own_most[THREADS];
     unsigned bin_weight[LIMBS][BINS], bin_count[BINS];
     unsigned listed, gathered, room;
     int found;
@@ -240,19 +240,19 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     };
     u64 all[2], front;
 
-    // ---- the largest logit; with top-k that of groups of 1 to 32 threads too, which every CTA gets
+    // ---- the largest logit; with top-k that of at least 2 k groups of 1 to 512 threads too, which every CTA gets
     const bool k_on = k > 0 && k < vocab, p_on = p > 0.f && p < 1.f, m_on = least > 0.0;
     float most = -INFINITY;                                          // NaN is passed over
     for_all(-INFINITY, [&](float x, int) { most = fmaxf(most, x); });
-    int width = 32;
-    while (width > 1 && (int)ctas * THREADS / width < 2 * min(k, GROUPS)) width /= 2;
-    const int groups = (int)ctas * THREADS / width;
+    int width = THREADS;
+    while (width > 1 && (int)ctas * (THREADS / width) < max(4, 2 * min(k, GROUPS))) width /= 2;
+    const int own_groups = THREADS / width, groups = (int)ctas * own_groups;
     const bool grouped = k_on && groups >= 2 * k && groups <= GROUPS;
-    float group = most;
+    if (width == 1) s.own_most[tid] = most;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        if (2 * o == width) group = most;
+        if (2 * o == width && lane % width == 0) s.own_most[tid / width] = most;
     }
     if (lane == 0) s.floats[warp] = most;
     __syncthreads();
@@ -260,8 +260,14 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
 #pragma unroll
     for (int o = WARPS / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-    if (grouped && tid % width == 0)
-        for (unsigned q = 0; q < ctas; ++q) remote_store(remote(&s.group_most[(rank * THREADS + tid) / width], q), group);
+    if (grouped)
+        for (int i = tid; i < groups; i += THREADS) {                // one of this CTA's groups for one CTA
+            const int group = i / (int)ctas;
+            float value = width <= 32 ? s.own_most[group] : -INFINITY;
+            if (width > 32)
+                for (int w = 0; w < width / 32; ++w) value = fmaxf(value, s.floats[group * (width / 32) + w]);
+            remote_store(remote(&s.group_most[(int)rank * own_groups + group], i % ctas), value);
+        }
     exchange(key_of(most), 0, true, all, front);
     const unsigned top = (unsigned)all[0];
     const float largest = value_of(top);
