@@ -31,8 +31,7 @@ constexpr int LIMBS = 3, LIMB_BITS = 14;                             // of a wei
 constexpr int SLICE = 20480, MOST_SLICE = 49664;                     // logits of a slice: two CTAs an SM, and what fits at all
 constexpr double ONE = 4398046511104.0;                              // 2^42: with 2^20 tokens sums stay below 2^62
 constexpr int MOST_TOKENS = 1 << 20;
-constexpr float COUNT_RANGE = 32.f, WEIGHT_RANGE = 30.f;             // what a histogram's steps span below the largest logit; of weights in units of T
-constexpr int WEIGHTY_STEPS = 500;                                   // whose tokens all have a weight: exp(-30 500 / 512) 2^42 > 0.8
+constexpr float COUNT_RANGE = 32.f, WEIGHT_RANGE = 16.f;             // what a histogram's steps span below the largest logit; of weights in units of T
 constexpr float NO_WEIGHT = 31.f;                                    // exp(-31) 2^42 < 1/4
 
 // larger numbers have larger keys; NaN has key 0
@@ -543,12 +542,10 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
             exchange(block_join<false>(sum, s), 0, false, all, front);
             whole = all[0];
         }
-        // what is far below min-p's border (by more than a float's rounding moves it) needs no weight
+        // everything down to min-p's border and a little further (by more than a float's rounding moves it): the list's own cut is exact
         const float border = m_on ? largest + T * (logf(fminf(min_p[r], 1.f)) - 1e-3f) - 1e-5f * fabsf(largest) : -INFINITY;
         for_all(border, [&](float x, int i) {
-            if (x < border || !(x > -INFINITY)) return;
-            const u64 w = weight(x);
-            if (w > 0 && (double)w >= least) put_in_list(token_of(key_of(x), lo + i));
+            if (!(x < border) && x > -INFINITY) put_in_list(token_of(key_of(x), lo + i));
         });
         if (finish_list(false, whole)) return;
     }
@@ -565,7 +562,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         unsigned low_key = last_step || !(high - 1.f / scale - slack > -INFINITY) ? MINUS_INFINITY_KEY + 1 : key_of(high - 1.f / scale - slack);
         auto is_inside = [&](float x, u64 token) {
             const unsigned key = (unsigned)(token >> 32);
-            return token >= last && key >= low_key && key <= high_key && step_of(x, scale) == cut.step && (!by_weight || cut.step < WEIGHTY_STEPS || weight(x) > 0);
+            return token >= last && key >= low_key && key <= high_key && step_of(x, scale) == cut.step && (!by_weight || !last_step || weight(x) > 0);
         };
         while (inside > LIST) {
             if (high_key == low_key) break;
