@@ -58,7 +58,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     __shared__ int ups[STAGED_NODES];
     __shared__ float row_ml[2 * BM];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_flag, latest, holes;
+    __shared__ int abort_flag, latest, holes, poison;                // poison: values that are not finite have been met, and zeroed
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = blockIdx.x % p.max_parts, kvh = blockIdx.x / p.max_parts % p.num_kv_heads;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_addr = base, k_ring = base + S::Q_BYTES, v_ring = k_ring + STAGES * S::TILE_BYTES;
@@ -109,7 +109,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             mbar_init(&p_full[i], row_warps);
             mbar_init(&o_done[i], 1);
         }
-        abort_flag = latest = holes = 0;
+        abort_flag = latest = holes = poison = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
@@ -241,7 +241,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         const int edge = max(first, latest);
         const float scale_log2 = p.scale * 1.4426950408889634f;
         float m = -INFINITY, l = 0.f;
-        bool ok = true, poison = false;                              // poison: values that are not finite have been met
+        bool ok = true;
         for (int j = 0; j < ntiles; ++j) {
             const int b = j % SCORES, key0 = (begin + j) * KEYS;
             ok = __all_sync(0xffffffffu, mbar_wait(&s_full[b], (j / SCORES) & 1, &abort_flag, p.status));      // the warp stays together
@@ -265,7 +265,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 for (int x = 0; x < 64; ++x)
                     if (!(bits >> x & 1)) s[x] = -INFINITY;
             }
-            // (a hole's values are zeros.  Every warp looks at the whole tile, so that none waits for another: a warp whose wait gave up would not come)
+            // (a hole's values are zeros.  Every warp looks at the whole tile, so that none waits for another: a warp whose wait gave up would not come.  What one
+            // has zeroed another may not meet any more, so the flag is all warps')
             if (key0 + KEYS > e.context || key0 < edge) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % STAGES], (j / STAGES) & 1, &abort_flag, p.status));
                 if (!ok) break;
@@ -278,11 +279,12 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                     for (int x = 0; x < 4; ++x) odd |= (w[x] & 0x7f80u) == 0x7f80u || (w[x] & 0x7f800000u) == 0x7f800000u;
                 }
                 if (__any_sync(0xffffffffu, odd)) {
+                    *(volatile int*)&poison = 1;
+                    __threadfence_block();
                     for (int i = lane; i < S::TILE_BYTES / 2; i += 32) {
                         bf16* const at = reinterpret_cast<bf16*>(values) + i;
                         if (!isfinite(__bfloat162float(*at))) *at = __float2bfloat16_rn(0.f);
                     }
-                    poison = true;
                     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                 }
             }
@@ -342,6 +344,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[(ntiles - 1) % SCORES], ((ntiles - 1) / SCORES) & 1, &abort_flag, p.status));
         tc_fence_after();
         rows_done = ok;
+        const bool poisoned = *(volatile int*)&poison;               // every warp has been through every tile: the last product waited for their weights
         row_scale = parts > 1 ? 1.f : l > 0.f ? 1.f / l : l;         // nothing seen: 0; NaN stays
         row_ml[2 * row] = rows_done ? m : -INFINITY;
         row_ml[2 * row + 1] = rows_done ? l : 0.f;
@@ -356,7 +359,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 float v[32];
 #pragma unroll
                 for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(o[x]);
-                if (poison)                                          // values that are not finite, where they are seen
+                if (poisoned)                                        // values that are not finite, where they are seen
                     for (int j = 0; j < ntiles; ++j) {
                         const int key0 = (begin + j) * KEYS;
                         if (key0 + KEYS <= e.context && key0 >= edge) continue;

@@ -256,6 +256,21 @@ def test_attention_tree_hidden_places_may_hold_anything(heads, bad, dtype):
     assert int(step.status) == 0
 
 
+@pytest.mark.parametrize("parts", [1, 4])
+@pytest.mark.parametrize("row_tile", [0, 128])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (64, 1, 64)])
+def test_attention_tree_every_row_meets_what_is_not_a_number(heads, row_tile, parts):
+    """Values that are not finite, in a tile that reaches into the tree: every row that sees them has them, whichever warps of a CTA the rows are in."""
+    step = Step([*heads, row_tile], [40, 18], [70, 200], *heads, 16, kind="star")
+    step.cache[step.table[0, 70 // 16], 1, :, 70 % 16, :8] = math.inf                 # node 0 of entry 0, every node's ancestor
+    step.cache[step.table[1, 199 // 16], 1, :, 199 % 16, 3] = -math.inf               # entry 1's last cached key
+    for _ in range(20):
+        got = run_plan(step, (row_tile, parts, 1)).view(-1, heads[0], heads[2])
+        assert int(step.status) == 0
+        assert bool((got[:40, :, :8] == math.inf).all()) and bool(torch.isfinite(got[:40, :, 8:]).all())
+        assert bool((got[40:58, :, 3] == -math.inf).all()) and bool(torch.isfinite(got[40:58, :, 4:]).all())
+
+
 def test_attention_tree_window_hides_what_is_not_a_number():
     """Values that some rows' windows have left and others' have not."""
     step = Step(5, [40], [100], 14, 2, 64, 16, kind="chain")
