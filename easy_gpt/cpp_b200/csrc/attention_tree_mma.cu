@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
         const float n0 = fmaxf(m0, t0 * scale_log2), n1 = fmaxf(m1, t1 * scale_log2);
         const float r0 = n0 == -INFINITY ? 0.f : n0, r1 = n1 == -INFINITY ? 0.f : n1;
-        const float c0 = exp2_fast(m0 - r0), c1 = exp2_fast(m1 - r1);
+        // (before the first score there is nothing to scale, but for infinities and NaN of this tile, which 0 would not leave as they are)
+        const float c0 = m0 == -INFINITY ? 1.f : exp2_fast(m0 - r0), c1 = m1 == -INFINITY ? 1.f : exp2_fast(m1 - r1);
         m0 = n0;
         m1 = n1;
         l0 *= c0;

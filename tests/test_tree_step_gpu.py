@@ -257,7 +257,7 @@ def test_attention_tree_hidden_places_may_hold_anything(heads, bad, dtype):
 
 
 @pytest.mark.parametrize("parts", [1, 4])
-@pytest.mark.parametrize("row_tile", [0, 128])
+@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
 @pytest.mark.parametrize("heads", [(14, 2, 64), (28, 4, 128), (64, 1, 64)])
 def test_attention_tree_every_row_meets_what_is_not_a_number(heads, row_tile, parts):
     """Values that are not finite, in a tile that reaches into the tree: every row that sees them has them, whichever warps of a CTA the rows are in."""
