@@ -71,12 +71,12 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
     if (!tree::find_tile(p, blockIdx.x / p.max_parts / p.num_kv_heads, ROWS, r, e, within)) return;
     const int D = p.head_dim, row0 = within * ROWS, count = min(ROWS, e.n * group - row0);
     const int last_node = (row0 + count - 1) / group;
-    const int first = tree::first_key(p, e), end = e.context + last_node + 1;    // the tile's keys: first .. end - 1
+    bool hole;                                                       // a page that is none has been met
+    const int first = tree::first_key(p, e), end = tree::end_key(p, e, first, last_node, hole);      // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
     if (part >= parts) return;
     const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
 
-    bool hole = false;                                               // a page that is none has been met
     auto list_keys = [&](int tile) {                                 // the places of tiles tile .. tile + LISTED - 1
         for (int i = tid; i < LISTED * KEYS; i += THREADS) {
             const int at = tile * KEYS + i, slot = at / p.page_size;

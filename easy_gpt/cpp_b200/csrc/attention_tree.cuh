@@ -41,7 +41,7 @@ struct Entry {
 // Entry r as the metadata has it; n = 0 where its rows cannot be what they say (and a status bit).
 __device__ __forceinline__ Entry sound(const Params& p, int first, int end, int context) {
     Entry e = {first, end - first, context};
-    if (first < 0 || end < first || end > p.rows || context < 0 || context > 0x7fffffff - e.n) {
+    if (first < 0 || end < first || end > p.rows || context < 0 || context > 0x7fffffff - 4096 - e.n) {      // (the kernels look a few tiles ahead)
         atomicOr(p.status, EG_STATUS_BAD_TREE);
         e.n = 0;
     }
@@ -108,6 +108,17 @@ __device__ __forceinline__ bool find_tile(const Params& p, int tile, int row_til
 
 // A tile's first key that any of its rows may see, and the key behind its last one.
 __device__ __forceinline__ int first_key(const Params& p, const Entry& e) { return p.window > 0 && e.context >= p.window ? e.context - p.window + 1 : 0; }
+
+// The key behind a tile's last one.  The block table has no place for keys from table_pages * page_size on: a tile's keys end there (one stays, so that there
+// is something to go through), `beyond` says so, and so does the status.
+__device__ __forceinline__ int end_key(const Params& p, const Entry& e, int first, int last_node, bool& beyond) {
+    const int end = e.context + last_node + 1;
+    const long long room = (long long)p.table_pages * p.page_size;
+    beyond = end > room;
+    if (!beyond) return end;
+    if (threadIdx.x == 0) atomicOr(p.status, EG_STATUS_BAD_PAGE);
+    return max((int)room, first + 1);
+}
 
 __device__ __forceinline__ int parts_of(const Params& p, int key_tiles) { return max(1, min(p.max_parts, key_tiles / p.part_tiles)); }
 

@@ -58,7 +58,8 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
     Entry e;
     if (!tree::find_tile(p, blockIdx.x / p.max_parts / p.num_kv_heads, ROWS, r, e, within)) return;
     const int row0 = within * ROWS, count = min(ROWS, e.n * group - row0), last_node = (row0 + count - 1) / group;
-    const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
+    bool holes;                                                      // a page that is none has been met
+    const int first = tree::first_key(p, e), end = tree::end_key(p, e, first, last_node, holes);     // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
     if (part >= parts) return;
     const int begin = tile0 + (int)((long long)tiles * part / parts), stop = tile0 + (int)((long long)tiles * (part + 1) / parts);
@@ -79,7 +80,6 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
             page[i] = needed && slot < p.table_pages ? __ldg(table + slot) : -1;
         }
     };
-    bool holes = false;                                              // a page that is none has been met
     auto load = [&](int tile, const int (&page)[LOOKUPS]) {
         unsigned char* const ks = ring + (tile - begin) % STAGES * L::STAGE_BYTES;
 #pragma unroll

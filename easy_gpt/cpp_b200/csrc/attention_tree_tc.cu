@@ -69,7 +69,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     Entry e;
     if (!tree::find_tile(p, blockIdx.x / p.max_parts / p.num_kv_heads, maps.nodes * group, r, e, within)) return;
     const int node0 = within * maps.nodes, nodes = min(maps.nodes, e.n - node0), count = nodes * group, last_node = node0 + nodes - 1;
-    const int first = tree::first_key(p, e), end = e.context + last_node + 1;     // the tile's keys: first .. end - 1
+    bool beyond;
+    const int first = tree::first_key(p, e), end = tree::end_key(p, e, first, last_node, beyond);    // the tile's keys: first .. end - 1
     const int tile0 = first / KEYS, tiles = (end - 1) / KEYS - tile0 + 1, parts = tree::parts_of(p, tiles);
     if (part >= parts) return;
     const int begin = tile0 + (int)((long long)tiles * part / parts), ntiles = tile0 + (int)((long long)tiles * (part + 1) / parts) - begin;
@@ -109,7 +110,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             mbar_init(&p_full[i], row_warps);
             mbar_init(&o_done[i], 1);
         }
-        abort_flag = latest = holes = poison = 0;
+        abort_flag = latest = poison = 0;
+        holes = beyond;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {

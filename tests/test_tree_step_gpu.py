@@ -361,6 +361,38 @@ def test_attention_tree_keys_beyond_the_block_table():
     assert float(off.max()) < 1
 
 
+@pytest.mark.parametrize("window", [None, 40])
+@pytest.mark.parametrize("parts", [1, 4])
+@pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
+def test_attention_tree_contexts_far_beyond_the_block_table(row_tile, parts, window):
+    """What no table has room for takes no time: the keys that there are places for are seen, behind a window none, the other entry as ever."""
+    step = Step([row_tile, parts], [6, 10], [40, 50], 14, 2, 64, 16)
+    table_keys = step.block_table.shape[1] * 16
+    want = step.plain(window)
+    for context in (1 << 20, (1 << 31) - 1 - 4096 - 6):
+        step.context[0] = context
+        step.status.zero_()
+        step.out.fill_(7.0)
+        got = run_plan(step, (row_tile, parts, 1), window).double()
+        assert int(step.status) == 2
+        assert float(((got[6:16] - want[6:16]).norm(dim=1) / want[6:16].norm(dim=1)).max()) <= tolerance(step.dtype, 64)
+        if window:
+            assert not bool(got[:6].any())
+        else:
+            step.contexts[0], nodes, step.nodes[0] = int((step.table[0] >= 0).sum()) * 16, step.nodes[0], 0
+            k, v = step.rows_of(0, 0), step.rows_of(0, 1)
+            step.contexts[0], step.nodes[0] = 40, nodes
+            q = step.q[:6].double().view(6, 2, 7, 64)
+            w = (torch.einsum("nghd,gkd->nghk", q, k[:, :table_keys]) * 0.125).softmax(-1)
+            sure = torch.einsum("nghk,gkd->nghd", w, v[:, :table_keys]).reshape(6, -1)
+            assert float(((got[:6] - sure).norm(dim=1) / sure.norm(dim=1)).max()) <= tolerance(step.dtype, 64)
+    step.context[0] = (1 << 31) - 1 - 4096 - 5                          # of this one nothing can be
+    step.status.zero_()
+    step.out.fill_(7.0)
+    got = run_plan(step, (row_tile, parts, 1), window)
+    assert int(step.status) == 16 and bool((got[:6] == 7).all())
+
+
 def test_attention_tree_replayed_and_on_another_stream():
     """A captured call, replayed with other trees, contexts and values, while an eager one runs on another stream."""
     a, b = Step(21, [12, 30], [3000, 700], 14, 2, 64, 64), Step(22, [12, 30], [2999, 705], 14, 2, 64, 64)
