@@ -1,12 +1,16 @@
 // Attention over drafted trees and the paged cache (attention_tree.cuh says which keys a row sees) in 32-bit arithmetic, for float32 and
 // bfloat16, any head size up to 256, any page size and alignment.
 //
-// A CTA takes 64 rows (node, query head) of an entry and KV head and a part of the keys, 32 at a time, in shared memory as float32; 256
-// threads have 4 rows x 2 keys of the scores and 4 rows x (head size / 16) columns of the output each.  Sums, reference and exponents are
-// 32-bit, the reference is the running maximum.  Where rows of float32 are whole 16-byte pieces, the next tile comes by
-// asynchronous copies while this one is worked on; else a tile is read and converted when it is its turn.  Bound by shared memory: a 16-byte read of
-// a warp takes four cycles whatever its lanes share, 9,200 cycles a tile (5 us) where the multiply-adds take 4,100; thread tiles of 8 x 8 would
-// halve that and leave a CTA two warps.  (Four requests of up to 1,000 keys, 12 heads of 128: 34 us, of which 15 are the start and the adding up.)
+// A CTA takes 32 or 64 rows (node, query head) of an entry and KV head, eight a warp, and a part of the keys, 32 at a time, in shared memory as
+// float32.  A lane has 8 rows x 4 keys of the scores in a fourth of the head's quads, whose sums the warp then joins, so that a lane has the softmax of
+// two rows; and 8 rows x 8 columns of the output from its share of the tile's keys.  Sums, reference and exponents are 32-bit, the reference is the
+// running maximum.  Where rows of float32 are whole 16-byte pieces, the next tile comes by asynchronous copies while this one is worked on; else a tile is
+// read and converted when it is its turn.
+//
+// A 16-byte read of a warp takes shared memory four cycles whatever its lanes share: 2,600 cycles for a tile of 32 rows and heads of 128, beside 2,100 of
+// multiply-adds, and two CTAs an SM come to 3,300 (tiles of 4 rows x 2 keys a lane: 9,200 for 64 rows).  What the rest waits for is the latency of those
+// reads: 240 registers a lane leave four warps a CTA.  32 requests of 32 nodes and 2,000 keys, 12 heads of 128: 430 us, 29 TFLOP/s (685 with 4 x 2); 4 of up
+// to 13 nodes and 1,000 keys 25, of which 9 are the start and the adding up.
 //
 // Which keys a row sees is decided by a select, never by adding: a hidden score may be anything.  A hidden value takes part as 0 * v; where
 // there are values that are not finite, every row leaves out those that it does not see.
@@ -18,7 +22,9 @@ namespace {
 using tree::Entry;
 using tree::Params;
 
-constexpr int ROWS = 64, KEYS = 32, THREADS = 256, STAGED_NODES = 1024;
+constexpr int KEYS = 32, STAGED_NODES = 1024;
+// Rows of a CTA, eight a warp.  Two CTAs of 32 share an SM where tiles come by asynchronous copies; else, and where two do not fit, one of 64.
+constexpr int rows_of(int dim, bool async) { return async && dim <= 128 ? 32 : 64; }
 constexpr int LISTED = 16;                                           // key tiles whose places in the cache are looked up at a time
 
 // two float32 in 64 bits, for the packed instructions
@@ -41,19 +47,27 @@ __device__ __forceinline__ u64 mul_pair(u64 a, u64 b) {
     return d;
 }
 
-template <int DMAX>
+__device__ __forceinline__ u64 add_pair(u64 a, u64 b) {
+    u64 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+template <int DMAX, bool ASYNC>
 struct Layout {
+    static constexpr int ROWS = rows_of(DMAX, ASYNC), THREADS = 4 * ROWS;
     static constexpr int LD = DMAX + 4;                              // floats of a row: eight rows' quads meet no bank twice
-    static constexpr int P_LD = KEYS + 4;
+    static constexpr int P_LD = ROWS + 4;                            // weights, a line a key
     static constexpr int STAGE = 2 * KEYS * LD;                      // keys, then values
-    static constexpr int FLOATS = ROWS * LD + 2 * STAGE + ROWS * P_LD;
+    static constexpr int FLOATS = ROWS * LD + 2 * STAGE + KEYS * P_LD;
 };
 
 // ASYNC: float32 in whole 16-byte pieces, two stages of keys and values.
 template <typename T, int DMAX, bool ASYNC>
-__global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_kernel(const Params p) {
-    using L = Layout<DMAX>;
-    constexpr int COLS = DMAX / 64;                                  // quads of output columns a thread has
+__global__ void __launch_bounds__(Layout<DMAX, ASYNC>::THREADS, Layout<DMAX, ASYNC>::ROWS == 32 ? 2 : 1) attention_tree_kernel(const Params p) {
+    using L = Layout<DMAX, ASYNC>;
+    constexpr int ROWS = L::ROWS, THREADS = L::THREADS;
+    constexpr int QUADS = 2, LANES = DMAX / (4 * QUADS), SPLIT = 32 / LANES;       // of the output: lanes with these many quads of columns, and shares of a tile's keys
     extern __shared__ __align__(16) float smem[];
     float* const q_s = smem;
     float* const ring = q_s + ROWS * L::LD;
@@ -163,17 +177,17 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
         }
         lowest[tid] = low;
     }
-    const int tx = tid & 15, ty = tid >> 4;                          // keys tx, tx + 16; rows 4 ty ..; columns 4 tx + 64 c ..
+    // A warp has 8 rows.  Of their scores a lane has those with 4 keys, key_of + 8 j, in every fourth quad of the head; of their output 8 columns from a
+    // share of the keys.
+    const int lane = tid & 31, row_of = tid / 32 * 8, key_of = lane & 7, quarter = lane >> 3, share = lane / LANES, column = lane % LANES * 4;
+    const int mine = row_of + 2 * quarter;                           // the two rows whose softmax a lane has
     const float scale_log2 = p.scale * 1.4426950408889634f;
-    float m[4], l[4];
-    u64 acc[4][COLS][2];                                             // pairs of columns
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};          // l: of the lane's keys
+    u64 acc[8][QUADS][2];                                            // pairs of columns: column .. column + 3, and those DMAX / 2 on
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        m[i] = -INFINITY;
-        l[i] = 0.f;
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) acc[i][c][0] = acc[i][c][1] = 0;
-    }
+        for (int h = 0; h < QUADS; ++h) acc[i][h][0] = acc[i][h][1] = 0;
     for (int tile = begin; tile < stop; ++tile) {
         const int key0 = tile * KEYS;
         if constexpr (ASYNC) {
@@ -199,8 +213,9 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
         const float* const k_s = stage_of(tile);
         const float* const v_s = k_s + KEYS * L::LD;
         // ---- a tile that reaches into the tree, over a window's edge or onto a page that is none (of this run of tiles): which keys a row sees
-        bool masked = key0 + KEYS > e.context || key0 < max(first, latest), odd = false;
-        masked = __syncthreads_or(masked || hole);
+        const bool checked = __syncthreads_or(hole);                 // the same for all threads: pages are looked at again
+        const bool masked = key0 + KEYS > e.context || key0 < max(first, latest) || checked;
+        bool odd = false;
         if (masked) {
             if (tid < ROWS) {
                 unsigned bits = 0;
@@ -210,121 +225,149 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
                     int left = p.window > 0 ? p.window : 0x7fffffff;
                     for (int i = (row0 + tid) / group; i >= 0 && e.context + i >= key0 && left > 0; i = up_of(i), --left)
                         if (e.context + i < key0 + KEYS) bits |= 1u << (e.context + i - key0);
-                    for (int key = 0; key < KEYS; ++key) {           // on pages that are there
+                    for (int key = 0; checked && key < KEYS; ++key) {      // on pages that are there
                         const int slot = (key0 + key) / p.page_size, page = slot < p.table_pages ? p.block_table[(size_t)r * p.table_stride + slot] : -1;
                         if ((bits >> key & 1) && (page < 0 || page >= p.num_pages)) bits &= ~(1u << key);
                     }
                 }
                 seen[tid] = bits;
             }
-            for (int i = tid; i < KEYS * DMAX; i += THREADS) odd |= !isfinite(v_s[i / DMAX * L::LD + i % DMAX]);
+            for (int i = tid; i < KEYS * DMAX / 4; i += THREADS) {
+                const float4 v = *reinterpret_cast<const float4*>(v_s + i / (DMAX / 4) * L::LD + i % (DMAX / 4) * 4);
+                odd |= !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
+            }
             odd = __syncthreads_or(odd);
         }
+        if (row_of >= count) continue;                               // a warp whose rows are all filling
         // ---- scores
         // (multiply-adds on pairs: of neighbouring terms here, of neighbouring columns below; half the instructions)
-        float s[4][2];
+        float s[2][4];
         {
-            u64 sums[4][2] = {};
-#pragma unroll 8
-            for (int d = 0; d < DMAX; d += 4) {
-                ulonglong2 a[4], b[2];
+            u64 sums[8][4] = {};
+#pragma unroll 2
+            for (int d = 4 * quarter; d < DMAX; d += 16) {
+                ulonglong2 b[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const ulonglong2*>(q_s + (4 * ty + i) * L::LD + d);
+                for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(k_s + (key_of + 8 * j) * L::LD + d);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) b[j] = *reinterpret_cast<const ulonglong2*>(k_s + (tx + 16 * j) * L::LD + d);
+                for (int i = 0; i < 8; ++i) {
+                    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(q_s + (row_of + i) * L::LD + d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) sums[i][j] = fma_pair(a[i].y, b[j].y, fma_pair(a[i].x, b[j].x, sums[i][j]));
+                    for (int j = 0; j < 4; ++j) sums[i][j] = fma_pair(a.y, b[j].y, fma_pair(a.x, b[j].x, sums[i][j]));
+                }
             }
+            // the quarters' sums: a lane keeps half of the rows and gives the other half away, twice
+            float half[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) s[i][j] = low_of(sums[i][j]) + high_of(sums[i][j]);
-        }
+                for (int j = 0; j < 4; ++j) {
+                    const float low = low_of(sums[i][j]) + high_of(sums[i][j]), high = low_of(sums[4 + i][j]) + high_of(sums[4 + i][j]);
+                    half[i][j] = (quarter & 2 ? high : low) + __shfl_xor_sync(0xffffffffu, quarter & 2 ? low : high, 16);
+                }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned bits = masked ? seen[4 * ty + i] : ~0u;
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    s[i][j] = (quarter & 1 ? half[2 + i][j] : half[i][j]) + __shfl_xor_sync(0xffffffffu, quarter & 1 ? half[i][j] : half[2 + i][j], 8);
+        }
+        float keep[2];
+        float2 weights[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const unsigned bits = (masked ? seen[mine + i] : ~0u) >> key_of;
             float top = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                s[i][j] = bits >> (tx + 16 * j) & 1 ? s[i][j] * scale_log2 : -INFINITY;
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = bits >> (8 * j) & 1 ? s[i][j] * scale_log2 : -INFINITY;
                 top = fmaxf(top, s[i][j]);
             }
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const float now = fmaxf(m[i], top), ref = now == -INFINITY ? 0.f : now;     // a row that has seen nothing: every weight 0
-            const float keep = exp2f(m[i] - ref);
+            keep[i] = exp2f(m[i] - ref);
+            m[i] = now;
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const float w = exp2f(s[i][j] - ref);
-                p_s[(4 * ty + i) * L::P_LD + tx + 16 * j] = w;
+                (i ? weights[j].y : weights[j].x) = w;
                 sum += w;
             }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l[i] = l[i] * keep + sum;
-            m[i] = now;
-            const u64 both = pair_of(keep, keep);
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) acc[i][c][0] = mul_pair(acc[i][c][0], both), acc[i][c][1] = mul_pair(acc[i][c][1], both);
+            l[i] = l[i] * keep[i] + sum;
         }
-        __syncwarp();                                                // a row's weights come from its own half warp
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(p_s + (key_of + 8 * j) * L::P_LD + mine) = weights[j];
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float c = __shfl_sync(0xffffffffu, keep[i & 1], i / 2 * 8);
+                const u64 both = pair_of(c, c);
+#pragma unroll
+                for (int h = 0; h < QUADS; ++h) acc[i][h][0] = mul_pair(acc[i][h][0], both), acc[i][h][1] = mul_pair(acc[i][h][1], both);
+            }
+        }
+        __syncwarp();                                                // a row's weights come from its own warp
         // ---- output
+        const int from = share * (KEYS / SPLIT);
         if (!odd) {
 #pragma unroll 2
-            for (int key = 0; key < KEYS; key += 4) {
-                float4 w[4];
+            for (int key = from; key < from + KEYS / SPLIT; ++key) {
+                const float4 w0 = *reinterpret_cast<const float4*>(p_s + key * L::P_LD + row_of), w1 = *reinterpret_cast<const float4*>(p_s + key * L::P_LD + row_of + 4);
+                ulonglong2 v[QUADS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const float4*>(p_s + (4 * ty + i) * L::P_LD + key);
+                for (int h = 0; h < QUADS; ++h) v[h] = *reinterpret_cast<const ulonglong2*>(v_s + key * L::LD + h * (DMAX / 2) + column);
+                const float each[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-                for (int c = 0; c < COLS; ++c) {
-                    ulonglong2 v[4];
+                for (int i = 0; i < 8; ++i) {
+                    const u64 both = pair_of(each[i], each[i]);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) v[x] = *reinterpret_cast<const ulonglong2*>(v_s + (key + x) * L::LD + 4 * tx + 64 * c);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float each[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const u64 both = pair_of(each[x], each[x]);
-                            acc[i][c][0] = fma_pair(both, v[x].x, acc[i][c][0]);
-                            acc[i][c][1] = fma_pair(both, v[x].y, acc[i][c][1]);
-                        }
-                    }
+                    for (int h = 0; h < QUADS; ++h) acc[i][h][0] = fma_pair(both, v[h].x, acc[i][h][0]), acc[i][h][1] = fma_pair(both, v[h].y, acc[i][h][1]);
                 }
             }
         } else {
-            for (int key = 0; key < KEYS; ++key)
+            for (int key = from; key < from + KEYS / SPLIT; ++key) {
+                ulonglong2 v[QUADS];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!(seen[4 * ty + i] >> key & 1)) continue;
-                    const float w = p_s[(4 * ty + i) * L::P_LD + key];
+                for (int h = 0; h < QUADS; ++h) v[h] = *reinterpret_cast<const ulonglong2*>(v_s + key * L::LD + h * (DMAX / 2) + column);
 #pragma unroll
-                    for (int c = 0; c < COLS; ++c) {
-                        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(v_s + key * L::LD + 4 * tx + 64 * c);
-                        acc[i][c][0] = fma_pair(pair_of(w, w), v.x, acc[i][c][0]);
-                        acc[i][c][1] = fma_pair(pair_of(w, w), v.y, acc[i][c][1]);
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    if (!(seen[row_of + i] >> key & 1)) continue;
+                    const float w = p_s[key * L::P_LD + row_of + i];
+                    const u64 both = pair_of(w, w);
+#pragma unroll
+                    for (int h = 0; h < QUADS; ++h) acc[i][h][0] = fma_pair(both, v[h].x, acc[i][h][0]), acc[i][h][1] = fma_pair(both, v[h].y, acc[i][h][1]);
                 }
+            }
         }
     }
+    // ---- a row's sum over its lanes, its output over the shares of the keys
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
+#pragma unroll
+    for (int o = LANES; o < 32; o *= 2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int x = 0; x < 2 * QUADS; ++x) acc[i][x / 2][x % 2] = add_pair(acc[i][x / 2][x % 2], __shfl_xor_sync(0xffffffffu, acc[i][x / 2][x % 2], o));
     // where a row's results go
     auto line_of = [&](int row) {
         return static_cast<T*>(p.out) + (size_t)(e.first + (row0 + row) / group) * p.ldo + (size_t)(kvh * group + (row0 + row) % group) * D;
     };
     if (parts == 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (4 * ty + i >= count) continue;
-            T* const line = line_of(4 * ty + i);
-            const float inv = l[i] > 0.f ? 1.f / l[i] : l[i];
+        for (int i = 0; i < 8; ++i) {
+            const float sum = __shfl_sync(0xffffffffu, l[i & 1], i / 2 * 8), inv = sum > 0.f ? 1.f / sum : sum;
+            if (i % SPLIT != share || row_of + i >= count) continue;
+            T* const line = line_of(row_of + i);
 #pragma unroll
-            for (int c = 0; c < COLS; ++c)
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    if (4 * tx + 64 * c + x < D) line[4 * tx + 64 * c + x] = from_f32<T>((x & 1 ? high_of(acc[i][c][x / 2]) : low_of(acc[i][c][x / 2])) * inv);
+            for (int x = 0; x < 4 * QUADS; ++x) {
+                const u64 pair = acc[i][x / 4][x / 2 % 2];
+                const int d = x / 4 * (DMAX / 2) + column + x % 4;
+                if (d < D) line[d] = from_f32<T>((x & 1 ? high_of(pair) : low_of(pair)) * inv);
+            }
         }
         return;
     }
@@ -332,11 +375,15 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
     float* const o_s = q_s;
     float* const ml_s = ring;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
+        if (i % SPLIT != share) continue;
 #pragma unroll
-        for (int c = 0; c < COLS; ++c)
-            *reinterpret_cast<ulonglong2*>(o_s + (4 * ty + i) * L::LD + 4 * tx + 64 * c) = make_ulonglong2(acc[i][c][0], acc[i][c][1]);
-        if (tx == 0) *reinterpret_cast<float2*>(ml_s + 2 * (4 * ty + i)) = make_float2(m[i], l[i]);
+        for (int h = 0; h < QUADS; ++h)
+            *reinterpret_cast<ulonglong2*>(o_s + (row_of + i) * L::LD + h * (DMAX / 2) + column) = make_ulonglong2(acc[i][h][0], acc[i][h][1]);
+    }
+    if (key_of == 0) {
+        *reinterpret_cast<float2*>(ml_s + 2 * mine) = make_float2(m[0], l[0]);
+        *reinterpret_cast<float2*>(ml_s + 2 * mine + 2) = make_float2(m[1], l[1]);
     }
     tree::add_parts<THREADS>(o_s, L::LD, ml_s, count, DMAX, parts, [&](int row, int d, float4 v) {
         T* const line = line_of(row);
@@ -349,10 +396,11 @@ __global__ void __launch_bounds__(THREADS, DMAX <= 128 ? 2 : 1) attention_tree_k
 
 template <typename T, int DMAX, bool ASYNC>
 int launch(cudaStream_t stream, const Params& p, long long tiles) {
-    constexpr int bytes = Layout<DMAX>::FLOATS * 4;
+    using L = Layout<DMAX, ASYNC>;
+    constexpr int bytes = L::FLOATS * 4;
     static unsigned long long seen = 0;
     if (const int code = tree::prepare_kernel(attention_tree_kernel<T, DMAX, ASYNC>, bytes, seen)) return code;
-    return tree::launch_clusters(attention_tree_kernel<T, DMAX, ASYNC>, p.max_parts, p.num_kv_heads, tiles, THREADS, bytes, stream, p);
+    return tree::launch_clusters(attention_tree_kernel<T, DMAX, ASYNC>, p.max_parts, p.num_kv_heads, tiles, L::THREADS, bytes, stream, p);
 }
 template <typename T, bool ASYNC>
 int launch_any(cudaStream_t stream, const Params& p, long long tiles) {
@@ -370,7 +418,8 @@ int launch_any(cudaStream_t stream, const Params& p, long long tiles) {
 // 64 requests of 16 nodes at 700 keys 46 against 21).  Parts: as many as keep one CTA an SM with three key tiles a part, or two CTAs with eight;
 // more of them cost more than they save (32 requests of 9 nodes at 1,000 keys in 1, 2, 4 and 8 parts 18.7, 16.2, 14.6 and 23.8 us; 64 requests of 16 at 700
 // in 1, 2 and 4 parts 21, 25 and 36), and clusters of 16 find little room.  Long contexts are cut into four in any case, for an even end (16 requests of up
-// to 32,768 keys, wide trees, in 1, 2, 4 and 8 parts 563, 460, 399 and 428).
+// to 32,768 keys, wide trees, in 1, 2, 4 and 8 parts 556, 375, 360 and 412).  The 32-bit kernel's CTAs of 32 rows go two to an SM from the first (4
+// requests of 13 nodes at 1,000 keys, 12 heads on 2, in 4, 8 and 16 parts 31, 24 and 33; one node at 4,000, 12 on 12, in 8 and 16 46 and 29).
 EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count,
                                   int* plan) {
     if (rows < 1 || entries < 1 || num_kv_heads < 1 || num_heads % num_kv_heads || num_heads < 1 || page_size < 1 || sm_count < 1 || !plan) return (int)cudaErrorInvalidValue;
@@ -378,15 +427,17 @@ EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries,
     const long long lines = ((long long)rows * group + entries - 1) / entries;      // of an entry, on the average
     const long long key_tiles = ((long long)max_context + 63) / 64;
     const bool tiled = dtype == EG_BF16 && aligned && page_size % 16 == 0 && head_dim % 8 == 0;
+    const bool pieces = dtype == EG_F32 && aligned;                  // the 32-bit kernel's asynchronous copies
     const bool wide = tiled && aligned > 1 && (head_dim == 64 || head_dim == 128) && group <= 128;
     const auto units_of = [&](long long tile) { return entries * ((lines + tile - 1) / tile) * num_kv_heads; };
     int row_tile = !tiled ? 0 : lines <= 16 ? 16 : lines <= 32 ? 32 : 64;
     if (wide && (key_tiles > 16 || units_of(64) * 8 > sm_count)) row_tile = 128;
     else if (tiled && units_of(16) * 8 <= sm_count) row_tile = 16;
-    const long long units = units_of(row_tile == 128 ? 128 / group * group : row_tile ? row_tile : ROWS);
-    const int most = head_dim > 128 ? 8 : row_tile == 0 || row_tile == 128 ? 8 : 16;
+    const long long units = units_of(row_tile == 128 ? 128 / group * group : row_tile ? row_tile : rows_of(head_dim, pieces));
+    const bool pairs = row_tile == 0 && rows_of(head_dim, pieces) == 32;             // two CTAs an SM from the first
+    const int most = head_dim > 128 || row_tile == 128 || (row_tile == 0 && !pairs) ? 8 : 16;
     int parts = 1;
-    while (parts < most && ((units * parts * 2 <= sm_count && key_tiles >= parts * (row_tile == 128 ? 6 : 2)) || (units * parts * 2 <= 2ll * sm_count && key_tiles >= parts * 16))) parts *= 2;
+    while (parts < most && ((units * parts * 2 <= (pairs ? 2ll : 1ll) * sm_count && key_tiles >= parts * (row_tile == 128 ? 6 : pairs && parts == 8 ? 4 : 2)) || (units * parts * 2 <= 2ll * sm_count && key_tiles >= parts * 16))) parts *= 2;
     while (parts < 4 && key_tiles > parts * 64) parts *= 2;
     plan[0] = row_tile;
     plan[1] = parts;
@@ -409,7 +460,8 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
     // what the tensor-core kernels ask of addresses and strides
     const long long rows_at = (long long)((uintptr_t)a.q | (uintptr_t)a.out) | (a.ldq | a.ldo) * 2;
     const bool tiled = a.dtype == EG_BF16 && (((uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.page_stride | a.head_stride) & 7) == 0 && rows_at % 4 == 0;
-    const int aligned = !tiled ? 0 : rows_at % 16 || a.page_stride % dim || a.head_stride % dim || a.page_stride <= 0 || a.head_stride <= 0 ? 1 : 2;
+    const bool pieces = a.dtype == EG_F32 && (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.ldq | a.page_stride | a.head_stride | a.head_dim) & 3) == 0;
+    const int aligned = !tiled ? pieces : rows_at % 16 || a.page_stride % dim || a.head_stride % dim || a.page_stride <= 0 || a.head_stride <= 0 ? 1 : 2;
     int plan[3] = {(int)a.row_tile, (int)a.max_parts, (int)a.part_tiles};
     if (a.row_tile < 0) {
         // a window's worth of keys and the nodes, where that is less
@@ -424,7 +476,7 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
     const int row_tile = plan[0];
     if (row_tile && (!tiled || dim % 8 || a.page_size % 16)) return (int)cudaErrorInvalidValue;
     if (row_tile == 128 && (aligned < 2 || (dim != 64 && dim != 128) || group > 128)) return (int)cudaErrorInvalidValue;
-    const int tile_rows = row_tile ? row_tile : ROWS, tile_keys = row_tile ? 64 : KEYS;
+    const int tile_rows = row_tile ? row_tile : rows_of(dim, pieces), tile_keys = row_tile ? 64 : KEYS;
     const long long tiles = a.rows * group / tile_rows + a.entries;   // at most: every entry's last tile may be a short one
     const Params p = {a.q, a.ldq, a.k_cache, a.v_cache, a.page_stride, a.head_stride, a.block_table, (int)a.table_stride, (int)a.table_pages, (int)a.num_pages,
                       a.entry_starts, a.context, a.parents, a.out, a.ldo, (int)a.rows, (int)a.entries, (int)a.num_heads, (int)a.num_kv_heads, dim, (int)a.page_size,
@@ -432,6 +484,5 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
     if (row_tile == 128) return tree::launch_tc(stream, p);
     if (row_tile) return tree::launch_mma(stream, p, row_tile, tiles);
     if (a.dtype == EG_BF16) return launch_any<bf16, false>(stream, p, tiles);
-    const bool pieces = (((uintptr_t)a.q | (uintptr_t)a.k_cache | (uintptr_t)a.v_cache) & 15) == 0 && ((a.ldq | a.page_stride | a.head_stride | a.head_dim) & 3) == 0;
     return pieces ? launch_any<float, true>(stream, p, tiles) : launch_any<float, false>(stream, p, tiles);
 }
