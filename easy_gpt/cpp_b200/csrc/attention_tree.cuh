@@ -122,6 +122,13 @@ __device__ __forceinline__ int end_key(const Params& p, const Entry& e, int firs
 
 __device__ __forceinline__ int parts_of(const Params& p, int key_tiles) { return max(1, min(p.max_parts, key_tiles / p.part_tiles)); }
 
+// Whether there are infinities or NaN among bfloat16: the largest magnitudes in the upper and the lower halves of words, and what those say.
+__device__ __forceinline__ unsigned largest_halves(unsigned largest, uint4 v) {
+    largest = __vmaxu2(largest, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu));
+    return __vmaxu2(largest, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+}
+__device__ __forceinline__ bool not_finite(unsigned largest) { return (largest & 0xffffu) >= 0x7f80u || largest >> 16 >= 0x7f80u; }
+
 // The kernel in attention_tree_mma.cu (16, 32 or 64 rows a CTA, key tiles of 64).  Its caller has checked what it takes.
 int launch_mma(cudaStream_t stream, const Params& p, int row_tile, long long tiles);
 // The kernel in attention_tree_tc.cu (128 rows a CTA, or as many as whole nodes have; key tiles of 64).  Its caller has checked what it takes, but for the

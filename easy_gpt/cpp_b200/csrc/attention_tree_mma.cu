@@ -188,14 +188,10 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
                 seen[tid] = bits;
             }
             // values that are not finite: they are added where they are seen, and zeros take part in the product
-            bool odd = false;
-            for (int i = tid; i < KEYS * L::CHUNKS; i += THREADS) {
-                const uint4 v = *reinterpret_cast<const uint4*>(vs + i * 16);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int x = 0; x < 4; ++x) odd |= (w[x] & 0x7f80u) == 0x7f80u || (w[x] & 0x7f800000u) == 0x7f800000u;
-            }
-            if (__syncthreads_or(odd)) {
+            unsigned largest = 0;
+#pragma unroll 4
+            for (int i = tid; i < KEYS * L::CHUNKS; i += THREADS) largest = tree::largest_halves(largest, *reinterpret_cast<const uint4*>(vs + i * 16));
+            if (__syncthreads_or(tree::not_finite(largest))) {
                 for (int key = wk * KW; key < (wk + 1) * KW; ++key) {
                     const bool a = seen[wr * 16 + gid] >> key & 1, b = seen[wr * 16 + gid + 8] >> key & 1;
 #pragma unroll

@@ -273,14 +273,15 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 ok = __all_sync(0xffffffffu, mbar_wait(&v_full[j % STAGES], (j / STAGES) & 1, &abort_flag, p.status));
                 if (!ok) break;
                 unsigned char* const values = aligned + S::Q_BYTES + (STAGES + j % STAGES) * S::TILE_BYTES;
-                bool odd = false;
-                for (int i = lane; i < S::TILE_BYTES / 16; i += 32) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(values + i * 16);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                // the keys that not every row sees: below the edge, in the tree
+                const int from = key0 < edge ? 0 : max(0, e.context - key0), to = key0 + KEYS > e.context ? KEYS : min(KEYS, edge - key0);
+                uint32_t largest = 0;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) odd |= (w[x] & 0x7f80u) == 0x7f80u || (w[x] & 0x7f800000u) == 0x7f800000u;
-                }
-                if (__any_sync(0xffffffffu, odd)) {
+                for (int sub_tile = 0; sub_tile < S::SUBS; ++sub_tile)
+#pragma unroll 4
+                    for (int i = from * 8 + lane; i < to * 8; i += 32)
+                        largest = tree::largest_halves(largest, *reinterpret_cast<const uint4*>(values + sub_tile * S::SUB_BYTES + i * 16));
+                if (__any_sync(0xffffffffu, tree::not_finite(largest))) {
                     *(volatile int*)&poison = 1;
                     __threadfence_block();
                     for (int i = lane; i < S::TILE_BYTES / 2; i += 32) {
