@@ -20,6 +20,10 @@
 // are a short list (or all equal); then every CTA sums what is kept of its slice, and the one in whose part the draw falls finds it.
 //
 // (A histogram's weights are three sums of 14 bits each: shared-memory atomics on 64 bits are loops of compare-and-swap, 5 to 18 times slower.)
+//
+// Measured, one row and 192 rows of 151,936 (0.6 MB and 117 MB), us: greedy 5.1 and 50, top-k 20 7.3 and 64, min-p 0.05 7.2 and 63, nothing cut 9.6 and 112,
+// top-p 0.95 alone over flat logits 28 and 310.  One row is bound by latency: the load 1.6, an exchange over the cluster 1 each.  Many rows are 296 CTAs at a
+// time, 8 us each when greedy, of which the load is half; flat rows are bound by weights in 64 bits (0.65 cycles a token and SM a pass) and histograms.
 #include "common.cuh"
 
 namespace {
@@ -133,7 +137,7 @@ __device__ __forceinline__ void block_scan(u64& a, u64& b, Shared& s) {
 }
 
 // Descending, n a power of two up to 2 THREADS.  A thread has two neighbours in registers; their partners up to 32 places away are in its warp, the others
-// come through shared memory.  (All stages there: 5 us for 1,024.)
+// come through shared memory.  (A row of 151,936 with top-k 500, two sorts: 17 us, 20 with all stages there.)
 __device__ __forceinline__ void sort_descending(u64* list, int n) {
     const int t = threadIdx.x;
     const bool mine = t < n / 2;
@@ -307,8 +311,8 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     };
     const float weighty = largest < INFINITY ? largest - NO_WEIGHT * T * 1.0001f - 1e-5f * fabsf(largest) : largest;      // nothing below it has a weight
 
-    // ---- the short list, in the first CTA: every CTA gathers its own tokens and finds room for all of them at once (a remote atomic a token had 600
-    // tokens take 11 us)
+    // ---- the short list, in the first CTA: every CTA gathers its own tokens and finds room for all of them at once (192 rows of 151,936 with top-k 500: 113 us,
+    // 117 with a remote atomic a token)
     auto put_in_list = [&](u64 token) {
         const unsigned place = atomicAdd(&s.gathered, 1u);
         if (place < LIST) s.weights[place] = token;
