@@ -559,6 +559,34 @@ def test_sample_min_p_large_vocabularies(vocab):
         assert got[r] == want or room < vocab * 2.0 ** -43, (r, SETTINGS[r], got[r], want, room)
 
 
+def test_sample_min_p_on_two_streams_at_once():
+    """Calls that share the GPU, as sizes and settings of each ask for other clusters, draw what they draw alone."""
+    from easy_gpt.cpp_b200 import kernels
+
+    calls = []
+    for seed, (rows, vocab) in enumerate([(24, 151936), (60, 32001), (3, 1000), (40, 70001)]):
+        rng, g = np.random.default_rng(seed), torch.Generator("cuda").manual_seed(seed)
+        x = torch.randn((rows, vocab), generator=g, device="cuda") * 2
+        f32 = lambda v: torch.tensor(v, dtype=torch.float32, device="cuda")  # noqa: E731
+        top_k = torch.tensor(rng.choice([0, 1, 20, 700], rows), dtype=torch.int32, device="cuda")
+        calls.append((x, f32(rng.choice([0.0, 0.7, 1.3], rows)), top_k, f32(rng.choice([1.0, 0.9], rows)), f32(rng.choice([0.0, 0.01], rows)), f32(rng.random(rows))))
+    alone = []
+    for call in calls:
+        out = torch.empty(call[0].shape[0], dtype=torch.int32, device="cuda")
+        kernels.sample_min_p(*call, out)
+        alone.append(out)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        outs = [torch.full_like(out, -1) for out in alone]
+        torch.cuda.synchronize()
+        for call, out, stream in zip(calls, outs, streams):
+            with torch.cuda.stream(stream):
+                kernels.sample_min_p(*call, out)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, outs))
+
+
 def test_sample_min_p_agrees_with_sample():
     """Without min-p the rule is ``sample``'s."""
     from easy_gpt.cpp_b200 import kernels
