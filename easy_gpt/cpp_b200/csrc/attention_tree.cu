@@ -411,7 +411,8 @@ int launch_any(cudaStream_t stream, const Params& p, long long tiles) {
 
 // How a step's work is laid out, from sizes alone: plan[0] the rows of a CTA (128: the tcgen05 kernel; 16, 32 or 64: the warp-level one;
 // 0: the 32-bit one), plan[1] and plan[2] the max_parts and part_tiles of eg_attention_tree.  aligned: the caches, their pages and heads start on
-// 16-byte boundaries, and q, out and their rows on 16-byte (2) or 4-byte (1) ones.  max_context: the most keys of an entry, as far as known.
+// 16-byte boundaries, and q, out and their rows on 16-byte (2) or 4-byte (1) ones; of float32 not 0 where rows of q and the caches are whole 16-byte
+// pieces.  max_context: the most keys of an entry, as far as known.
 //
 // A key tile of 64 takes a CTA 1 us on the tcgen05 kernel whatever its rows, and 1 us (16 rows of 64) to 2.6 us (64 rows of 128) on the warp-level one,
 // whose start and end are 2 us shorter: that one takes short contexts of few units where both would do (a chain of 8 at 500 keys 7.6 us against 9.4;

@@ -947,7 +947,8 @@ def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
 
 def attention_tree_plan(dtype: int, aligned: int, rows: int, entries: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_context: int):
     """(rows of a CTA: 128 the tcgen05 kernel, 16 to 64 the warp-level one, 0 the 32-bit one; the most parts a row tile's keys are cut into; the fewest
-    times 64 keys of a part) that ``attention_tree`` goes by; aligned: 2 rows of q and out on 16-byte boundaries, 1 on 4-byte ones, 0 neither."""
+    times 64 keys of a part) that ``attention_tree`` goes by; aligned: 2 rows of q and out on 16-byte boundaries, 1 on 4-byte ones, 0 neither;
+    of float32 whether rows of q and the caches are whole 16-byte pieces."""
     plan = (c_int * 3)()
     _need(library().eg_attention_tree_plan(dtype, aligned, rows, entries, num_heads, num_kv_heads, head_dim, page_size, max_context, sm_count(), plan) == 0, "sizes of a step")
     return tuple(plan)

@@ -1,4 +1,5 @@
 """What the operators of a step over drafted trees refuse before anything is launched (no GPU): by their Python faces, and by the launchers alone."""
+import ctypes
 import math
 
 import pytest
@@ -115,3 +116,16 @@ def test_plans():
         for nodes in (1, 9, 64, 300):
             parts = [plan(kernels.BF16, aligned, nodes * entries, entries, 28, 4, 128, 64, 4000)[1] for entries in (1, 4, 16, 64, 256)]
             assert parts == sorted(parts, reverse=True) and all(p in (1, 2, 4, 8, 16) for p in parts) and parts[-1] == 1, parts
+
+
+def test_plans_of_float32():
+    """Rows in whole 16-byte pieces go in CTAs of 32, two an SM, in up to 16 parts where the keys are many; others, and heads of more than 128, in 8 at most."""
+    def parts(aligned, *sizes):
+        plan = (ctypes.c_int * 3)()
+        assert kernels.library().eg_attention_tree_plan(kernels.F32, aligned, *sizes, 148, plan) == 0 and plan[0] == 0
+        return plan[1]
+
+    assert [parts(2, 1, 1, 12, 12, 128, 16, keys) for keys in (100, 1000, 4000)] == [2, 8, 16]
+    assert [parts(0, 1, 1, 12, 12, 128, 16, keys) for keys in (100, 1000, 4000)] == [2, 8, 8]
+    assert parts(2, 1, 1, 12, 12, 256, 16, 4000) == 8
+    assert [parts(2, 13 * n, n, 12, 2, 128, 16, 1000) for n in (4, 16, 64)] == [8, 2, 1]

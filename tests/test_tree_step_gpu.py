@@ -152,6 +152,19 @@ def test_attention_tree_every_kernel(heads, window, row_tile, parts, part_tiles)
     assert float(((got[:total] - want[:total]).norm(dim=1) / want[:total].norm(dim=1)).max()) <= tolerance(step.dtype, step.dim)
 
 
+@pytest.mark.parametrize("parts, part_tiles", [(1, 1), (2, 3), (4, 1), (8, 1), (16, 1)])
+@pytest.mark.parametrize("heads, window", [((14, 2, 64), None), ((14, 2, 64), 50), ((12, 2, 128), None), ((16, 1, 128), 200), ((5, 5, 32), 90), ((6, 2, 30), None), ((8, 1, 256), 33), ((4, 2, 200), None)])
+def test_attention_tree_float32_cuts(heads, window, parts, part_tiles):
+    """The 32-bit kernel on float32: CTAs of 32 rows and of 64, whole 16-byte pieces (all but heads of 30) and not, every number of parts."""
+    if parts == 16 and heads[2] > 128:
+        pytest.skip("no room for clusters of 16")
+    step = Step([*heads, parts], [1, 4, 5, 0, 18, 37, 70], [0, 1000, 31, 7, 640, 1, 333], *heads, 32, torch.float32)
+    got, want = run_plan(step, (0, parts, part_tiles), window).double(), step.plain(window)
+    total = sum(step.nodes)
+    assert int(step.status) == 0 and torch.equal(got[total:], want[total:])
+    assert float(((got[:total] - want[:total]).norm(dim=1) / want[:total].norm(dim=1)).max()) <= tolerance(step.dtype, step.dim)
+
+
 @pytest.mark.parametrize("parts", [1, 4])
 @pytest.mark.parametrize("row_tile", [0, 16, 32, 64, 128])
 @pytest.mark.parametrize("heads", [(14, 2, 64), (12, 2, 128)])
