@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
         unsigned char* const vs = const_cast<unsigned char*>(ks) + L::TILE_BYTES;
         const int key0 = tile * KEYS;
         const bool masked = key0 + KEYS > e.context || key0 < max(first, latest) || checked;
+        bool odd = false;                                            // values that are not finite, in a tile with masks: the same for all threads
         if (masked) {
             if (tid < ROWS) {
                 unsigned long long bits = 0;
@@ -190,34 +191,12 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
                 }
                 seen[tid] = bits;
             }
-            // values that are not finite: they are added where they are seen, and zeros take part in the product
             unsigned largest = 0;
 #pragma unroll 4
             for (int i = tid; i < KEYS * L::CHUNKS; i += THREADS) largest = tree::largest_halves(largest, *reinterpret_cast<const uint4*>(vs + i * 16));
-            if (__syncthreads_or(tree::not_finite(largest))) {
-                for (int key = wk * KW; key < (wk + 1) * KW; ++key) {
-                    const bool a = seen[wr * 16 + gid] >> key & 1, b = seen[wr * 16 + gid + 8] >> key & 1;
-#pragma unroll
-                    for (int j = 0; j < HD / 8; ++j) {
-                        const bf16* const at = reinterpret_cast<const bf16*>(vs + L::offset(key, j)) + 2 * tig;
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const float v = __bfloat162float(at[x]);
-                            if (isfinite(v)) continue;
-                            if (a) acc[j][x] += v;
-                            if (b) acc[j][2 + x] += v;
-                        }
-                    }
-                }
-                __syncthreads();
-                for (int i = tid; i < KEYS * HD; i += THREADS) {
-                    bf16* const at = reinterpret_cast<bf16*>(vs) + i;
-                    if (!isfinite(__bfloat162float(*at))) *at = __float2bfloat16_rn(0.f);
-                }
-                __syncthreads();
-            }
+            odd = __syncthreads_or(tree::not_finite(largest));
         }
-        if (idle) continue;
+        if (idle && !odd) continue;
 
         // ---- scores
         float s[2 * KB][4];
@@ -263,8 +242,7 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
         t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
         const float n0 = fmaxf(m0, t0 * scale_log2), n1 = fmaxf(m1, t1 * scale_log2);
         const float r0 = n0 == -INFINITY ? 0.f : n0, r1 = n1 == -INFINITY ? 0.f : n1;
-        // (before the first score there is nothing to scale, but for infinities and NaN of this tile, which 0 would not leave as they are)
-        const float c0 = m0 == -INFINITY ? 1.f : exp2_fast(m0 - r0), c1 = m1 == -INFINITY ? 1.f : exp2_fast(m1 - r1);
+        const float c0 = exp2_fast(m0 - r0), c1 = exp2_fast(m1 - r1);
         m0 = n0;
         m1 = n1;
         l0 *= c0;
@@ -293,6 +271,29 @@ __global__ void __launch_bounds__(THREADS) attention_tree_mma_kernel(const Param
             acc[j][1] *= c0;
             acc[j][2] *= c1;
             acc[j][3] *= c1;
+        }
+        // ---- values that are not finite: they are added where they are seen (behind the scaling, whose factor may be 0), and zeros take part in the product
+        if (odd) {
+            for (int key = wk * KW; key < (wk + 1) * KW; ++key) {
+                const bool a = seen[wr * 16 + gid] >> key & 1, b = seen[wr * 16 + gid + 8] >> key & 1;
+#pragma unroll
+                for (int j = 0; j < HD / 8; ++j) {
+                    const bf16* const at = reinterpret_cast<const bf16*>(vs + L::offset(key, j)) + 2 * tig;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float v = __bfloat162float(at[x]);
+                        if (isfinite(v)) continue;
+                        if (a) acc[j][x] += v;
+                        if (b) acc[j][2 + x] += v;
+                    }
+                }
+            }
+            __syncthreads();
+            for (int i = tid; i < KEYS * HD; i += THREADS) {
+                bf16* const at = reinterpret_cast<bf16*>(vs) + i;
+                if (!isfinite(__bfloat162float(*at))) *at = __float2bfloat16_rn(0.f);
+            }
+            __syncthreads();
         }
         // ---- output
 #pragma unroll
