@@ -63,7 +63,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t q_addr = base, k_ring = base + S::Q_BYTES, v_ring = k_ring + STAGES * S::TILE_BYTES;
     unsigned char* const aligned = smem_raw + (base - smem_addr(smem_raw));
-    pdl_enter();
+    pdl_wait();
     const int group = p.num_heads / p.num_kv_heads;
     int r, within;
     Entry e;
@@ -121,6 +121,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_start_next();                                                // not before this CTA has its tensor memory
     const uint32_t tmem = tmem_slot;
 
     // a row's result, its columns c0 .. c0 + 31

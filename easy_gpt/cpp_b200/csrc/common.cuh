@@ -93,9 +93,13 @@ struct TraceScope {
 // everything before it, since that kernel waited too), then lets the kernel behind it start, whose weights (gemm_stream.cu)
 // are then on their way while this one works.  (Measured on B200, us a decode step of 8 requests: Zodosun 435 -> 400, Lasizen
 // 496 -> 463; a step of eight prompts of 250 tokens at the 0.5B sizes 2,690 -> 2,456.)
+// (A kernel with tensor memory lets the one behind it start when it has its columns: CTAs that took the last of them in front of their own wait would wait
+// for this kernel, and it for the columns.)
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+__device__ __forceinline__ void pdl_start_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::); }
 __device__ __forceinline__ void pdl_enter() {
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;\n" ::);
+    pdl_wait();
+    pdl_start_next();
 }
 // asks the L2 for n float32 weights that a block reads once its input is there: for the time in front of pdl_enter()
 __device__ __forceinline__ void prefetch_weights(const float* p, int n) {

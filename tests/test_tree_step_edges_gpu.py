@@ -1,6 +1,7 @@
 """Attention over drafted trees where its kernels could differ from one another or from the formula."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -28,3 +29,38 @@ def test_the_likeliest_value_may_be_infinite(heads, row_tile, parts, bad):
     assert bool((got[:58, :, :8] == bad).all())
     got, want = got[:58, :, 8:].double().flatten(1), want[:58, :, 8:].flatten(1)
     assert float(((got - want).norm(dim=1) / want.norm(dim=1)).max()) <= tolerance(torch.bfloat16, heads[2])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_products_right_behind_it(dim):
+    """The attention on tcgen05 and products that allocate tensor memory in front of their wait for it, in turn on one stream: the rows and sums that each
+    gives alone, bit for bit."""
+    from test_gemm_batch_gpu import RESID, library
+
+    lib, rng, stream = library(), np.random.default_rng(dim), torch.cuda.current_stream().cuda_stream
+    M, N, K = 64, 896, 896
+    f32 = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda()  # noqa: E731
+    W, x, resid, gain = f32(N, K).bfloat16(), f32(M, K).bfloat16(), f32(M, N) * 30, f32(N)
+    parts = lib.eg_gemm_batch_takes(RESID, N, K, 0)
+    step = Step(dim, [24] * 16, [2000] * 16, 14, 2, dim, 64)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def product(r, xn, ss, mode):
+        assert lib.eg_gemm_batch(stream, RESID, mode, W.data_ptr(), K, None, M, N, K, x.data_ptr(), K, 1e-6, None, 0, None, 0, 0, 0, 0, None, None, None, None, 1, 0, 0, 0, r.data_ptr(),
+                                 gain.data_ptr(), xn.data_ptr(), ss.data_ptr(), None, 0, status.data_ptr()) == 0
+
+    new = lambda: (resid.clone(), torch.empty(M, N, device="cuda", dtype=torch.bfloat16), torch.empty(M, parts, device="cuda"))  # noqa: E731
+    alone, rows = new(), run_plan(step, (128, 4, 1)).clone()
+    torch.cuda.synchronize()
+    for _ in range(12):
+        product(*alone, 0)
+        torch.cuda.synchronize()
+    for mode in (1, 2):
+        together = new()
+        step.out.fill_(7.0)
+        for _ in range(12):
+            run_plan(step, (128, 4, 1))
+            product(*together, mode)
+        torch.cuda.synchronize()
+        assert int(status) == 0 and int(step.status) == 0 and torch.equal(step.out, rows)
+        assert all(torch.equal(a, b) for a, b in zip(alone, together))
