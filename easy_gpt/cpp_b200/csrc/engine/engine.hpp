@@ -108,6 +108,8 @@ public:
         for (int64_t t : prompt)
             if (t < 0 || t >= model->spec.vocab_size)
                 throw std::invalid_argument("token id " + std::to_string(t) + " is outside the vocabulary of " + std::to_string(model->spec.vocab_size));
+        if (params.min_p > 0.0f && !params.is_greedy() && model->lm_head->vocab() > eg_sample_min_p_most_tokens())
+            throw std::invalid_argument("Min-p needs a vocabulary of at most " + std::to_string(eg_sample_min_p_most_tokens()) + " tokens");
         RequestRecord r;
         r.id = scheduler->add((long long)prompt.size(), max_new_tokens);
         r.prompt = prompt;

@@ -234,6 +234,8 @@ int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* args);
 int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count, int* plan);
 // sampling_min_p.cu
 int eg_sample_min_p(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* out);
+// sampling_min_p.cu
+int eg_sample_min_p_most_tokens(void);
 // tree_step.cu
 int eg_tree_accept(cudaStream_t stream, const eg_tree_accept_args* args);
 // tree_step.cu

@@ -751,6 +751,9 @@ int launch(cudaStream_t stream, int ctas, int slice, const float* logits, long l
 
 }  // namespace
 
+// the largest vocabulary that eg_sample_min_p takes
+EG_API int eg_sample_min_p_most_tokens(void) { return MOST_TOKENS; }
+
 // logits [rows, vocab] with row stride ld; temperature, top_k, top_p, min_p, uniform, out: [rows].
 EG_API int eg_sample_min_p(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p,
                            const float* min_p, const float* uniform, int* out) {

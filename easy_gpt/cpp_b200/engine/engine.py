@@ -14,7 +14,7 @@ import time
 
 import torch
 
-from .. import log
+from .. import kernels, log
 from ..sampling.params import SamplingParams
 from ..sampling.sampler import Sampler
 from .model import Model
@@ -63,6 +63,8 @@ class GptEngine:
         for t in prompt:
             if not 0 <= int(t) < vocab:
                 raise ValueError(f"token id {t} is outside the vocabulary of {vocab}")
+        if params.min_p > 0.0 and not params.is_greedy and vocab > kernels.SAMPLE_MAX_VOCAB:
+            raise ValueError(f"Min-p needs a vocabulary of at most {kernels.SAMPLE_MAX_VOCAB} tokens")
         request = self.scheduler.add(prompt, params, max_new_tokens)
         if log.enabled("info"):
             self._added_at[request.id] = time.perf_counter()
