@@ -95,9 +95,9 @@ public:
         if (so.max_batch_tokens <= 0 || so.chunk_size <= 0 || so.max_active <= 0 || so.prefill_batch <= 0) throw std::invalid_argument("scheduler limits must be positive");
         scheduler.reset(new host::SchedulerCore(&runner->cache.core, so));
         const size_t rows = (size_t)std::max(opt.max_active, 1);
-        sample_params_dev_.allocate(5 * rows * 4);
+        sample_params_dev_.allocate(6 * rows * 4);
         sample_out_dev_.allocate(rows * 4);
-        sample_params_host_.ensure(5 * rows * 4);
+        sample_params_host_.ensure(6 * rows * 4);
         sample_out_host_.ensure(rows * 4);
         max_rows_ = rows;
     }
@@ -217,7 +217,8 @@ public:
 private:
     static double now() { return std::chrono::duration<double>(std::chrono::steady_clock::now().time_since_epoch()).count(); }
 
-    // one kernel launch for the whole batch, greedy rows and sampled rows together; the tokens come back to the host
+    // One kernel launch for the whole batch, greedy rows and sampled rows together; rows with min-p go through a kernel of their own, so that a request's
+    // tokens do not hang on what it shares its batch with: two launches where both are there.  The tokens come back to the host.
     std::vector<long long> sample(const float* logits, const std::vector<const host::ScheduledEntry*>& sampling) {
         const size_t rows = sampling.size();
         if (rows > max_rows_) throw StepError("more sampling rows than live requests");
@@ -246,19 +247,16 @@ private:
                 ((int*)h)[3 * max_rows_ + r] = p.top_k;
                 h[4 * max_rows_ + r] = p.is_greedy() ? 0.0f : p.min_p;
             }
-            EG_CUDA(cudaMemcpyAsync(sample_params_dev_.get(), h, 5 * max_rows_ * 4, cudaMemcpyHostToDevice, stream));
-            const float* d = sample_params_dev_.as<float>();
-            // rows with min-p go through a kernel of their own, so that a request's tokens do not hang on what it shares its batch with: a launch for
-            // every run of rows of one kind
-            for (size_t start = 0, end; start < rows; start = end) {
-                const bool with_min_p = h[4 * max_rows_ + start] > 0.0f;
-                for (end = start + 1; end < rows && (h[4 * max_rows_ + end] > 0.0f) == with_min_p;) ++end;
-                const float* x = logits + start * (size_t)vocab;
-                const float *temperature = d + start, *top_p = d + max_rows_ + start, *u = d + 2 * max_rows_ + start, *min_p = d + 4 * max_rows_ + start;
-                const int* top_k = (const int*)(d + 3 * max_rows_ + start);
-                if (with_min_p) launch_check(eg_sample_min_p(stream, x, vocab, (int)(end - start), vocab, temperature, top_k, top_p, min_p, u, out + start), "sample_min_p");
-                else launch_check(eg_sample(stream, x, vocab, (int)(end - start), vocab, temperature, top_k, top_p, u, out + start), "sample");
-            }
+            // the rows without min-p, then those with it
+            int* const order = (int*)h + 5 * max_rows_;
+            int plain = 0, next = 0;
+            for (size_t r = 0; r < rows; ++r) plain += !(h[4 * max_rows_ + r] > 0.0f);
+            for (size_t r = 0, at = plain; r < rows; ++r) order[h[4 * max_rows_ + r] > 0.0f ? at++ : next++] = (int)r;
+            EG_CUDA(cudaMemcpyAsync(sample_params_dev_.get(), h, 6 * max_rows_ * 4, cudaMemcpyHostToDevice, stream));
+            const float *temperature = sample_params_dev_.as<float>(), *top_p = temperature + max_rows_, *u = top_p + max_rows_, *min_p = u + 2 * max_rows_;
+            const int *top_k = (const int*)(u + max_rows_), *which = (const int*)(min_p + max_rows_), n = (int)rows;
+            if (plain) launch_check(eg_sample_rows(stream, logits, vocab, n, vocab, temperature, top_k, top_p, u, out, plain < n ? which : nullptr, plain), "sample");
+            if (plain < n) launch_check(eg_sample_min_p_rows(stream, logits, vocab, n, vocab, temperature, top_k, top_p, min_p, u, out, plain ? which + plain : nullptr, n - plain), "sample_min_p");
         }
         EG_CUDA(cudaMemcpyAsync(sample_out_host_.as<int>(), out, rows * 4, cudaMemcpyDeviceToHost, stream));
         EG_CUDA(cudaStreamSynchronize(stream));

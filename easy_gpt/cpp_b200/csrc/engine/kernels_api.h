@@ -49,6 +49,8 @@ int eg_rope_cache(cudaStream_t stream, int dtype, void* qkv, int ld, const float
 int eg_argmax(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, int* out, int blocks_per_row, float* part_val, int* part_idx, int* counters);
 // sampling.cu
 int eg_sample(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p, const float* uniform, int* out);
+// sampling.cu
+int eg_sample_rows(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p, const float* uniform, int* out, const int* which, int picked);
 // decode_fused.cu
 int eg_decode_fused_smem(int stages, int xs_bytes, int num_ops, int num_tmpls);
 // decode_fused.cu
@@ -234,6 +236,8 @@ int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* args);
 int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count, int* plan);
 // sampling_min_p.cu
 int eg_sample_min_p(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* out);
+// sampling_min_p.cu
+int eg_sample_min_p_rows(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p, const float* min_p, const float* uniform, int* out, const int* which, int picked);
 // sampling_min_p.cu
 int eg_sample_min_p_most_tokens(void);
 // tree_step.cu

@@ -193,7 +193,7 @@ __device__ __forceinline__ float block_max_float(float v, float* scratch) {
 __global__ void __launch_bounds__(SAMPLE_THREADS)
 sample_kernel(const float* __restrict__ logits, long long ld, int vocab, const float* __restrict__ temperature,
               const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ uniform,
-              int* __restrict__ out) {
+              int* __restrict__ out, const int* __restrict__ which, int rows) {
     __shared__ ArgMax arg_scratch[32];
     __shared__ float f_scratch[32];
     __shared__ int i_scratch[32];
@@ -201,7 +201,8 @@ sample_kernel(const float* __restrict__ logits, long long ld, int vocab, const f
     __shared__ int seg_eq[SAMPLE_THREADS];
     __shared__ int chosen;
 
-    const int r = blockIdx.x;
+    const int r = which ? which[blockIdx.x] : blockIdx.x;
+    if (r < 0 || r >= rows) return;                              // no row of the batch
     const float* row = logits + (size_t)r * ld;
     const float T = temperature[r];
     const int tid = threadIdx.x;
@@ -372,9 +373,15 @@ sample_kernel(const float* __restrict__ logits, long long ld, int vocab, const f
     }
 }
 
+// Of logits [rows, vocab] and one value per row of the others the rows which[0 .. picked - 1]; numbers that no row has are passed over.
+EG_API int eg_sample_rows(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature,
+                          const int* top_k, const float* top_p, const float* uniform, int* out, const int* which, int picked) {
+    if (rows <= 0 || picked <= 0) return 0;
+    sample_kernel<<<picked, SAMPLE_THREADS, 0, stream>>>(logits, ld, vocab, temperature, top_k, top_p, uniform, out, which, rows);
+    return eg_launch_status();
+}
+
 EG_API int eg_sample(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature,
                      const int* top_k, const float* top_p, const float* uniform, int* out) {
-    if (rows <= 0) return 0;
-    sample_kernel<<<rows, SAMPLE_THREADS, 0, stream>>>(logits, ld, vocab, temperature, top_k, top_p, uniform, out);
-    return eg_launch_status();
+    return eg_sample_rows(stream, logits, ld, rows, vocab, temperature, top_k, top_p, uniform, out, nullptr, rows);
 }

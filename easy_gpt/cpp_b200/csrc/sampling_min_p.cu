@@ -177,13 +177,13 @@ __device__ __forceinline__ int power_of_two(int n) { return n <= 2 ? 2 : 1 << (3
 template <bool RESIDENT>
 __global__ void __launch_bounds__(THREADS, 2)
 sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, int slice, const float* __restrict__ temperature, const int* __restrict__ top_k,
-                    const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniform, int* __restrict__ out) {
+                    const float* __restrict__ top_p, const float* __restrict__ min_p, const float* __restrict__ uniform, int* __restrict__ out,
+                    const int* __restrict__ which, int rows) {
     extern __shared__ __align__(16) float slice_s[];
     __shared__ Shared s;
     const unsigned rank = cluster_rank(), ctas = cluster_size();
-    const int r = blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int lo = min(vocab, (int)rank * slice), n = min(vocab, lo + slice) - lo;      // this CTA's tokens: lo .. lo + n - 1
-    const float* const row = logits + (size_t)r * ld + lo;
     static_assert(BINS == THREADS, "a thread a step");
     auto clear_bins = [&]() { s.bin_count[tid] = s.bin_weight[0][tid] = s.bin_weight[1][tid] = s.bin_weight[2][tid] = 0; };
     clear_bins();
@@ -191,6 +191,12 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     if (tid < POWERS) s.power[tid] = exp2((double)tid / POWERS);
     asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");      // the others may write here once they know that this CTA runs
     pdl_enter();
+    const int r = which ? which[blockIdx.x / ctas] : (int)(blockIdx.x / ctas);
+    if (r < 0 || r >= rows) {                                        // no row of the batch: the whole cluster leaves
+        asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+        return;
+    }
+    const float* const row = logits + (size_t)r * ld + lo;
     const float T = temperature[r], p = top_p[r], u = uniform[r];
     const int k = top_k[r];
     const double least = (double)fminf(min_p[r], 1.f) * ONE;         // NaN: 1, which only the largest pass
@@ -721,7 +727,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
 
 template <bool RESIDENT>
 int launch(cudaStream_t stream, int ctas, int slice, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p,
-           const float* min_p, const float* uniform, int* out) {
+           const float* min_p, const float* uniform, int* out, const int* which, int picked) {
     const int bytes = RESIDENT ? slice * 4 : 0;
     const auto kernel = sample_min_p_kernel<RESIDENT>;
     static unsigned long long seen = 0;
@@ -733,7 +739,7 @@ int launch(cudaStream_t stream, int ctas, int slice, const float* logits, long l
         eg_done_on_device(seen, device);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)rows * ctas));
+    cfg.gridDim = dim3((unsigned)((long long)picked * ctas));
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = stream;
@@ -745,7 +751,7 @@ int launch(cudaStream_t stream, int ctas, int slice, const float* logits, long l
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    (void)cudaLaunchKernelEx(&cfg, kernel, logits, ld, vocab, slice, temperature, top_k, top_p, min_p, uniform, out);
+    (void)cudaLaunchKernelEx(&cfg, kernel, logits, ld, vocab, slice, temperature, top_k, top_p, min_p, uniform, out, which, rows);
     return eg_launch_status();
 }
 
@@ -754,15 +760,21 @@ int launch(cudaStream_t stream, int ctas, int slice, const float* logits, long l
 // the largest vocabulary that eg_sample_min_p takes
 EG_API int eg_sample_min_p_most_tokens(void) { return MOST_TOKENS; }
 
-// logits [rows, vocab] with row stride ld; temperature, top_k, top_p, min_p, uniform, out: [rows].
-EG_API int eg_sample_min_p(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p,
-                           const float* min_p, const float* uniform, int* out) {
-    if (rows <= 0) return 0;
-    if (vocab < 1 || vocab > MOST_TOKENS || rows > 0x7fffffff / MOST_CTAS) return (int)cudaErrorInvalidValue;
+// logits [rows, vocab] with row stride ld; temperature, top_k, top_p, min_p, uniform, out: [rows].  Of these the rows which[0 .. picked - 1]; numbers that no
+// row has are passed over.
+EG_API int eg_sample_min_p_rows(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p,
+                                const float* min_p, const float* uniform, int* out, const int* which, int picked) {
+    if (rows <= 0 || picked <= 0) return 0;
+    if (vocab < 1 || vocab > MOST_TOKENS || picked > 0x7fffffff / MOST_CTAS) return (int)cudaErrorInvalidValue;
     // as many CTAs a row as its slices need, and for few rows more
     int ctas = 1;
-    while (ctas < MOST_CTAS && ((long long)vocab > (long long)ctas * SLICE || (rows * ctas < 64 && vocab > ctas * 8192))) ctas *= 2;
+    while (ctas < MOST_CTAS && ((long long)vocab > (long long)ctas * SLICE || (picked * ctas < 64 && vocab > ctas * 8192))) ctas *= 2;
     const int slice = ((vocab + ctas - 1) / ctas + 3) & ~3;
-    if (slice <= MOST_SLICE) return launch<true>(stream, ctas, slice, logits, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out);
-    return launch<false>(stream, ctas, slice, logits, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out);
+    const auto launch_it = slice <= MOST_SLICE ? launch<true> : launch<false>;
+    return launch_it(stream, ctas, slice, logits, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out, which, picked);
+}
+
+EG_API int eg_sample_min_p(cudaStream_t stream, const float* logits, long long ld, int rows, int vocab, const float* temperature, const int* top_k, const float* top_p,
+                           const float* min_p, const float* uniform, int* out) {
+    return eg_sample_min_p_rows(stream, logits, ld, rows, vocab, temperature, top_k, top_p, min_p, uniform, out, nullptr, rows);
 }

@@ -99,7 +99,9 @@ class _Signatures:
     eg_argmax = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p]
     eg_wait_probe = [c_void_p, ctypes.c_uint, c_int, c_void_p, c_void_p]
     eg_sample = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    eg_sample_rows = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int]
     eg_sample_min_p = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    eg_sample_min_p_rows = [c_void_p, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int]
     eg_attention_tree = [c_void_p, ctypes.c_char_p]
     eg_attention_tree_plan = [c_int] * 10 + [c_void_p]
     eg_tree_accept = [c_void_p, ctypes.c_char_p]
@@ -905,17 +907,20 @@ def argmax(logits: torch.Tensor, out: torch.Tensor) -> None:
 
 
 def sample(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor,
-           uniform: torch.Tensor, out: torch.Tensor) -> None:
+           uniform: torch.Tensor, out: torch.Tensor, which: Optional[torch.Tensor] = None) -> None:
     """Per row: temperature <= 0 -> greedy; else softmax(logits / T) cut by top_k
-    (0 = off) and top_p (1 = off), drawn by inverse CDF in index order with uniform[r]."""
-    _cuda(logits, temperature, top_k, top_p, uniform, out)
+    (0 = off) and top_p (1 = off), drawn by inverse CDF in index order with uniform[r].
+    ``which``: numbers of rows, in any order; only those are sampled, the others' places in out are left (a number that no row has
+    is passed over)."""
+    _cuda(logits, temperature, top_k, top_p, uniform, out, which)
     rows = logits.shape[0]
+    _need(which is None or (which.dim() == 1 and which.dtype == torch.int32 and which.is_contiguous()), "int32 numbers of rows, contiguous")
     _need(logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1, "float32 rows")
     _need(temperature.dtype == top_p.dtype == uniform.dtype == torch.float32 and top_k.dtype == torch.int32
           and out.dtype == torch.int32, "float32 temperature/top_p/uniform, int32 top_k/out")
     _need(min(temperature.numel(), top_k.numel(), top_p.numel(), uniform.numel(), out.numel()) >= rows, "one value per row")
-    _check(library().eg_sample(_stream(), _ptr(logits), logits.stride(0), rows, logits.shape[1], _ptr(temperature),
-                               _ptr(top_k), _ptr(top_p), _ptr(uniform), _ptr(out)), "sample")
+    _check(library().eg_sample_rows(_stream(), _ptr(logits), logits.stride(0), rows, logits.shape[1], _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                    _ptr(uniform), _ptr(out), _ptr(which), rows if which is None else which.numel()), "sample")
 
 
 SAMPLE_MAX_VOCAB = 1 << 20
@@ -923,15 +928,15 @@ _F32, _I32 = torch.float32, torch.int32
 
 
 def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
-                 uniform: torch.Tensor, out: torch.Tensor) -> None:
+                 uniform: torch.Tensor, out: torch.Tensor, which: Optional[torch.Tensor] = None) -> None:
     """``sample`` with a further cut, and with its sums in 64 bits: per row temperature <= 0 -> greedy; else softmax(logits / T)
     cut by top_k (0 = off), then top_p (1 = off), then to the tokens with at least min_p times the largest one's probability
     (0 = off), drawn by inverse CDF in index order with uniform[r].  Ties go to the lower index; NaN is never kept; tokens of less
-    than 2^-43 of the largest one's probability are never drawn; a row without a number above -inf gives 0."""
-    device = _device_of(logits, temperature, top_k, top_p, min_p, uniform, out)
+    than 2^-43 of the largest one's probability are never drawn; a row without a number above -inf gives 0.  ``which`` as in ``sample``."""
+    device = _device_of(logits, temperature, top_k, top_p, min_p, uniform, out, *(() if which is None else (which,)))
     if device != _current_device():
         with torch.cuda.device(device):
-            return sample_min_p(logits, temperature, top_k, top_p, min_p, uniform, out)
+            return sample_min_p(logits, temperature, top_k, top_p, min_p, uniform, out, which)
     if logits.dim() != 2 or logits.dtype is not _F32:
         raise KernelError("float32 rows")
     (rows, vocab), (ld, step) = logits.shape, logits.stride()
@@ -941,8 +946,11 @@ def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
             and temperature.is_contiguous() and top_k.is_contiguous() and top_p.is_contiguous() and min_p.is_contiguous() and uniform.is_contiguous()
             and out.is_contiguous() and min(temperature.numel(), top_k.numel(), top_p.numel(), min_p.numel(), uniform.numel(), out.numel()) >= rows):
         raise KernelError("float32 temperature/top_p/min_p/uniform, int32 top_k/out, one value per row, contiguous")
-    _check(library().eg_sample_min_p(_stream_of(device), logits.data_ptr(), ld, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
-                                     min_p.data_ptr(), uniform.data_ptr(), out.data_ptr()), "sample_min_p")
+    if which is not None and not (which.dtype is _I32 and which.dim() == 1 and which.is_contiguous()):
+        raise KernelError("int32 numbers of rows, contiguous")
+    _check(library().eg_sample_min_p_rows(_stream_of(device), logits.data_ptr(), ld, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+                                          min_p.data_ptr(), uniform.data_ptr(), out.data_ptr(), None if which is None else which.data_ptr(),
+                                          rows if which is None else which.numel()), "sample_min_p")
 
 
 def attention_tree_plan(dtype: int, aligned: int, rows: int, entries: int, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int, max_context: int):

@@ -1,7 +1,7 @@
 """Sampling of next tokens from float32 logits on the device: one kernel launch
 for the whole batch, greedy rows and sampled rows together (rows with min-p go
 through a kernel of their own, so that a request's tokens do not hang on what it
-shares its batch with: a launch for every run of rows of one kind)."""
+shares its batch with: two launches where both are there)."""
 from __future__ import annotations
 
 from typing import Sequence
@@ -24,13 +24,13 @@ class Sampler:
         if rows <= self._cap:
             return
         self._cap = max(rows, 2 * self._cap)
-        # pinned float32 blocks [5, cap]: temperature, top_p, uniform, top_k (as int bits), min_p.  Several in turn, each
+        # pinned float32 blocks [6, cap]: temperature, top_p, uniform, top_k (as int bits), min_p, rows by kind (as int bits).  Several in turn, each
         # with the event of the copy that last read it: the host runs ahead of the device, and a block written
         # again before its copy has run would hand that step the next step's numbers.
-        self._hosts = [torch.empty((5, self._cap), dtype=torch.float32).pin_memory() for _ in range(4)]
+        self._hosts = [torch.empty((6, self._cap), dtype=torch.float32).pin_memory() for _ in range(4)]
         self._host_events = [None] * len(self._hosts)
         self._host_turn = 0
-        self._dev = torch.empty((5, self._cap), dtype=torch.float32, device=self.device)
+        self._dev = torch.empty((6, self._cap), dtype=torch.float32, device=self.device)
         # two output buffers in turn: a step's tokens stay readable (they feed the next step on the
         # device, and their copy to the host is read late) while the next step's are being written
         self._outs = [torch.empty(self._cap, dtype=torch.int32, device=self.device) for _ in range(2)]
@@ -63,22 +63,20 @@ class Sampler:
             h[2, r] = 0.0 if p.is_greedy else uniform(p.seed, int(request_ids[r]), int(token_indices[r]))
             h[4, r] = p.min_p
         h[3, :rows].view(np.int32)[:] = [p.top_k for p in params]
+        # the rows without min-p, then those with it
+        plain = [r for r, p in enumerate(params) if p.is_greedy or not p.min_p > 0.0]
+        with_min_p = [r for r, p in enumerate(params) if p.min_p > 0.0 and not p.is_greedy]
+        h[5, :rows].view(np.int32)[:] = plain + with_min_p
         self._dev[:, :rows].copy_(host[:, :rows], non_blocking=True)
         if self._host_events[i] is None:
             self._host_events[i] = torch.cuda.Event()
         self._host_events[i].record()
-        with_min_p = [p.min_p > 0.0 and not p.is_greedy for p in params]
-        start = 0
-        while start < rows:
-            end = start + 1
-            while end < rows and with_min_p[end] == with_min_p[start]:
-                end += 1
-            temperature, top_p, u, top_k, min_p = self._dev[:, start:end]
-            if with_min_p[start]:
-                kernels.sample_min_p(logits[start:end], temperature, top_k.view(torch.int32), top_p, min_p, u, self._out[start:end])
-            else:
-                kernels.sample(logits[start:end], temperature, top_k.view(torch.int32), top_p, u, self._out[start:end])
-            start = end
+        temperature, top_p, u, top_k, min_p, which = self._dev
+        top_k, which = top_k.view(torch.int32), which.view(torch.int32)[:rows]
+        if plain:
+            kernels.sample(logits, temperature, top_k, top_p, u, self._out, which[:len(plain)] if with_min_p else None)
+        if with_min_p:
+            kernels.sample_min_p(logits, temperature, top_k, top_p, min_p, u, self._out, which[len(plain):] if plain else None)
         return self._out[:rows]
 
     def to_host_async(self, tokens: torch.Tensor):
