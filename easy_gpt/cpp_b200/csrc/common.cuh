@@ -105,9 +105,13 @@ __device__ __forceinline__ void pdl_enter() {
 __device__ __forceinline__ void prefetch_weights(const float* p, int n) {
     for (int i = threadIdx.x * 32; i < n; i += blockDim.x * 32) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(p + i));
 }
+// EASY_GPT_PDL=0, for measurements: no kernel is launched as one
+static inline bool eg_pdl_on() {
+    static const bool on = !(getenv("EASY_GPT_PDL") && atoi(getenv("EASY_GPT_PDL")) == 0);
+    return on;
+}
 template <class... P, class... A>
 static inline void eg_pdl_launch_if(bool early, void (*kernel)(P...), dim3 grid, dim3 block, size_t shared_bytes, cudaStream_t stream, A... args) {
-    static const bool on = !(getenv("EASY_GPT_PDL") && atoi(getenv("EASY_GPT_PDL")) == 0);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -117,7 +121,7 @@ static inline void eg_pdl_launch_if(bool early, void (*kernel)(P...), dim3 grid,
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = on && early ? 1 : 0;
+    cfg.numAttrs = early && eg_pdl_on() ? 1 : 0;
     (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);       // its error is the launch status
 }
 template <class... P, class... A>

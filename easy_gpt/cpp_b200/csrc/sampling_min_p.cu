@@ -750,7 +750,7 @@ int launch(cudaStream_t stream, int ctas, int slice, const float* logits, long l
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = eg_pdl_on() ? 2 : 1;
     (void)cudaLaunchKernelEx(&cfg, kernel, logits, ld, vocab, slice, temperature, top_k, top_p, min_p, uniform, out, which, rows);
     return eg_launch_status();
 }
