@@ -9,8 +9,8 @@
 // without a number above -inf gives 0.
 //
 // Each of the three cuts keeps a run from the top of the row's descending order.  A token's decision hangs on sums over a whole vocabulary,
-// and a uniform number may lie next to a token's border; so weights are taken in 64 bits and summed as whole numbers of 2^-42, whose sums
-// are the same in every order (shared-memory atomics among them).  Tokens below half of that have no weight.
+// and a uniform number may lie next to a token's border; so weights are taken in 64 bits (off by at most 2^-46 of themselves) and summed as whole numbers
+// of 2^-42 (rounded, by 2^-43 at most), whose sums are the same in every order (shared-memory atomics among them).  Tokens below half of that have no weight.
 //
 // A row is a cluster's, up to 16 CTAs with a slice of it each in shared memory, so that it is read once however often it is passed over.
 // What most rows come to is a short list: the k largest, or what min-p or top-p leave.  The tokens that can be among those, at most 1,024, go to the
@@ -295,8 +295,10 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         if (rank == 0 && tid == 0) out[r] = index_of(all[0]);
         return;
     }
-    // exp(t) for t in -31 .. 0 as 2^(n / 16) exp(z) with n the whole number next to 16 t / ln 2 and |z| <= ln 2 / 32, where the powers up to
-    // z^5 / 120 leave 2e-13; n = 16 e + i, a table has 2^(i / 16), and adding e + 42 to its exponent scales it to whole 2^-42.  Adding 1.5 2^52 and
+    // exp(t) for t in -31 .. 0 as 2^(n / 16) exp(z) with n the whole number next to 16 t / ln 2 and |z| <= a = ln 2 / 32.  The powers up to z^5 / 120 leave
+    // z^6 / 720, up to 1.4e-13 and always above; of it 3 a^2 z^4 / 2 - 9 a^4 z^2 / 16, which differs from z^6 by at most a^6 / 16 (by the Chebyshev polynomial of
+    // that degree, whose constant is left out), goes into the coefficients of z^4 and z^2: 9e-15 are left, 2^-46, beside the 2^-43 of rounding to whole 2^-42.
+    // n = 16 e + i, a table has 2^(i / 16), and adding e + 42 to its exponent scales it to whole 2^-42.  Adding 1.5 2^52 and
     // taking it off rounds to a whole number, which then stands in the low bits.  No branches, so that several tokens' chains overlap.  (192 rows of
     // 151,936, nothing cut: with exp() 194 us, with 64 powers 130, so 111.)
     const double per_step = POWERS / 0.69314718055994530942 / (double)T, step_size = 0.69314718055994530942 / POWERS;
@@ -309,7 +311,8 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         const double z = (y - (shifted - WHOLE)) * step_size;
         const double power = s.power[whole & (POWERS - 1)];
         const double scaled = __hiloint2double(__double2hiint(power) + ((whole >> 4) + 42 << 20), __double2loint(power));
-        const double series = fma(fma(fma(fma(z, 1.0 / 120, 1.0 / 24), z, 1.0 / 6), z, 0.5), z * z, z);
+        constexpr double A2 = 0.69314718055994530942 / 32 * (0.69314718055994530942 / 32), FOURTH = 1.0 / 24 + A2 / 480, SECOND = 0.5 - A2 * A2 / 1280;
+        const double series = fma(fma(fma(fma(z, 1.0 / 120, FOURTH), z, 1.0 / 6), z, SECOND), z * z, z);
         const double w = fma(scaled, series, scaled) + WHOLE;        // exp(z) = 1 + series
         const u64 found = (u64)__double_as_longlong(w) & 0x7ffffffffffffull;
         const bool some = x > -INFINITY && largest - x <= no_weight; // (a NaN has none)

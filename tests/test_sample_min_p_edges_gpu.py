@@ -2,11 +2,36 @@
 import os
 import subprocess
 import sys
+from decimal import Decimal, getcontext
 from pathlib import Path
 
+import numpy as np
 import pytest
+import torch
+
+from test_tree_step_gpu import run_sample
 
 ROOT = Path(__file__).resolve().parent.parent
+
+# (logit, ones, others): exp(logit) lies above ones / others by 1.14 to 1.47 times 2^-43
+BORDERS = [("-0x1.bee89ep-4", 492187, 548928), ("-0x1.5e909cp-6", 112589, 115024), ("-0x1.1fdca4p-2", 254872, 337605), ("-0x1.e9a53cp-3", 373766, 474715), ("-0x1.4bf1a6p-2", 345056, 477169),
+           ("-0x1.910474p-3", 401512, 488357), ("-0x1.0c29a2p-4", 297768, 317915)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("logit, ones, others", BORDERS)
+def test_weights_are_off_by_hardly_more_than_half_a_unit(logit, ones, others):
+    """`ones` tokens of weight 1, which is exact, then `others` of weight w = exp(logit), drawn with 1/2: the last of the ones if ones >= others * w, else the
+    first of the others.  Whole numbers of 2^-42 round w by at most 2^-43, and the exponential is off by at most 2^-46 w (a series to z^5, with the sixth
+    power spread over the second and fourth; 64-bit roundings beside it): 1.125 times 2^-43, less than what is between w and the border."""
+    getcontext().prec = 50
+    x = float.fromhex(logit)
+    assert float(np.float32(x)) == x and ones + others <= 1 << 20
+    above = (Decimal(x).exp() - Decimal(ones) / Decimal(others)) * 2 ** 43
+    assert Decimal("1.14") < above < Decimal("1.5")
+    row = torch.cat([torch.zeros(ones), torch.full((others,), x)])[None].cuda()
+    assert run_sample(row, np.float32(1), 0, np.float32(1), np.float32(0), np.float32(0.5)).tolist() == [ones]
+
 
 EDGES = """
 import ctypes
