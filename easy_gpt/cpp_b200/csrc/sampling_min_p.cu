@@ -5,8 +5,8 @@
 //   top-p    of those in descending order the shortest run from the top whose weights reach p of all of theirs, one at least, if 0 < p < 1
 //   min-p    of those the ones with w_i >= min_p (the largest has w = 1), if min_p > 0; min_p above 1 counts as 1
 // and of what is kept the first token in the order of the indices whose running sum of weights passes u times their sum.  T <= 0 (or NaN):
-// the largest, the lower index on a tie.  NaN is never kept, -inf has no weight; with +inf among the logits only those have one.  A row
-// without a number above -inf gives 0.
+// the largest, the lower index on a tie.  u below 0 or NaN is 0, and with 1 or more the last token that is kept is drawn.  NaN is never kept, -inf
+// has no weight; with +inf among the logits only those have one.  A row without a number above -inf gives 0.
 //
 // Each of the three cuts keeps a run from the top of the row's descending order.  A token's decision hangs on sums over a whole vocabulary,
 // and a uniform number may lie next to a token's border; so weights are taken in 64 bits (off by at most 2^-46 of themselves) and summed as whole numbers
@@ -335,11 +335,12 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
         if (tid == 0) s.gathered = 0;
         cluster_barrier();
     };
-    // The first token whose running sum passes u times the whole: at least 1, and at most the whole itself.
+    // The first token whose running sum passes u times the whole: at least 1, and at most the whole itself (u from 1 on, where the product may
+    // be beyond 64 bits).
     auto goal_of = [&](u64 total) -> u64 {
         const double asked = (double)u * (double)total;
-        const u64 passed = asked > 0 ? (u64)asked + 1 : 1;
-        return passed < total ? passed : total;
+        if (!(asked > 0)) return 1;                                  // (NaN too)
+        return asked < (double)total ? min((u64)asked + 1, total) : total;
     };
     // The list's cuts and the draw.  by_k: top-k is still to be cut, and top-p goes by what that leaves; else by `whole`.
     auto draw_from_list = [&](int listed, bool by_k, u64 whole) {

@@ -931,8 +931,9 @@ def sample_min_p(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.T
                  uniform: torch.Tensor, out: torch.Tensor, which: Optional[torch.Tensor] = None) -> None:
     """``sample`` with a further cut, and with its sums in 64 bits: per row temperature <= 0 -> greedy; else softmax(logits / T)
     cut by top_k (0 = off), then top_p (1 = off), then to the tokens with at least min_p times the largest one's probability
-    (0 = off), drawn by inverse CDF in index order with uniform[r].  Ties go to the lower index; NaN is never kept; tokens of less
-    than 2^-43 of the largest one's probability are never drawn; a row without a number above -inf gives 0.  ``which`` as in ``sample``."""
+    (0 = off), drawn by inverse CDF in index order with uniform[r] (below 0 or NaN: the first token that is kept, 1 or more: the last).
+    Ties go to the lower index; NaN is never kept; tokens of less than 2^-43 of the largest one's probability are never drawn; a row
+    without a number above -inf gives 0.  ``which`` as in ``sample``."""
     device = _device_of(logits, temperature, top_k, top_p, min_p, uniform, out, *(() if which is None else (which,)))
     if device != _current_device():
         with torch.cuda.device(device):

@@ -1,4 +1,5 @@
 """Sampling with min-p, and the kernels of drafted trees, at the edges."""
+import math
 import os
 import subprocess
 import sys
@@ -31,6 +32,22 @@ def test_weights_are_off_by_hardly_more_than_half_a_unit(logit, ones, others):
     assert Decimal("1.14") < above < Decimal("1.5")
     row = torch.cat([torch.zeros(ones), torch.full((others,), x)])[None].cuda()
     assert run_sample(row, np.float32(1), 0, np.float32(1), np.float32(0), np.float32(0.5)).tolist() == [ones]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab, k, p, low", [(300, 20, 1.0, 0.0), (9000, 20, 0.9, 0.0), (9000, 400, 1.0, 0.0), (9000, 0, 1.0, 0.0), (151936, 0, 1.0, 0.0), (151936, 0, 0.5, 0.0), (151936, 0, 1.0, 0.1)])
+def test_numbers_outside_of_zero_to_one(vocab, k, p, low):
+    """What is below 0 or none draws the first token that is kept, 1 and more the last one."""
+    x = np.random.default_rng(vocab + k).normal(0, 1, vocab).astype(np.float32)
+    w = np.exp((x.astype(np.float64) - x.max()))
+    order = np.argsort(-x, kind="stable")[:k if k else vocab]
+    run = np.cumsum(w[order])
+    kept = order[:1 + int((run[:-1] < float(np.float32(p)) * run[-1]).sum())] if p < 1 else order
+    kept = kept[w[kept] >= low]
+    numbers = [-math.inf, -1.0, 0.0, math.nan, 1.0, 2.0, 1e6, 1e7, 1e30, math.inf]
+    logits = torch.from_numpy(np.broadcast_to(x, (len(numbers), vocab)).copy()).cuda()
+    got = run_sample(logits, np.float32(1), k, np.float32(p), np.float32(low), np.array(numbers, np.float32)).tolist()
+    assert got == [int(kept.min())] * 4 + [int(kept.max())] * 6
 
 
 EDGES = """
