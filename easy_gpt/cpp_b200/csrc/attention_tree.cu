@@ -455,7 +455,7 @@ EG_API int eg_attention_tree(cudaStream_t stream, const eg_attention_tree_args* 
     if ((a.dtype != EG_F32 && a.dtype != EG_BF16) || a.num_kv_heads < 1 || a.num_heads < 1 || a.num_heads > INT || a.num_heads % a.num_kv_heads || a.num_kv_heads > 65535 ||
         a.head_dim < 1 || a.head_dim > 256 || a.page_size < 1 || a.page_size > INT || a.num_pages < 1 || a.num_pages > INT || a.table_pages < 0 || a.table_pages > INT ||
         a.table_stride < 0 || a.table_stride > INT || a.entries > 65535 || a.rows > INT || a.rows * a.num_heads > INT || a.window < 0 || a.window > INT ||
-        !(a.scale > 0.0) || !(a.scale < 3e38) || !a.status)
+        !((float)a.scale > 0.f) || !(a.scale < 2e38) || !a.status)      // (a scale of 0 in 32 bits, or of infinity with the exponents' base in it, makes NaN of hidden scores)
         return (int)cudaErrorInvalidValue;
     const int dim = (int)a.head_dim, group = (int)(a.num_heads / a.num_kv_heads);
     // what the tensor-core kernels ask of addresses and strides

@@ -18,7 +18,7 @@ typedef struct eg_attention_tree_args {
     long long window;               /* 0: none */
     long long max_context;          /* the most keys an entry has, cached and its own, as far as known: how the work is split follows it */
     long long row_tile, max_parts, part_tiles;      /* a plan (eg_attention_tree_plan); row_tile below 0: made by the call */
-    double scale;                   /* above 0 */
+    double scale;                   /* above 0 in 32 bits, below 2e38 */
 } eg_attention_tree_args;
 
 /* eg_tree_accept (tree_step.cu) */

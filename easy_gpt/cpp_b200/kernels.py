@@ -976,7 +976,7 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     and values were stored at cache position context[r] + i (and rotated at position context[r] + depth).  A node sees the cached keys, its
     ancestors and itself; with a window, those of them whose position is above its own minus the window.  Caches [pages, NKV, page_size,
     HD], block_table [entries, pages of a request], all int32 but q, out and the caches (float32 or bfloat16); at most 65,535 entries.  scale
-    is above 0.
+    is above 0 in 32 bits (1e-45) and below 2e38.
     ``max_context``: the most keys an entry has, cached and its own, as far as the caller knows (how the work is split follows it; by
     default what the block table has room for).  Bits of ``status``: 16 rows or a parent that cannot be (such rows are left, such a node
     has no parent), 2 a page that is none (its keys are not seen), 8 a bounded wait inside the kernel gave up."""
@@ -1006,8 +1006,8 @@ def attention_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if (table_step != 1 and table_pages > 1) or entry_starts.numel() != entries + 1 or context.numel() < entries or not entry_starts.is_contiguous() \
             or not context.is_contiguous() or not parents.is_contiguous() or status.numel() < 1:
         raise KernelError("block table rows, entry_starts [entries + 1], context [entries], parents [T], all contiguous")
-    if (window is not None and window <= 0) or not 0 < scale < math.inf:
-        raise KernelError("a window of one key at least, a scale above 0")
+    if (window is not None and window <= 0) or not 1e-45 <= scale < 2e38:
+        raise KernelError("a window of one key at least, a scale above 0 in 32 bits and below 2e38")
     page_size = cache_shape[2]
     _check(library().eg_attention_tree(_stream_of(device), _pack_attention_tree(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), entry_starts.data_ptr(), context.data_ptr(), parents.data_ptr(), out.data_ptr(),
