@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_tree_step_gpu import Step, run_plan, tolerance
+from test_tree_step_gpu import Step, line_of, run_plan, tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -29,6 +29,25 @@ def test_the_likeliest_value_may_be_infinite(heads, row_tile, parts, bad):
     assert bool((got[:58, :, :8] == bad).all())
     got, want = got[:58, :, 8:].double().flatten(1), want[:58, :, 8:].flatten(1)
     assert float(((got - want).norm(dim=1) / want.norm(dim=1)).max()) <= tolerance(torch.bfloat16, heads[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (4, 2, 32), (3, 1, 80)])
+def test_keys_beyond_the_block_table_are_not_seen(heads, dtype):
+    """A table of 48 places: an entry of 46 keys has all of them, one of 60 (its nodes behind the 50th among them) those that there are places for."""
+    step = Step(4, [6, 10], [40, 50], *heads, 16, dtype)
+    step.block_table = step.block_table[:, :3].contiguous()
+    got, at, group = step.run().double(), 0, heads[0] // heads[1]
+    assert int(step.status) == 2
+    for r, (n, c) in enumerate(zip(step.nodes, step.contexts)):
+        k, v = step.rows_of(r, 0), step.rows_of(r, 1)
+        for i in range(n):
+            seen = [x for x in [*range(c), *(c + a for a in line_of(step.parents[r], i))] if x < 48]
+            q = step.q[at + i].double().view(heads[1], group, heads[2])
+            w = (torch.einsum("ghd,gkd->ghk", q, k[:, seen]) * heads[2] ** -0.5).softmax(-1)
+            want = torch.einsum("ghk,gkd->ghd", w, v[:, seen]).reshape(-1)
+            assert float((got[at + i] - want).norm() / want.norm()) <= tolerance(dtype, heads[2]), (r, i)
+        at += n
 
 
 @pytest.mark.parametrize("dim", [64, 128])
