@@ -38,10 +38,14 @@ struct Params {
 struct Entry {
     int first, n, context;
 };
+// The most nodes of an entry.  A row's mask in a key tile is a walk up its ancestors, so a chain of n nodes takes time by the square of n (1,024 nodes 0.8 ms,
+// 4,096 21 ms; trees as drafts grow them, whose depth is some dozens, 0.04 and 0.3): from here on a call would take seconds, and one walk come near the
+// limit of the waits for it.
+constexpr int MOST_NODES = 1 << 14;
 // Entry r as the metadata has it; n = 0 where its rows cannot be what they say (and a status bit).
 __device__ __forceinline__ Entry sound(const Params& p, int first, int end, int context) {
     Entry e = {first, end - first, context};
-    if (first < 0 || end < first || end > p.rows || context < 0 || context > 0x7fffffff - 4096 - e.n) {      // (the kernels look a few tiles ahead)
+    if (first < 0 || end < first || end > p.rows || e.n > MOST_NODES || context < 0 || context > 0x7fffffff - 4096 - e.n) {      // (the kernels look a few tiles ahead)
         atomicOr(p.status, EG_STATUS_BAD_TREE);
         e.n = 0;
     }

@@ -83,3 +83,23 @@ def test_products_right_behind_it(dim):
         torch.cuda.synchronize()
         assert int(status) == 0 and int(step.status) == 0 and torch.equal(step.out, rows)
         assert all(torch.equal(a, b) for a, b in zip(alone, together))
+
+
+@pytest.mark.parametrize("row_tile", [0, 16, 128])
+def test_the_most_nodes_of_an_entry(row_tile):
+    """16,384 nodes: right, in the first rows and the last.  One more: a status, and that entry's rows are left; the other's are as ever."""
+    step = Step(77, [16384, 5], [20, 40], 1, 1, 64, 64)
+    got = run_plan(step, (row_tile, 1, 1)).double()
+    assert int(step.status) == 0
+    k, v = step.rows_of(0, 0)[0], step.rows_of(0, 1)[0]
+    for i in (0, 1, 63, 64, 1000, 8191, 16320, 16383):
+        seen = [*range(20), *(20 + a for a in line_of(step.parents[0], i))]
+        want = ((k[seen] @ step.q[i].double()) * 0.125).softmax(0) @ v[seen]
+        assert float((got[i] - want).norm() / want.norm()) <= tolerance(torch.bfloat16, 64), i
+    other = got[16384:16389].clone()
+    step.starts[1] += 1                                               # 16,385 and 4
+    step.out.fill_(7.0)
+    got = run_plan(step, (row_tile, 1, 1)).double()
+    assert int(step.status) == 16 and bool((got[:16385] == 7).all()) and not bool((got[16385:16389] == 7).all(dim=1).any())
+    step.starts[1] -= 1
+    assert torch.equal(run_plan(step, (row_tile, 1, 1))[16384:16389].double(), other)
