@@ -415,12 +415,13 @@ int launch_any(cudaStream_t stream, const Params& p, long long tiles) {
 // pieces.  max_context: the most keys of an entry, as far as known.
 //
 // A key tile of 64 takes a CTA 1 us on the tcgen05 kernel whatever its rows, and 1 us (16 rows of 64) to 2.6 us (64 rows of 128) on the warp-level one,
-// whose start and end are 2 us shorter: that one takes short contexts of few units where both would do (a chain of 8 at 500 keys 7.6 us against 9.4;
+// whose start and end are 2 us shorter: that one takes short contexts of few units where both would do (a chain of 8 at 500 keys 7.2 us against 9.0;
 // 64 requests of 16 nodes at 700 keys 46 against 21).  Parts: as many as keep one CTA an SM with three key tiles a part, or two CTAs with eight;
-// more of them cost more than they save (32 requests of 9 nodes at 1,000 keys in 1, 2, 4 and 8 parts 18.7, 16.2, 14.6 and 23.8 us; 64 requests of 16 at 700
+// more of them cost more than they save (32 requests of 9 nodes at 1,000 keys in 1, 2, 4 and 8 parts 18.5, 15.9, 13.9 and 24.8 us; 64 requests of 16 at 700
 // in 1, 2 and 4 parts 21, 25 and 36), and clusters of 16 find little room.  Long contexts are cut into four in any case, for an even end (16 requests of up
-// to 32,768 keys, wide trees, in 1, 2, 4 and 8 parts 556, 375, 360 and 412).  The 32-bit kernel's CTAs of 32 rows go two to an SM from the first (4
-// requests of 13 nodes at 1,000 keys, 12 heads on 2, in 4, 8 and 16 parts 31, 24 and 33; one node at 4,000, 12 on 12, in 8 and 16 46 and 29).
+// to 32,768 keys, wide trees, in 1, 2, 4 and 8 parts 598, 409, 386 and 465: medians of 40 calls of each in turn, four fifths of them within 4%, at 1.7 GHz under the
+// power limit).  The 32-bit kernel's CTAs of 32 rows go two to an SM from the first (4
+// requests of 13 nodes at 1,000 keys, 12 heads on 2, in 4, 8 and 16 parts 29, 24.5 and 28.5; one node at 4,000, 12 on 12, in 8 and 16 47 and 30).
 EG_API int eg_attention_tree_plan(int dtype, int aligned, int rows, int entries, int num_heads, int num_kv_heads, int head_dim, int page_size, int max_context, int sm_count,
                                   int* plan) {
     if (rows < 1 || entries < 1 || num_kv_heads < 1 || num_heads % num_kv_heads || num_heads < 1 || page_size < 1 || sm_count < 1 || !plan) return (int)cudaErrorInvalidValue;

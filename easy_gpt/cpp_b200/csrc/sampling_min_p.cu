@@ -21,9 +21,10 @@
 //
 // (A histogram's weights are three sums of 14 bits each: shared-memory atomics on 64 bits are loops of compare-and-swap, 5 to 18 times slower.)
 //
-// Measured, one row and 192 rows of 151,936 (0.6 MB and 117 MB), us: greedy 5.1 and 50, top-k 20 7.3 and 64, min-p 0.05 7.2 and 63, nothing cut 9.6 and 112,
-// top-p 0.95 alone over flat logits 28 and 310.  One row is bound by latency: the load 1.6, an exchange over the cluster 1 each.  Many rows are 296 CTAs at a
-// time, 8 us each when greedy, of which the load is half; flat rows are bound by weights in 64 bits (0.65 cycles a token and SM a pass) and histograms.
+// Measured, one row and 192 rows of 151,936 (0.6 MB and 117 MB) with logits of a spread of 1 to 4, us: greedy 4.8 and 49, top-k 20 7.1 and 64, min-p 0.05 10.8 and 92,
+// nothing cut 9.5 and 112, top-p 0.95 alone 28 and 328, at a temperature of 3 31 and 355.  One row is bound by latency: the load 1.6, an exchange over the cluster 1
+// each.  Many rows are 296 CTAs at a time, 8 us each when greedy, of which the load is half; flat rows are bound by weights in 64 bits (0.65 cycles a token
+// and SM a pass) and histograms.
 #include "common.cuh"
 
 namespace {
@@ -302,7 +303,7 @@ sample_min_p_kernel(const float* __restrict__ logits, long long ld, int vocab, i
     // that degree, whose constant is left out), goes into the coefficients of z^4 and z^2: 9e-15 are left, 2^-46, beside the 2^-43 of rounding to whole 2^-42.
     // n = 16 e + i, a table has 2^(i / 16), and adding e + 42 to its exponent scales it to whole 2^-42.  Adding 1.5 2^52 and
     // taking it off rounds to a whole number, which then stands in the low bits.  No branches, so that several tokens' chains overlap.  (192 rows of
-    // 151,936, nothing cut: with exp() 194 us, with 64 powers 130, so 111.)
+    // 151,936, nothing cut: with exp() 194 us, with 64 powers 130, so 112.)
     const double per_step = POWERS / 0.69314718055994530942 / (double)T, step_size = 0.69314718055994530942 / POWERS;
     const double top_value = (double)largest;
     const float no_weight = largest < INFINITY ? NO_WEIGHT * T : -1.f;      // with +inf the largest, +inf alone has a weight
